@@ -210,6 +210,61 @@ size_t ncn_bwd_workspace_bytes(int64_t B, int64_t N, int64_t E, int n_cache, int
  * with NCN_TAPE in flags, each 2 x [B, N, E] fp32. */
 size_t ncn_ckpt_bytes(int64_t B, int64_t N, int64_t E, int L, int ckpt_every, int flags);
 
+/* ---- Attention next to the NCN layers.  No counterpart in the reference. ----
+ *
+ * Tensors: q and results [B, Nq, E], k and v [B, Nk, Ek]; head h holds the features h * d .. h * d + d - 1, d = E / n_head; keys and
+ * values have Ek / d heads, each shared by n_head * d / Ek consecutive heads of the queries.  Inputs may be views: `strides` (a host
+ * array, or null for contiguous tensors) gives {row, position} strides in elements of q, k, v (and of dy in the backward); the
+ * features of a position are next to each other.  Results are contiguous.  d up to 256 (attention), 512 (rotation).  bf16 with d a
+ * multiple of 8 up to 128, tensors on 16-byte boundaries and strides that are multiples of 8 runs on the tensor cores, the rest on the FMA pipes.
+ *
+ * Windowed attention.  Query i of row b is at position p = start_b + i, key j at position j, ctx_b = clamp(ctxlen[b], 0, Nk):
+ *   query i sees key j  where  j < ctx_b,  j <= p < ctx_b  and  (p - j < window or j < n_sink)
+ *   y = softmax over the visible keys of (scale q . k), times v
+ * A query that sees nothing (padding behind ctx_b, a position below zero) gives zeros and no gradient; what k, v, q and dy hold in such
+ * places is not used, NaN included.  (Keys that one query sees and a neighbour does not may share a tile: a NaN or infinity in such a
+ * key's v reaches, in the forward and backward, queries up to 256 positions from those that see it.)  ctxlen (int32 [B] on the device) null: Nk.
+ * q_start (int32 [B] on the device) null: start for every row.  window >= 1, n_sink >= 0, scale > 0. */
+
+/* Forward.  lse: null, or ncn_window_lse_bytes(...) bytes that ncn_window_bwd takes (opaque). */
+size_t ncn_window_lse_bytes(int64_t B, int64_t Nq, int n_head);
+int ncn_window_fwd(const void* q, const void* k, const void* v, void* y, float* lse, const int* ctxlen, const int* q_start,
+                   const int64_t* strides, int64_t B, int64_t Nq, int64_t Nk, int64_t E, int64_t Ek, int n_head, int64_t window,
+                   int64_t n_sink, int64_t start, double scale, int dtype, void* stream);
+
+/* Backward: dq, dk, dv (contiguous, every element written; with B = 0 or Nq = 0 nothing is).  workspace: 16-byte aligned.  The sums run in a fixed order:
+ * bitwise reproducible for equal arguments on one device. */
+size_t ncn_window_bwd_workspace_bytes(int64_t B, int64_t Nq, int64_t Nk, int64_t E, int64_t Ek, int n_head, int64_t window, int64_t n_sink,
+                                      int dtype);
+int ncn_window_bwd(const void* q, const void* k, const void* v, const void* y, const void* dy, const float* lse, void* dq, void* dk, void* dv,
+                   const int* ctxlen, const int* q_start, const int64_t* strides, void* workspace, size_t workspace_bytes, int64_t B,
+                   int64_t Nq, int64_t Nk, int64_t E, int64_t Ek, int n_head, int64_t window, int64_t n_sink, int64_t start, double scale,
+                   int dtype, void* stream);
+
+/* The queries are the last Nq positions of each row, start_b = ctx_b - Nq (one new token: Nq = 1), k and v caches of S positions.  For few
+ * queries: bound by reading the visible keys and values, the others are not read.  ctxlen must not be null.
+ * A cache that keeps only the sinks and a ring of the last `window` positions is read with window >= S and ctxlen = the places in use. */
+int ncn_window_decode(const void* q, const void* k, const void* v, void* y, const int* ctxlen, const int64_t* strides, int64_t B, int64_t Nq,
+                      int64_t S, int64_t E, int64_t Ek, int n_head, int64_t window, int64_t n_sink, double scale, int dtype, void* stream);
+
+/* Rotary positions, and with wq and wk (fp32 [d], one weight for all heads) the norm of every head in the same pass:
+ *   u = x w / sqrt(mean(x^2) + eps)  (or x);  pair i of the first R features of u is turned by position * freqs[i] and multiplied by
+ *   `magnitude`; the other features of u pass.  Pair i: features i and i + R / 2, or 2 i and 2 i + 1 if interleaved.
+ * freqs: double [R / 2] on the device, radians per position; angles are formed in 64 bits.  positions: int64 on the device,
+ * [N] with positions_stride 0 or [B, N] with the stride of its rows, or null: start, start + 1, ...  k may be absent (null, Ek = 0).
+ * inverse: turned the other way, which is the backward of a rotation without norm. */
+int ncn_qk_rotary(const void* q, const void* k, const float* wq, const float* wk, const double* freqs, const int64_t* positions,
+                  int64_t positions_stride, int64_t start, void* yq, void* yk, const int64_t* strides, int64_t B, int64_t N, int64_t E,
+                  int64_t Ek, int n_head, int64_t R, int interleaved, double eps, double magnitude, int inverse, int dtype, void* stream);
+
+/* Backward of ncn_qk_rotary with norms.  strides: of q, k, dyq, dyk.  dwq, dwk: fp32 [d], summed over rows, positions and heads in a
+ * fixed order. */
+size_t ncn_qk_norm_rotary_workspace_bytes(int64_t B, int64_t N, int64_t E, int n_head);
+int ncn_qk_norm_rotary_bwd(const void* q, const void* k, const float* wq, const float* wk, const double* freqs, const int64_t* positions,
+                           int64_t positions_stride, int64_t start, const void* dyq, const void* dyk, void* dq, void* dk, float* dwq,
+                           float* dwk, const int64_t* strides, void* workspace, size_t workspace_bytes, int64_t B, int64_t N, int64_t E,
+                           int64_t Ek, int n_head, int64_t R, int interleaved, double eps, double magnitude, int dtype, void* stream);
+
 /* Reads and clears the device status word (synchronises the device): NCN_OK, or
  * NCN_ERR_DEVICE_WAIT if a kernel abandoned a bounded wait since the last call. */
 int ncn_device_status(void);

@@ -5,6 +5,15 @@ this package is the host side: the reference's autograd Functions and nn.Modules
 re-implemented over that ABI.  There is no CPU fallback.
 """
 from . import ops
+from .attention import (
+    RotaryFunction,
+    WindowAttentionFunction,
+    fused_qk_norm_rotary,
+    fused_rotary,
+    fused_window_attention,
+    rotary_frequencies,
+    window_attention_decode,
+)
 from .ncn_pytorch import RefTorchNaive, group_pos_to_index_v2, ref_naive_fwd
 from .ncn_pytorch_invertible import NCNFunctionPytorch, RefInvTorchNaive
 from .ncn_pytorch_wrapper_v2 import (
@@ -26,5 +35,6 @@ __all__ = [
     "NCNNetTestCuda", "RefTorchNaive", "ref_naive_fwd", "group_pos_to_index_v2", "NCNFunctionPytorch",
     "RefInvTorchNaive", "NCNResidualStack", "allreduce_weight_grads", "shard_rows", "NCNContextFunction",
     "fused_ncn_cuda_ctxlen",
-    "set_stage_backward",
+    "set_stage_backward", "RotaryFunction", "WindowAttentionFunction", "fused_qk_norm_rotary", "fused_rotary",
+    "fused_window_attention", "rotary_frequencies", "window_attention_decode",
 ]

@@ -78,6 +78,31 @@ SIGNATURES = {
     "ncn_last_cuda_error": (c_char_p, []),
     "ncn_version": (c_int, []),
     "ncn_reload_env": (None, []),
+    "ncn_window_lse_bytes": (c_size_t, [c_int64] * 2 + [c_int]),
+    "ncn_window_fwd": (
+        c_int,
+        [c_void_p] * 8 + [c_int64] * 5 + [c_int] + [c_int64] * 3 + [c_double, c_int, c_void_p],
+    ),
+    "ncn_window_bwd_workspace_bytes": (c_size_t, [c_int64] * 5 + [c_int] + [c_int64] * 2 + [c_int]),
+    "ncn_window_bwd": (
+        c_int,
+        [c_void_p] * 12 + [c_void_p, c_size_t] + [c_int64] * 5 + [c_int] + [c_int64] * 3 + [c_double, c_int, c_void_p],
+    ),
+    "ncn_window_decode": (
+        c_int,
+        [c_void_p] * 6 + [c_int64] * 5 + [c_int] + [c_int64] * 2 + [c_double, c_int, c_void_p],
+    ),
+    "ncn_qk_rotary": (
+        c_int,
+        [c_void_p] * 6 + [c_int64] * 2 + [c_void_p] * 3 + [c_int64] * 4 + [c_int, c_int64, c_int]
+        + [c_double] * 2 + [c_int, c_int, c_void_p],
+    ),
+    "ncn_qk_norm_rotary_workspace_bytes": (c_size_t, [c_int64] * 3 + [c_int]),
+    "ncn_qk_norm_rotary_bwd": (
+        c_int,
+        [c_void_p] * 6 + [c_int64] * 2 + [c_void_p] * 7 + [c_void_p, c_size_t] + [c_int64] * 4 + [c_int, c_int64, c_int]
+        + [c_double] * 2 + [c_int, c_void_p],
+    ),
 }
 
 _lib = None

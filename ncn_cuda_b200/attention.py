@@ -1,0 +1,181 @@
+"""Attention next to the NCN layers: norms of queries and keys with rotary positions, a sliding window with sink tokens, and its
+form over a cache for single tokens.
+
+An NCN stage mixes fixed groups of positions by a recurrence; a local attention layer mixes what a window holds by content.
+Both take [B, N, E] activations whose features are cut into n_head heads, a context length per batch row for padded batches, and
+fp32 or bf16 storage.  Keys and values may have fewer heads than the queries (their features are a smaller multiple of the head
+size).  No counterpart in the reference.
+
+In training a layer calls fused_qk_norm_rotary (or fused_rotary) and then fused_window_attention; in serving the rotated keys go
+into a cache and window_attention_decode reads it.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib, ops
+
+SCALINGS = (None, "linear", "ntk", "yarn")
+
+
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
+                       trained_length: int = 4096, fast_turns: float = 32.0, slow_turns: float = 1.0,
+                       device=None) -> Tuple[torch.Tensor, float]:
+    """-> (frequencies, magnitude): radians per position of the rot_dim / 2 pairs, base^(-2 i / rot_dim), as a float64 tensor, and
+    what the rotated features are multiplied by.  For contexts `factor` times as long as trained_length:
+
+    "linear"  every frequency divided by factor
+    "ntk"     a larger base, so that the slowest pair is slowed down by factor and the fastest not at all
+    "yarn"    pairs that turn more than fast_turns times within trained_length keep their frequency, those below slow_turns are
+              divided by factor, a linear ramp between; magnitude 0.1 ln(factor) + 1 (the scores are sharpened by its square)
+
+    A program makes these once and keeps them."""
+    if rot_dim < 0 or rot_dim % 2:
+        raise ValueError(f"rot_dim must be even, got {rot_dim}")
+    if scaling not in SCALINGS:
+        raise ValueError(f"unknown scaling {scaling!r}: one of {SCALINGS}")
+    if not (factor >= 1.0 and base > 0 and trained_length > 0 and fast_turns > slow_turns):
+        raise ValueError("factor >= 1, base > 0, trained_length > 0 and fast_turns > slow_turns are needed")
+    i = torch.arange(0, rot_dim, 2, dtype=torch.float64)
+    magnitude = 1.0
+    if scaling == "ntk":
+        base = base * factor ** (rot_dim / max(rot_dim - 2, 1))
+    f = base ** (-i / max(rot_dim, 1))
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        turns = trained_length * f / (2 * math.pi)
+        keep = ((turns - slow_turns) / (fast_turns - slow_turns)).clamp(0, 1)
+        f = f * keep + f / factor * (1 - keep)
+        magnitude = 0.1 * math.log(factor) + 1.0
+    return f.to(device=device), magnitude
+
+
+class RotaryFunction(torch.autograd.Function):
+    """Rotation of queries and keys, with the norm of every head where weights are given.  `apply` goes to the native node of
+    csrc/attn_torch.cpp; forward and backward stand for the calls that the node declines."""
+
+    @classmethod
+    def apply(cls, *args):
+        if cls is not RotaryFunction:
+            return super().apply(*args)
+        q, k, wq, wk, freqs, positions, n_head, start, interleaved, eps, magnitude = args
+        out = _lib.native().rotary(q, k, wq, wk, freqs, positions, n_head, start, interleaved, eps, magnitude)
+        return super().apply(*args) if out is None else out
+
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, freqs, positions, n_head, start, interleaved, eps, magnitude):
+        ctx.cfg = (n_head, start, interleaved, eps, magnitude)
+        ctx.norm = wq is not None
+        ctx.save_for_backward(q if ctx.norm else None, k if ctx.norm else None, wq, wk, freqs, positions)
+        ctx.has_k = k is not None
+        return ops.qk_rotary(q, k, wq, wk, freqs, positions, *ctx.cfg)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        q, k, wq, wk, freqs, positions = ctx.saved_tensors
+        if not ctx.norm:
+            dx = ops.qk_rotary(dq, dk if ctx.has_k else None, None, None, freqs, positions, *ctx.cfg, inverse=True)
+            return (*dx, None, None, None, None, None, None, None, None, None)
+        dq, dk, dwq, dwk = ops.qk_norm_rotary_bwd(q, k, wq, wk, freqs, positions, dq, dk if ctx.has_k else None, *ctx.cfg)
+        dwq = dwq.to(wq.dtype).reshape(wq.shape)
+        dwk = None if dwk is None else dwk.to(wk.dtype).reshape(wk.shape)
+        return dq, dk, dwq, dwk, None, None, None, None, None, None, None
+
+
+def _positions(positions):
+    """-> (tensor or None, first position)"""
+    if positions is None:
+        return None, 0
+    if isinstance(positions, int):
+        return None, positions
+    return torch.as_tensor(positions), 0
+
+
+def fused_rotary(q, k, freqs, n_head, positions=None, interleaved=False, magnitude=1.0):
+    """q [B, N, E] and k [B, N, Ek] (or None) with the first 2 * len(freqs) features of every head turned by their positions; returns both.
+    freqs: from rotary_frequencies.  positions: None (0, 1, ...), the first position as an int, or whole numbers [N] or [B, N].
+    Pair i of a head: features i and i + len(freqs), or 2 i and 2 i + 1 with interleaved=True.  Differentiable in q and k."""
+    pos, start = _positions(positions)
+    return RotaryFunction.apply(q, k, None, None, freqs, pos, n_head, start, interleaved, 0.0, magnitude)
+
+
+def fused_qk_norm_rotary(q, k, wq, wk, freqs, n_head, positions=None, interleaved=False, magnitude=1.0, eps=1e-6):
+    """fused_rotary of the normalised queries and keys: every head of q is divided by its root mean square (eps under the root) and
+    multiplied by wq [E / n_head], k likewise by wk, in the pass that turns them.  freqs of length 0: norms alone.
+    Differentiable in q, k, wq and wk."""
+    if wq is None:
+        raise ValueError("fused_qk_norm_rotary needs weights; fused_rotary turns without a norm")
+    pos, start = _positions(positions)
+    return RotaryFunction.apply(q, k, wq, wk, freqs, pos, n_head, start, interleaved, eps, magnitude)
+
+
+class WindowAttentionFunction(torch.autograd.Function):
+    """Windowed attention; `apply` goes to the native node, as in RotaryFunction."""
+
+    @classmethod
+    def apply(cls, *args):
+        if cls is not WindowAttentionFunction:
+            return super().apply(*args)
+        out = _lib.native().window(*args)
+        return super().apply(*args) if out is None else out
+
+    @staticmethod
+    def forward(ctx, q, k, v, n_head, window, n_sink, scale, ctxlen, q_start, start):
+        ctx.cfg = (n_head, window, n_sink, scale, start)
+        y, lse = ops.window_fwd(q, k, v, *ctx.cfg, ctxlen=ctxlen, q_start=q_start, want_lse=True)
+        ctx.save_for_backward(q, k, v, y, lse, ctxlen, q_start)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        q, k, v, y, lse, ctxlen, q_start = ctx.saved_tensors
+        dq, dk, dv = ops.window_bwd(q, k, v, y, dy, lse, *ctx.cfg, ctxlen=ctxlen, q_start=q_start)
+        return dq, dk, dv, None, None, None, None, None, None, None
+
+
+def _window(window, n_sink, scale, q, n_head):
+    window = ops.NO_WINDOW if window is None else int(window)
+    if window < 1 or n_sink < 0:
+        raise ValueError(f"window must be at least 1 and n_sink at least 0, got {window} and {n_sink}")
+    if scale is None:
+        scale = 1.0 / math.sqrt(max(q.shape[-1] // max(n_head, 1), 1))
+    if not (math.isfinite(scale) and scale > 0):
+        raise ValueError(f"scale must be positive, got {scale}")
+    return window, float(scale)
+
+
+def fused_window_attention(q, k, v, n_head, window, n_sink=0, scale=None, ctxlen=None, q_start=None):
+    """Causal attention in which a query sees the last `window` positions up to its own, and the first n_sink.
+
+    q [B, Nq, E], k and v [B, Nk, Ek] -> [B, Nq, E].  window None: all positions before.  scale: 1 / sqrt(E / n_head) unless given.
+    ctxlen (int tensor [B], None: Nk): the keys of each row that count; queries at or behind it are padding and give zeros.
+    q_start: the position of the first query, an int or an int tensor [B]; None: Nk - Nq, so that the last query is at the last key (a
+    chunk of a prompt behind a cache; 0 where both have one length).  Differentiable in q, k and v."""
+    window, scale = _window(window, n_sink, scale, q, n_head)
+    if ctxlen is not None:
+        ctxlen = torch.as_tensor(ctxlen)
+    start = 0
+    if q_start is None:
+        start = k.shape[1] - q.shape[1]
+    elif isinstance(q_start, int):
+        start, q_start = q_start, None
+    else:
+        q_start = torch.as_tensor(q_start)
+    return WindowAttentionFunction.apply(q, k, v, n_head, window, n_sink, scale, ctxlen, q_start, start)
+
+
+def window_attention_decode(q, k_cache, v_cache, ctxlen, n_head, window, n_sink=0, scale=None):
+    """fused_window_attention of the last Nq positions of each row, for serving: q [B, Nq, E] (Nq = 1: one new token, already in the
+    cache), k_cache and v_cache [B, S, Ek], ctxlen int tensor [B] with the new tokens counted.  Reads only the visible keys.
+    No gradient.
+
+    A ring cache (sinks in the first n_sink places, position p at n_sink + (p - n_sink) % window) holds just what one new token
+    sees, in an order that does not matter: call with window=None and ctxlen = the number of places in use."""
+    window, scale = _window(window, n_sink, scale, q, n_head)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_cache, v_cache)):
+        raise RuntimeError("window_attention_decode has no gradient: use fused_window_attention, or torch.no_grad()")
+    return _lib.native().window_decode(q, k_cache, v_cache, torch.as_tensor(ctxlen), n_head, window, n_sink, scale)

@@ -1,0 +1,930 @@
+// Windowed attention on the 5th-generation tensor cores: bf16 storage, heads of up to 128 features (a multiple of 8), fp32 sums.
+//
+// All three kernels have the same parts.  One warp fetches tiles of 128 positions by TMA into a ring of slots in shared memory, one
+// warp issues the matrix instructions (tcgen05.mma, one thread), eight warps work on the scores.  Scores and sums stay in
+// tensor memory; the weights go back there in bf16, over the scores that they came from, and are the left operand of the second
+// product straight from there.  A tile is DP / 64 blocks of [128 positions][64 features], each row of 128 bytes swizzled by the
+// TMA unit; the same tile serves as an operand along its features (scores) and along its positions (second products).
+// Heads whose size is not 64 or 128 are filled up with zeros by the TMA unit.
+//
+// Rows of padding (behind ctxlen) may hold anything, NaN included: scores are masked by selection, and the rows that a second
+// product would multiply by zero weights are cleared in shared memory first.
+//
+// The backward is two kernels, one that owns queries and one that owns keys.  It computes the scores twice, 7 products for 5, and in
+// return no sum depends on the order in which CTAs finish.
+#include <cuda.h>
+
+#include "attn_tensor.h"
+#include "ncn_common.cuh"
+
+namespace ncn {
+namespace {
+
+constexpr int kT = 128;               // positions of a tile
+constexpr int kThreads = 320;         // warps 0-7 scores, 8 products, 9 TMA
+constexpr uint32_t kBlockBytes = kT * 128;
+constexpr uint64_t kWaitLimitNs = 4000000000ull;
+
+// ------------------------------------------------------------------ PTX
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t at, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(cols));
+}
+__device__ __forceinline__ void tmem_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 32 columns of the lane's row
+__device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t (&x)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]),
+        "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]),
+        "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]),
+        "=r"(x[31])
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&x)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31};" ::"r"(x[0]),
+      "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]), "r"(x[11]), "r"(x[12]),
+      "r"(x[13]), "r"(x[14]), "r"(x[15]), "r"(x[16]), "r"(x[17]), "r"(x[18]), "r"(x[19]), "r"(x[20]), "r"(x[21]), "r"(x[22]), "r"(x[23]),
+      "r"(x[24]), "r"(x[25]), "r"(x[26]), "r"(x[27]), "r"(x[28]), "r"(x[29]), "r"(x[30]), "r"(x[31]), "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_load32f(uint32_t at, float (&x)[32]) { tmem_load32(at, reinterpret_cast<uint32_t(&)[32]>(x)); }
+__device__ __forceinline__ void tmem_store32f(uint32_t at, float (&x)[32]) { tmem_store32(at, reinterpret_cast<uint32_t(&)[32]>(x)); }
+// Waits for the loads; the values are tied to it, so that nothing made of them is moved ahead of the wait.
+__device__ __forceinline__ void tmem_tie(float (&x)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+f"(x[i]), "+f"(x[i + 1]), "+f"(x[i + 2]), "+f"(x[i + 3]), "+f"(x[i + 4]), "+f"(x[i + 5]), "+f"(x[i + 6]), "+f"(x[i + 7]));
+}
+template <int N>
+__device__ __forceinline__ void tmem_loaded(float (&x)[N][32]) {
+  tmem_wait_load();
+#pragma unroll
+  for (int c = 0; c < N; ++c) tmem_tie(x[c]);
+}
+__device__ __forceinline__ void tmem_loaded(float (&x)[32]) {
+  tmem_wait_load();
+  tmem_tie(x);
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// arrives on `bar` when the products issued so far are done
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+               "l"(b), "r"(idesc), "r"((int)add)
+               : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+               "l"(b), "r"(idesc), "r"((int)add)
+               : "memory");
+}
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int c, int head, int row, int b, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+                   smem_u32(dst)),
+               "l"(map), "r"(c), "r"(head), "r"(row), "r"(b), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+
+// Operand descriptors: 128-byte swizzle, groups of 8 rows 1024 bytes apart.  Along the features ("k-major") the 16 features of an
+// instruction are 32 bytes on; along the positions ("mn-major") the 64-feature blocks are kBlockBytes apart, 16 positions 2048 on.
+__device__ __forceinline__ uint64_t desc_of(uint32_t smem, uint32_t lead) {
+  return ((smem & 0x3ffffu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+template <int N, bool MN>
+__device__ __forceinline__ constexpr uint32_t idesc_of() {  // fp32 sums, bf16 operands, 128 x N
+  return (1u << 4) | (1u << 7) | (1u << 10) | (MN ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kT >> 4) << 24);
+}
+// D[128 x 128] = A B^T over DP features; A, B tiles
+template <int DP>
+__device__ __forceinline__ void product_scores(uint32_t d, uint32_t a, uint32_t b) {
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) {
+    const uint32_t off = (k / 4) * kBlockBytes + (k % 4) * 32;
+    mma_ss(d, desc_of(a + off, 16), desc_of(b + off, 16), idesc_of<kT, false>(), k > 0);
+  }
+}
+// D[128 x DP] (+)= W V over 128 positions; W bf16 in tensor memory, positions 64 .. 127 `upper` columns on; V a tile
+template <int DP>
+__device__ __forceinline__ void product_sums(uint32_t d, uint32_t w, uint32_t upper, uint32_t v, bool add) {
+#pragma unroll
+  for (int k = 0; k < kT / 16; ++k)
+    mma_ts(d, w + (k / 4) * upper + (k % 4) * 8, desc_of(v + k * 2048, kBlockBytes), idesc_of<DP, true>(), add || k > 0);
+}
+
+// A wait that gives up: the kernel then leaves an error in the status word, and its other warps stop waiting too.
+struct Waiter {
+  volatile int* stop;
+  int* status;
+  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t begin = now_ns();
+    while (!mbar_try_wait(bar, parity)) {
+      if (*stop) return false;
+      if (now_ns() - begin > kWaitLimitNs) {
+        *stop = 1;
+        if (status) atomicExch(status, (int)DEV_WAIT_TIMEOUT);
+        return false;
+      }
+    }
+    return true;
+  }
+};
+
+// A ring of tile slots: loads 0, 1, 2, ... in order, slot i % SLOTS
+template <int SLOTS>
+struct Ring {
+  uint64_t *full, *empty;
+  uint8_t* mem;
+  uint32_t bytes;
+  __device__ __forceinline__ uint8_t* at(int i) const { return mem + (i % SLOTS) * bytes; }
+  __device__ __forceinline__ bool wait_full(const Waiter& w, int i) const { return w(full + i % SLOTS, (i / SLOTS) & 1); }
+  __device__ __forceinline__ bool wait_empty(const Waiter& w, int i) const { return i < SLOTS || w(empty + i % SLOTS, (i / SLOTS + 1) & 1); }
+  __device__ __forceinline__ void release(int i) const { mma_commit(empty + i % SLOTS); }
+};
+
+template <int DP>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, int head, int row, int b, uint64_t* bar) {
+#pragma unroll
+  for (int c = 0; c < DP / 64; ++c) tma_load(dst + c * kBlockBytes, map, c * 64, head, row, b, bar);
+}
+// Clears the rows outside [lo, hi) of a tile that has arrived; a whole warp.
+template <int DP>
+__device__ __forceinline__ void clear_rows(uint8_t* tile, int lo, int hi) {
+  const int lane = threadIdx.x % 32;
+  for (int e = lane; e < kT * DP / 8; e += 32) {
+    const int r = e % (kT * 8) / 8;
+    if (r < lo || r >= hi) *reinterpret_cast<uint4*>(tile + e / (kT * 8) * kBlockBytes + e % (kT * 8) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async();
+  __syncwarp();
+}
+
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// 32 features of a row to global memory, c0 .. c0 + 31 of d (a multiple of 8)
+__device__ __forceinline__ void store_row(__nv_bfloat16* row, const float (&x)[32], float f, int c0, int d) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 8)
+    if (c0 + e < d)
+      *reinterpret_cast<uint4*>(row + c0 + e) = make_uint4(pack(x[e] * f, x[e + 1] * f), pack(x[e + 2] * f, x[e + 3] * f),
+                                                           pack(x[e + 4] * f, x[e + 5] * f), pack(x[e + 6] * f, x[e + 7] * f));
+}
+
+struct Maps {
+  CUtensorMap q, k, v, dy;
+};
+
+// The keys of tile k0 that a query at `pos` sees, as columns: [lo, hi), and those below `sink`
+struct Columns {
+  int lo, hi, sink;
+};
+__device__ __forceinline__ Columns columns_of(const AttnParams& p, int pos, int end, int k0) {
+  Columns c;
+  const bool live = pos >= 0 && pos < end;
+  c.hi = live ? pos + 1 - k0 : 0;
+  c.lo = pos - p.window + 1 - k0;
+  c.sink = p.n_sink - k0;
+  return c;
+}
+__device__ __forceinline__ bool visible(const Columns& c, int x) { return x < c.hi && (x >= c.lo || x < c.sink); }
+
+// ------------------------------------------------------------------ forward
+// Two tiles of 128 queries per CTA, four warps each: while one's scores are exponentiated, the other's products run.  A thread owns a
+// row.  Tensor memory: scores of both (128 columns each; the weights over them), sums of both (DP each).
+// The running maximum is followed lazily: sums are rescaled only where it has grown by 2^8 since, which bf16 weights and
+// fp32 sums carry without loss.
+constexpr float kLazy = 8.f;
+
+template <int DP, int SLOTS>
+struct FwdSmem {
+  static constexpr uint32_t tile = kT * DP * 2;
+  static constexpr uint32_t bytes = (2 + SLOTS) * tile + 256;
+};
+
+template <int DP, int SLOTS>
+__global__ void __launch_bounds__(kThreads, 1) attn_tensor_fwd_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ Maps maps) {
+  constexpr uint32_t TILE = FwdSmem<DP, SLOTS>::tile;
+  extern __shared__ __align__(1024) uint8_t base[];
+  if (smem_u32(base) & 1023) {  // (the swizzle goes by the address)
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, (int)DEV_WAIT_TIMEOUT);
+    return;
+  }
+  uint8_t* const Q = base;
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(base + (2 + SLOTS) * TILE);
+  uint64_t *const q_full = bars, *const s_full = bars + 1, *const p_ready = bars + 3, *const o_full = bars + 5;
+  const Ring<SLOTS> ring{bars + 7, bars + 7 + SLOTS, base + 2 * TILE, TILE};
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 7 + 2 * SLOTS);
+  volatile int* const stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int x = 0; x < 2; ++x) mbar_init(s_full + x, 1), mbar_init(p_ready + x, kT), mbar_init(o_full + x, 1);
+    for (int i = 0; i < SLOTS; ++i) mbar_init(ring.full + i, 1), mbar_init(ring.empty + i, 1);
+    fence_mbar_init();
+    *stop = 0;
+  }
+  tmem_before();
+  __syncthreads();
+  tmem_after();
+  const uint32_t tmem = *tmem_slot;
+  wait_for_inputs();
+
+  const Block at = block_of(p.H, (p.Nq + 2 * kT - 1) / (2 * kT));
+  const int i0 = at.last_first * 2 * kT, h = at.head, b = at.b, hk = h / p.G;
+  const RowGeom g = row_geom(p, b);
+  const KeyTiles all = key_tiles<kT>(p, g, i0, i0 + 2 * kT);
+  const int n = all.count();
+  const Waiter wait{stop, p.status};
+
+  if (warp == 9) {
+    if (lane == 0 && n > 0) {
+      const int queries = i0 + kT < p.Nq ? 2 : 1;
+      mbar_expect_tx(q_full, queries * TILE);
+      for (int x = 0; x < queries; ++x) load_tile<DP>(Q + x * TILE, &maps.q, h, i0 + x * kT, b, q_full);
+      bool ok = true;
+      int i = 0;
+      for (; i < 2 * n && ok; ++i) {
+        ok = ring.wait_empty(wait, i);
+        if (!ok) break;
+        uint64_t* const bar = ring.full + i % SLOTS;
+        mbar_expect_tx(bar, TILE);
+        load_tile<DP>(ring.at(i), i % 2 ? &maps.v : &maps.k, hk, all.tile(i / 2) * kT, b, bar);
+      }
+      if (!ok) {  // what is on its way arrives before the memory is given up
+        mbar_wait_bounded(q_full, 0);
+        for (int e = i > SLOTS ? i - SLOTS : 0; e < i; ++e) mbar_wait_bounded(ring.full + e % SLOTS, (e / SLOTS) & 1);
+      }
+    }
+  } else if (warp == 8) {
+    const KeyTiles kt[2] = {key_tiles<kT>(p, g, i0, i0 + kT), key_tiles<kT>(p, g, i0 + kT, i0 + 2 * kT)};
+    const uint32_t qs = smem_u32(Q);
+    int left[2] = {kt[0].count(), kt[1].count()};
+    bool begun[2] = {false, false};
+    uint32_t phase[2] = {0, 0};
+    bool ok = n == 0 || (wait(q_full, 0) && ring.wait_full(wait, 0));
+    if (ok && n > 0 && lane == 0) {
+      const uint32_t ks = smem_u32(ring.at(0));
+      for (int x = 0; x < 2; ++x)
+        if (kt[x].needs(all.tile(0)) && left[x]) {
+          product_scores<DP>(tmem + x * kT, qs + x * TILE, ks);
+          mma_commit(s_full + x);
+        }
+      ring.release(0);
+    }
+    for (int j = 0; ok && j < n; ++j) {
+      const int t = all.tile(j), next = j + 1 < n ? all.tile(j + 1) : -1;
+      if (!(ok = ring.wait_full(wait, 2 * j + 1) && (next < 0 || ring.wait_full(wait, 2 * j + 2)))) break;
+      if (t * kT + kT > g.ctx && g.ctx < p.Nk) clear_rows<DP>(ring.at(2 * j + 1), 0, g.ctx - t * kT);
+      const uint32_t vs = smem_u32(ring.at(2 * j + 1)), ks = smem_u32(ring.at(2 * j + 2));
+      for (int x = 0; x < 2; ++x) {
+        const bool mine = left[x] > 0 && kt[x].needs(t);
+        if (mine) {
+          if (!(ok = wait(p_ready + x, phase[x]))) break;
+          phase[x] ^= 1;
+          tmem_after();
+          if (lane == 0) product_sums<DP>(tmem + 2 * kT + x * 128, tmem + x * kT, 32, vs, begun[x]);
+          begun[x] = true;
+          if (--left[x] == 0 && lane == 0) mma_commit(o_full + x);
+        }
+        if (next >= 0 && left[x] > 0 && kt[x].needs(next) && lane == 0) {
+          product_scores<DP>(tmem + x * kT, qs + x * TILE, ks);
+          mma_commit(s_full + x);
+        }
+      }
+      if (lane == 0 && ok) {
+        ring.release(2 * j + 1);
+        if (next >= 0) ring.release(2 * j + 2);
+      }
+    }
+  } else {
+    const int x = warp / 4, r = threadIdx.x % kT, qi = i0 + x * kT + r, pos = g.start + qi;
+    const int end = min(g.ctx, g.start + p.Nq);
+    const KeyTiles kt = key_tiles<kT>(p, g, i0 + x * kT, i0 + x * kT + kT);
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+    const uint32_t ts = tmem + x * kT + lanes, to = tmem + 2 * kT + x * 128 + lanes;
+    const int p_lo = g.start + i0 + x * kT, p_hi = p_lo + kT - 1;  // positions of the tile, padding included
+    const int mine = kt.count();
+    float ref = -INFINITY, l = 0.f;  // (ref in log2 units)
+    bool ok = true;
+    for (int j = 0; j < mine; ++j) {
+      if (!(ok = wait(s_full + x, j & 1))) break;
+      tmem_after();
+      const int k0 = kt.tile(j) * kT;
+      float s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_load32f(ts + 32 * c, s[c]);
+      tmem_loaded(s);
+      const bool whole = k0 + kT - 1 <= p_lo && k0 + kT <= g.ctx && (k0 > p_hi - p.window || k0 + kT <= p.n_sink);
+      if (!whole) {
+        const Columns col = columns_of(p, pos, end, k0);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!visible(col, 32 * c + e)) s[c][e] = -INFINITY;
+      }
+      float mx[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx[c] = s[c][0];
+#pragma unroll
+        for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], s[c][e]);
+      }
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+      const bool grown = top > ref + kLazy;  // (also the first score of a row: ref is -inf)
+      if (__any_sync(~0u, grown && ref != -INFINITY)) {  // the sums that the products so far have left: they are done, the scores came after them
+        const float keep = grown ? ex2(ref - top) : 1.f;
+        l *= keep;
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          float o[32];
+          tmem_load32f(to + c, o);
+          tmem_loaded(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= keep;
+          tmem_store32f(to + c, o);
+        }
+      }
+      if (grown) ref = top;
+      const float bias = ref == -INFINITY ? 0.f : ref;
+      float sum[4];
+#pragma unroll
+      for (int c = 0; c < 4; c += 2) {
+        uint32_t w[32];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          sum[c + u] = 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float a = ex2(fmaf(s[c + u][e], p.scale_log2, -bias)), bb = ex2(fmaf(s[c + u][e + 1], p.scale_log2, -bias));
+            sum[c + u] += a + bb;
+            w[16 * u + e / 2] = pack(a, bb);
+          }
+        }
+        tmem_store32(ts + 16 * c, w);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_stored();
+      tmem_before();
+      mbar_arrive(p_ready + x);
+    }
+    if (mine > 0 && ok) ok = wait(o_full + x, 0);
+    tmem_after();
+    if (ok) {
+      const bool some = mine > 0 && !(l == 0.f);
+      const float inv = some ? 1.f / l : 0.f;
+      __nv_bfloat16* const row = static_cast<__nv_bfloat16*>(p.y) + ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        float o[32];
+        if (mine > 0) {
+          tmem_load32f(to + c, o);
+          tmem_loaded(o);
+        }
+        if (!some) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (qi < p.Nq) store_row(row, o, inv, c, p.d);
+      }
+      if (p.lse && qi < p.Nq) p.lse[((long long)b * p.H + h) * p.Nqp + qi] = some ? ref + log2f(l) : INFINITY;
+    }
+    tmem_before();
+  }
+  __syncthreads();
+  if (warp == 8) {
+    tmem_after();
+    tmem_free(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------ backward of the queries
+// One tile of 128 queries per CTA.  dP = dy v^T, dS = P (dP - delta), dq = dS k.  Two threads per row, 64 keys each.  Tensor
+// memory: two buffers of scores (the next tile's are ready while this one's are worked on; dS over them), dP, dq.
+template <int DP, int SLOTS>
+struct BwdSmem {
+  static constexpr uint32_t tile = kT * DP * 2;
+  static constexpr uint32_t bytes = (2 + SLOTS) * tile + 2048 + 256;
+};
+
+template <int DP, int SLOTS>
+__global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ Maps maps) {
+  constexpr uint32_t TILE = BwdSmem<DP, SLOTS>::tile;
+  extern __shared__ __align__(1024) uint8_t base[];
+  if (smem_u32(base) & 1023) {  // (the swizzle goes by the address)
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, (int)DEV_WAIT_TIMEOUT);
+    return;
+  }
+  uint8_t *const Q = base, *const dY = base + TILE;
+  float* const halves = reinterpret_cast<float*>(base + (2 + SLOTS) * TILE);  // [2][128]
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(halves + 512);
+  uint64_t *const q_full = bars, *const s_full = bars + 1, *const dp_full = bars + 3, *const ds_ready = bars + 4, *const done = bars + 5;
+  const Ring<SLOTS> ring{bars + 6, bars + 6 + SLOTS, base + 2 * TILE, TILE};
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 6 + 2 * SLOTS);
+  volatile int* const stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1), mbar_init(s_full, 1), mbar_init(s_full + 1, 1), mbar_init(dp_full, 1), mbar_init(ds_ready, 256), mbar_init(done, 1);
+    for (int i = 0; i < SLOTS; ++i) mbar_init(ring.full + i, 1), mbar_init(ring.empty + i, 1);
+    fence_mbar_init();
+    *stop = 0;
+  }
+  tmem_before();
+  __syncthreads();
+  tmem_after();
+  const uint32_t tmem = *tmem_slot, t_dp = tmem + 256, t_dq = tmem + 384;
+  wait_for_inputs();
+
+  const Block at = block_of(p.H, (p.Nq + kT - 1) / kT);
+  const int i0 = at.last_first * kT, h = at.head, b = at.b, hk = h / p.G;
+  const RowGeom g = row_geom(p, b);
+  const KeyTiles kt = key_tiles<kT>(p, g, i0, i0 + kT);
+  const int n = kt.count();
+  const Waiter wait{stop, p.status};
+
+  if (warp == 9) {
+    if (lane == 0 && n > 0) {
+      mbar_expect_tx(q_full, 2 * TILE);
+      load_tile<DP>(Q, &maps.q, h, i0, b, q_full);
+      load_tile<DP>(dY, &maps.dy, h, i0, b, q_full);
+      bool ok = true;
+      int i = 0;
+      for (; i < 2 * n && ok; ++i) {
+        ok = ring.wait_empty(wait, i);
+        if (!ok) break;
+        uint64_t* const bar = ring.full + i % SLOTS;
+        mbar_expect_tx(bar, TILE);
+        load_tile<DP>(ring.at(i), i % 2 ? &maps.v : &maps.k, hk, kt.tile(i / 2) * kT, b, bar);
+      }
+      if (!ok) {
+        mbar_wait_bounded(q_full, 0);
+        for (int e = i > SLOTS ? i - SLOTS : 0; e < i; ++e) mbar_wait_bounded(ring.full + e % SLOTS, (e / SLOTS) & 1);
+      }
+    }
+  } else if (warp == 8) {
+    const uint32_t qs = smem_u32(Q), dys = smem_u32(dY);
+    // scores of tile j into buffer j % 2
+    auto scores = [&](int j) {
+      if (!ring.wait_full(wait, 2 * j)) return false;
+      const int k0 = kt.tile(j) * kT;
+      if (k0 + kT > g.ctx && g.ctx < p.Nk) clear_rows<DP>(ring.at(2 * j), 0, g.ctx - k0);
+      if (lane == 0) {
+        product_scores<DP>(tmem + (j & 1) * kT, qs, smem_u32(ring.at(2 * j)));
+        mma_commit(s_full + (j & 1));
+      }
+      return true;
+    };
+    auto grads = [&](int j) {
+      if (!ring.wait_full(wait, 2 * j + 1)) return false;
+      if (lane == 0) {
+        product_scores<DP>(t_dp, dys, smem_u32(ring.at(2 * j + 1)));
+        mma_commit(dp_full);
+        ring.release(2 * j + 1);
+      }
+      return true;
+    };
+    bool ok = n == 0 || (wait(q_full, 0) && scores(0) && grads(0) && (n < 2 || scores(1)));
+    for (int j = 0; ok && j < n; ++j) {
+      if (!(ok = wait(ds_ready, j & 1))) break;
+      tmem_after();
+      if (j + 1 < n && !(ok = grads(j + 1))) break;
+      if (lane == 0) {
+        product_sums<DP>(t_dq, tmem + (j & 1) * kT, 64, smem_u32(ring.at(2 * j)), j > 0);
+        ring.release(2 * j);
+      }
+      if (j + 2 < n) ok = scores(j + 2);
+    }
+    if (ok && n > 0 && lane == 0) mma_commit(done);
+  } else {
+    const int half = warp / 4, r = warp % 4 * 32 + lane, qi = i0 + r, pos = g.start + qi;
+    const int end = min(g.ctx, g.start + p.Nq);
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+    const int p_lo = g.start + i0, p_hi = p_lo + kT - 1;
+    const bool live = pos >= 0 && pos < end;
+    const long long head_row = ((long long)b * p.H + h) * p.Nqp + qi;
+    // delta: half of the features each
+    float sum = 0.f;
+    if (live) {
+      const __nv_bfloat16* y = static_cast<const __nv_bfloat16*>(p.y_in) + ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
+      const __nv_bfloat16* dy = static_cast<const __nv_bfloat16*>(p.dy) + b * p.sdy_b + qi * p.sdy_n + (long long)h * p.d;
+      for (int c = half * (DP / 2); c < min((half + 1) * (DP / 2), p.d); c += 8) {
+        const uint4 u = *reinterpret_cast<const uint4*>(y + c), w = *reinterpret_cast<const uint4*>(dy + c);
+        const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sum = fmaf(__uint_as_float(uu[e] << 16), __uint_as_float(ww[e] << 16), sum);
+          sum = fmaf(__uint_as_float(uu[e] & 0xffff0000u), __uint_as_float(ww[e] & 0xffff0000u), sum);
+        }
+      }
+    }
+    halves[half * kT + r] = sum;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const float delta = halves[r] + halves[kT + r];
+    if (half == 0 && qi < p.Nq) p.delta[head_row] = delta;
+    const float lse = live ? p.lse[head_row] : INFINITY;
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      const int k0 = kt.tile(j) * kT + half * 64;
+      const uint32_t ts = tmem + (j & 1) * kT + half * 64 + lanes;
+      if (!(ok = wait(s_full + (j & 1), (j >> 1) & 1))) break;
+      tmem_after();
+      float s[2][32];
+      tmem_load32f(ts, s[0]);
+      tmem_load32f(ts + 32, s[1]);
+      tmem_loaded(s);
+      const bool whole = k0 + 63 <= p_lo && p_hi < end && k0 + 64 <= g.ctx && (k0 > p_hi - p.window || k0 + 64 <= p.n_sink);
+      const Columns col = columns_of(p, pos, end, k0);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 32; ++e) s[c][e] = ex2(fmaf(s[c][e], p.scale_log2, -lse));
+      if (!(ok = wait(dp_full, j & 1))) break;
+      tmem_after();
+      uint32_t w[32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float dp[32];
+        tmem_load32f(t_dp + half * 64 + 32 * c + lanes, dp);
+        tmem_loaded(dp);
+        if (whole) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) dp[e] = s[c][e] * (dp[e] - delta);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) dp[e] = visible(col, 32 * c + e) ? s[c][e] * (dp[e] - delta) : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) w[16 * c + e / 2] = pack(dp[e], dp[e + 1]);
+      }
+      tmem_store32(ts, w);
+      tmem_stored();
+      tmem_before();
+      mbar_arrive(ds_ready);
+    }
+    if (n > 0 && ok) ok = wait(done, 0);
+    tmem_after();
+    if (ok) {
+      __nv_bfloat16* const row = static_cast<__nv_bfloat16*>(p.dq) + ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
+#pragma unroll 1
+      for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
+        float o[32];
+        if (n > 0) {
+          tmem_load32f(t_dq + c + lanes, o);
+          tmem_loaded(o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (qi < p.Nq) store_row(row, o, p.scale, c, p.d);
+      }
+    }
+    tmem_before();
+  }
+  __syncthreads();
+  if (warp == 8) {
+    tmem_after();
+    tmem_free(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------ backward of the keys
+// One tile of 128 keys per CTA, its group's heads and their query tiles one after the other.  Scores the other way round (keys are
+// rows): P^T and dS^T are left operands as they come.  dv = P^T dy, dk = dS^T q.  Two threads per row, 64 queries each.  Tensor
+// memory is full: scores (P over them), dP (dS over it), dv, dk; the next tile's scores wait for dv's product only, its dP for
+// dk's.
+template <int DP, int SLOTS>
+__global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ Maps maps) {
+  constexpr uint32_t TILE = BwdSmem<DP, SLOTS>::tile;
+  constexpr int STATS = 2;  // tiles whose lse and delta are held
+  extern __shared__ __align__(1024) uint8_t base[];
+  if (smem_u32(base) & 1023) {  // (the swizzle goes by the address)
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, (int)DEV_WAIT_TIMEOUT);
+    return;
+  }
+  uint8_t *const K = base, *const V = base + TILE;
+  float* const stats = reinterpret_cast<float*>(base + (2 + SLOTS) * TILE);  // [STATS][2][128]
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(stats + STATS * 2 * kT);
+  uint64_t *const kv_full = bars, *const s_full = bars + 1, *const dp_full = bars + 2, *const p_ready = bars + 3, *const ds_ready = bars + 4,
+           *const done = bars + 5, *const st_full = bars + 6, *const st_empty = bars + 6 + STATS;
+  const Ring<SLOTS> ring{bars + 6 + 2 * STATS, bars + 6 + 2 * STATS + SLOTS, base + 2 * TILE, TILE};
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 6 + 2 * STATS + 2 * SLOTS);
+  volatile int* const stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1), mbar_init(s_full, 1), mbar_init(dp_full, 1), mbar_init(p_ready, 256), mbar_init(ds_ready, 256), mbar_init(done, 1);
+    for (int i = 0; i < STATS; ++i) mbar_init(st_full + i, 1), mbar_init(st_empty + i, 8);
+    for (int i = 0; i < SLOTS; ++i) mbar_init(ring.full + i, 1), mbar_init(ring.empty + i, 1);
+    fence_mbar_init();
+    *stop = 0;
+  }
+  tmem_before();
+  __syncthreads();
+  tmem_after();
+  const uint32_t tmem = *tmem_slot, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
+  wait_for_inputs();
+
+  const Block at = block_of(p.Hk, (p.Nk + kT - 1) / kT + p.sink_tiles * p.chunks);
+  const int hk = at.head, b = at.b;
+  const RowGeom g = row_geom(p, b);
+  const KeyItem it = key_item<kT, kT>(p, g, at.first_last);
+  const int k0 = it.tile * kT, n = it.end - it.begin;
+  const Waiter wait{stop, p.status};
+  auto head_of = [&](int i) { return hk * p.G + (it.begin + i) / it.tiles; };
+  auto first_of = [&](int i) { return (it.first + (it.begin + i) % it.tiles) * kT; };
+
+  if (warp == 9) {
+    if (lane == 0 && n > 0) {
+      mbar_expect_tx(kv_full, 2 * TILE);
+      load_tile<DP>(K, &maps.k, hk, k0, b, kv_full);
+      load_tile<DP>(V, &maps.v, hk, k0, b, kv_full);
+      bool ok = true;
+      int i = 0, held = 0;  // tiles and stats under way
+      for (; i < 2 * n && ok; ++i) {
+        ok = ring.wait_empty(wait, i);
+        if (!ok) break;
+        const int u = i / 2, h = head_of(u), i0 = first_of(u);
+        uint64_t* const bar = ring.full + i % SLOTS;
+        mbar_expect_tx(bar, TILE);
+        load_tile<DP>(ring.at(i), i % 2 ? &maps.dy : &maps.q, h, i0, b, bar);
+        if (i % 2 == 1) {  // the stats last: their place is free only when tile u - STATS is done with
+          if (u >= STATS && !(ok = wait(st_empty + u % STATS, (u / STATS + 1) & 1))) {
+            ++i;
+            break;
+          }
+          float* const st = stats + u % STATS * 2 * kT;
+          const long long row = ((long long)b * p.H + h) * p.Nqp + i0;
+          mbar_expect_tx(st_full + u % STATS, 2 * kT * 4);
+          bulk_g2s(st, p.lse + row, kT * 4, st_full + u % STATS);
+          bulk_g2s(st + kT, p.delta + row, kT * 4, st_full + u % STATS);
+          held = u + 1;
+        }
+      }
+      if (!ok) {
+        mbar_wait_bounded(kv_full, 0);
+        for (int e = held > STATS ? held - STATS : 0; e < held; ++e) mbar_wait_bounded(st_full + e % STATS, (e / STATS) & 1);
+        for (int e = i > SLOTS ? i - SLOTS : 0; e < i; ++e) mbar_wait_bounded(ring.full + e % SLOTS, (e / SLOTS) & 1);
+      }
+    }
+  } else if (warp == 8) {
+    const uint32_t ks = smem_u32(K), vs = smem_u32(V);
+    // waits for a tile of queries (or their cotangents) and clears its rows of padding
+    auto arrived = [&](int load) {
+      if (!ring.wait_full(wait, load)) return false;
+      const int first = g.start + first_of(load / 2);
+      if (first < 0 || (first + kT > g.ctx && g.start + p.Nq > g.ctx)) clear_rows<DP>(ring.at(load), -first, g.ctx - first);
+      return true;
+    };
+    auto scores = [&](int i) {
+      if (!arrived(2 * i)) return false;
+      if (lane == 0) {
+        product_scores<DP>(tmem, ks, smem_u32(ring.at(2 * i)));
+        mma_commit(s_full);
+      }
+      return true;
+    };
+    auto grads = [&](int i) {
+      if (!arrived(2 * i + 1)) return false;
+      if (lane == 0) {
+        product_scores<DP>(t_dp, vs, smem_u32(ring.at(2 * i + 1)));
+        mma_commit(dp_full);
+      }
+      return true;
+    };
+    bool ok = n == 0 || (wait(kv_full, 0) && scores(0) && grads(0));
+    for (int i = 0; ok && i < n; ++i) {
+      if (!(ok = wait(p_ready, i & 1))) break;
+      tmem_after();
+      if (lane == 0) {
+        product_sums<DP>(t_dv, tmem, 64, smem_u32(ring.at(2 * i + 1)), i > 0);
+        ring.release(2 * i + 1);
+      }
+      if (i + 1 < n && !(ok = scores(i + 1))) break;
+      if (!(ok = wait(ds_ready, i & 1))) break;
+      tmem_after();
+      if (lane == 0) {
+        product_sums<DP>(t_dk, t_dp, 64, smem_u32(ring.at(2 * i)), i > 0);
+        ring.release(2 * i);
+      }
+      if (i + 1 < n) ok = grads(i + 1);
+    }
+    if (ok && n > 0 && lane == 0) mma_commit(done);
+  } else {
+    const int half = warp / 4, r = warp % 4 * 32 + lane, key = k0 + r;
+    const int end = min(g.ctx, g.start + p.Nq);
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16, ts = tmem + half * 64 + lanes, td = t_dp + half * 64 + lanes;
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const int first = g.start + first_of(i) + half * 64;  // position of column 0
+      const float *lse = stats + i % STATS * 2 * kT + half * 64, *delta = lse + kT;
+      if (!(ok = wait(st_full + i % STATS, (i / STATS) & 1) && wait(s_full, i & 1))) break;
+      tmem_after();
+      float s[2][32];
+      tmem_load32f(ts, s[0]);
+      tmem_load32f(ts + 32, s[1]);
+      tmem_loaded(s);
+      // queries key .. last of the columns see the key
+      const int lo = key - first, hi = min(end, key < p.n_sink ? end : key + p.window) - first;
+      const bool whole = k0 + kT - 1 <= first && first + 64 <= end && (first + 63 < k0 + p.window || k0 + kT <= p.n_sink);
+      uint32_t w[32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 ls = *reinterpret_cast<const float4*>(lse + 32 * c + e);
+          s[c][e] = ex2(fmaf(s[c][e], p.scale_log2, -ls.x));
+          s[c][e + 1] = ex2(fmaf(s[c][e + 1], p.scale_log2, -ls.y));
+          s[c][e + 2] = ex2(fmaf(s[c][e + 2], p.scale_log2, -ls.z));
+          s[c][e + 3] = ex2(fmaf(s[c][e + 3], p.scale_log2, -ls.w));
+        }
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (32 * c + e < lo || 32 * c + e >= hi) s[c][e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) w[16 * c + e / 2] = pack(s[c][e], s[c][e + 1]);
+      }
+      tmem_store32(ts, w);
+      tmem_stored();
+      tmem_before();
+      mbar_arrive(p_ready);
+      if (!(ok = wait(dp_full, i & 1))) break;
+      tmem_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float dp[32];
+        tmem_load32f(td + 32 * c, dp);
+        tmem_loaded(dp);
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 de = *reinterpret_cast<const float4*>(delta + 32 * c + e);
+          dp[e] = s[c][e] * (dp[e] - de.x);
+          dp[e + 1] = s[c][e + 1] * (dp[e + 1] - de.y);
+          dp[e + 2] = s[c][e + 2] * (dp[e + 2] - de.z);
+          dp[e + 3] = s[c][e + 3] * (dp[e + 3] - de.w);
+        }
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (32 * c + e < lo || 32 * c + e >= hi) dp[e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) w[16 * c + e / 2] = pack(dp[e], dp[e + 1]);
+      }
+      tmem_store32(td, w);
+      tmem_stored();
+      tmem_before();
+      mbar_arrive(ds_ready);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(st_empty + i % STATS);
+    }
+    if (n > 0 && ok) ok = wait(done, 0);
+    tmem_after();
+    const bool sinks = p.chunks > 0 && it.tile < p.sink_tiles, partial = sinks && key < p.n_sink;
+    if (ok) {
+      float* const part = sinks ? part_of(p, b, hk, it.tile, it.chunk < 0 ? p.chunks : it.chunk) : nullptr;
+      const long long row = ((long long)b * p.Nk + key) * p.Hk * p.d + (long long)hk * p.d;
+#pragma unroll 1
+      for (int which = 0; which < 2; ++which)
+#pragma unroll 1
+        for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
+          float o[32];
+          if (n > 0) {
+            tmem_load32f((which ? t_dv : t_dk) + c + lanes, o);
+            tmem_loaded(o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          }
+          const float f = which ? 1.f : p.scale;
+          if (partial) {
+            float* const at_part = part + ((long long)which * p.sink_rows + r) * p.d + c;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (c + e < p.d) *reinterpret_cast<float4*>(at_part + e) = make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
+          } else if (it.chunk < 0 && key < p.Nk) {
+            store_row(static_cast<__nv_bfloat16*>(which ? p.dv : p.dk) + row, o, f, c, p.d);
+          }
+        }
+    }
+    tmem_before();
+  }
+  __syncthreads();
+  if (warp == 8) {
+    tmem_after();
+    tmem_free(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------ host
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* at = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &at, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+      at = nullptr;
+    return reinterpret_cast<EncodeFn>(at);
+  }();
+  return fn;
+}
+// [B, N, heads, d] with boxes of 128 positions x 64 features
+cudaError_t encode(CUtensorMap& m, const void* at, int d, int heads, int N, int B, long long sn, long long sb) {
+  const EncodeFn fn = encode_fn();
+  if (!fn) return cudaErrorNotSupported;
+  const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)N, (cuuint64_t)B};
+  const cuuint64_t strides[3] = {(cuuint64_t)d * 2, (cuuint64_t)sn * 2, (cuuint64_t)sb * 2};
+  const cuuint32_t box[4] = {64, 1, kT, 1}, step[4] = {1, 1, 1, 1};
+  return fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(at), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? cudaSuccess
+             : cudaErrorInvalidValue;
+}
+
+template <int DP, int SLOTS>
+cudaError_t run_fwd(const AttnParams& p, const Maps& maps, cudaStream_t st) {
+  static SmemGrant grant;
+  constexpr uint32_t smem = FwdSmem<DP, SLOTS>::bytes;
+  const cudaError_t e = grant_smem(grant, attn_tensor_fwd_kernel<DP, SLOTS>, smem);
+  if (e != cudaSuccess) return e;
+  const int tiles = (p.Nq + 2 * kT - 1) / (2 * kT);
+  return launch_behind(attn_tensor_fwd_kernel<DP, SLOTS>, dim3((unsigned)(tiles * p.H * p.B)), kThreads, smem, st, p, maps);
+}
+template <int DP, int SLOTS>
+cudaError_t run_bwd(const AttnParams& p, const Maps& maps, cudaStream_t st) {
+  static SmemGrant g1, g2;
+  constexpr uint32_t smem = BwdSmem<DP, SLOTS>::bytes;
+  cudaError_t e = grant_smem(g1, attn_tensor_dq_kernel<DP, SLOTS>, smem);
+  if (e == cudaSuccess) e = grant_smem(g2, attn_tensor_dkv_kernel<DP, SLOTS>, smem);
+  if (e != cudaSuccess) return e;
+  e = launch_behind(attn_tensor_dq_kernel<DP, SLOTS>, dim3((unsigned)((p.Nq + kT - 1) / kT * p.H * p.B)), kThreads, smem, st, p, maps);
+  if (e != cudaSuccess) return e;
+  const int items = (p.Nk + kT - 1) / kT + p.sink_tiles * p.chunks;
+  return launch_behind(attn_tensor_dkv_kernel<DP, SLOTS>, dim3((unsigned)(items * p.Hk * p.B)), kThreads, smem, st, p, maps);
+}
+cudaError_t encode_all(Maps& m, const AttnParams& p, bool bwd) {
+  cudaError_t e = encode(m.q, p.q, p.d, p.H, p.Nq, p.B, p.sq_n, p.sq_b);
+  if (e == cudaSuccess) e = encode(m.k, p.k, p.d, p.Hk, p.Nk, p.B, p.sk_n, p.sk_b);
+  if (e == cudaSuccess) e = encode(m.v, p.v, p.d, p.Hk, p.Nk, p.B, p.sv_n, p.sv_b);
+  if (e == cudaSuccess && bwd) e = encode(m.dy, p.dy, p.d, p.H, p.Nq, p.B, p.sdy_n, p.sdy_b);
+  return e;
+}
+
+}  // namespace
+
+// bf16 rows that a tensor map describes: 16-byte aligned, strides multiples of 16 bytes, not zero and not negative.
+bool attn_tensor_covers(const AttnParams& p, int dtype) {
+  if (dtype != DT_BF16 || !p.vec || p.d > 128 || p.Nk < 1) return false;
+  const long long s[8] = {p.sq_b, p.sq_n, p.sk_b, p.sk_n, p.sv_b, p.sv_n, p.sdy_b, p.sdy_n};
+  for (const long long x : s)
+    if (x < 8 || x >= (1ll << 38)) return false;
+  const void* const out[5] = {p.y, p.y_in, p.dq, p.dk, p.dv};
+  for (const void* o : out)
+    if (reinterpret_cast<uintptr_t>(o) & 15u) return false;
+  return true;
+}
+
+cudaError_t launch_attn_tensor_fwd(const AttnParams& p, cudaStream_t st) {
+  Maps m;
+  const cudaError_t e = encode_all(m, p, false);
+  if (e != cudaSuccess) return e;
+  return p.d <= 64 ? run_fwd<64, 8>(p, m, st) : run_fwd<128, 5>(p, m, st);
+}
+cudaError_t launch_attn_tensor_bwd(const AttnParams& p, cudaStream_t st) {
+  Maps m;
+  cudaError_t e = encode_all(m, p, true);
+  if (e == cudaSuccess) e = p.d <= 64 ? run_bwd<64, 8>(p, m, st) : run_bwd<128, 5>(p, m, st);
+  if (e != cudaSuccess || p.chunks == 0) return e;
+  return launch_attn_sink_sum(p, DT_BF16, kT, st);
+}
+
+}  // namespace ncn

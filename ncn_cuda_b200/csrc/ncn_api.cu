@@ -9,6 +9,7 @@
 #include <vector>
 
 #include "../../include/ncn_b200.h"
+#include "ncn_host.h"
 #include "ncn_generic.cuh"
 #include "ncn_rows_launch.h"
 #include "ncn_lanes_launch.h"
@@ -24,20 +25,15 @@ static thread_local char tl_cuda_err[256] = "";
 
 // The error is reported here and nowhere else: what cudaGetLastError() still holds of it (cudaLaunchKernelEx and the attribute calls
 // leave it there) would be read as the failure of the next launch, of this library or of the caller.
-static int cuda_fail(cudaError_t e) {
+int cuda_fail(cudaError_t e) {
   cudaGetLastError();
   std::snprintf(tl_cuda_err, sizeof(tl_cuda_err), "%s: %s", cudaGetErrorName(e), cudaGetErrorString(e));
   return NCN_ERR_CUDA;
 }
 
-struct DevInfo {
-  int dev = -1, sms = 0, smem_optin = 0;
-  int* status = nullptr;
-};
-
 // Per-device facts, looked up once per device and cached (the table is tiny and written
 // idempotently, so a race between two first calls is harmless).
-static int get_dev(DevInfo& out) {
+int get_dev(DevInfo& out) {
   static DevInfo table[64];
   static std::atomic<int> ready[64];
   int dev = 0;

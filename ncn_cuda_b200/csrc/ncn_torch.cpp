@@ -29,6 +29,7 @@
 #include <vector>
 
 #include "../../include/ncn_b200.h"
+#include "ncn_torch.h"
 
 namespace py = pybind11;
 using at::Tensor;
@@ -37,7 +38,7 @@ using torch::autograd::Node;
 using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
-namespace {
+namespace ncn_ext {
 
 // A non-zero status as the NCNError of _lib.py; also from the engine's threads, which do not hold the GIL.
 void check_status(const char* fn, int status) {
@@ -52,6 +53,29 @@ void check_status(const char* fn, int status) {
     throw err;
   }
 }
+
+// Tensors the nodes can take: the memory is the value.  Not those with a forward gradient (the nodes have no
+// forward-mode rule and would drop it), nor wrappers of functorch or of Python subclasses with their own dispatch.
+bool plain(const Tensor& t) {
+  constexpr c10::DispatchKeySet wrapped({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                         c10::DispatchKey::BatchedNestedTensor, c10::DispatchKey::Functionalize,
+                                         c10::DispatchKey::Python});
+  return !t.key_set().has_any(wrapped) && !t._fw_grad(/*level=*/0).defined();
+}
+
+bool under_transform() {
+  const c10::impl::LocalDispatchKeySet tls = c10::impl::tls_local_dispatch_key_set();
+  constexpr c10::DispatchKeySet modes({c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::Python});
+  return torch::jit::tracer::isTracing() || tls.included_.has_any(modes);
+}
+
+}  // namespace ncn_ext
+
+namespace {
+
+using ncn_ext::check_status;
+using ncn_ext::plain;
+using ncn_ext::under_transform;
 
 void check_activations(const Tensor& x, const Tensor& xa) {
   if (!x.is_cuda()) throw std::runtime_error("NCN kernels run on CUDA tensors only; there is no CPU path in this package");
@@ -525,23 +549,12 @@ std::tuple<Tensor, Tensor> chain_forward(const Tensor& x_in, const Tensor& xa_in
 // What an entry returns where the Python Function (ncn_pytorch_wrapper_v2.py) has to take the call: nothing.
 using Result = std::optional<std::tuple<Tensor, Tensor>>;
 
-// Tensors the nodes can take: the memory is the value.  Not those with a forward gradient (the nodes have no
-// forward-mode rule and would drop it), nor wrappers of functorch or of Python subclasses with their own dispatch.
-bool plain(const Tensor& t) {
-  constexpr c10::DispatchKeySet wrapped({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
-                                         c10::DispatchKey::BatchedNestedTensor, c10::DispatchKey::Functionalize,
-                                         c10::DispatchKey::Python});
-  return !t.key_set().has_any(wrapped) && !t._fw_grad(/*level=*/0).defined();
-}
-
 // A call the native nodes must not answer: it goes through the Function, which records, transforms or refuses it as
 // any custom Function is.  Under torch.jit.trace the kernels leave no trace of themselves, and the graph would hold
 // the allocations of their results alone; with a functorch transform or a dispatch mode in effect the nodes would
 // pass it by.
 bool needs_function(const Tensor& x, const Tensor& xa, const variable_list& ws) {
-  const c10::impl::LocalDispatchKeySet tls = c10::impl::tls_local_dispatch_key_set();
-  constexpr c10::DispatchKeySet modes({c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::Python});
-  if (torch::jit::tracer::isTracing() || tls.included_.has_any(modes)) return true;
+  if (under_transform()) return true;
   if (!plain(x) || !plain(xa)) return true;
   for (const Tensor& w : ws)
     if (!plain(w)) return true;
@@ -690,4 +703,5 @@ PYBIND11_MODULE(_ncn_torch, m) {
   m.def("stages", &py_stages);
   m.def("stage_ctx", &py_stage_ctx);
   m.def("host_step", &py_host_step);
+  ncn_ext::bind_attention(m);
 }

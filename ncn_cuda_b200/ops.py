@@ -8,6 +8,7 @@ forward and backward, and tests.
 from __future__ import annotations
 
 import contextlib
+import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -311,6 +312,155 @@ def net_bwd(s0, s1, dy, dya, W, alpha, activation, n_cache, n_head, first_module
     if want_inputs:
         return dx, dxa, dW, xr, xar
     return dx, dxa, dW
+
+
+# ---------------------------------------------------------------- attention (attention.py)
+NO_WINDOW = 2**62  # every position before
+
+
+def _strided(*ts):
+    """The tensors with the features of a position next to each other, and their {row, position} strides for the C ABI."""
+    ts = [t if t.numel() and t.stride(2) == 1 else t.contiguous() for t in ts]
+    flat = [s for t in ts for s in (t.stride(0), t.stride(1))]
+    return ts, (ctypes.c_int64 * len(flat))(*flat)
+
+
+def _check_qkv(q, k, v, n_head):
+    _check_inputs(q)
+    for t in (k, v):
+        if t.dim() != 3 or t.shape[0] != q.shape[0] or t.dtype != q.dtype or t.device != q.device or t.shape != k.shape:
+            raise ValueError("q, k and v must agree in batch size, dtype and device, k and v in shape")
+    if n_head < 1 or q.shape[2] % n_head:
+        raise ValueError(f"n_head = {n_head} does not divide the {q.shape[2]} features of the queries")
+
+
+def _per_row(t, name, B, device):
+    if t is None:
+        return None
+    t = torch.as_tensor(t)
+    if t.numel() != B:
+        raise ValueError(f"{name} has {t.numel()} entries for {B} batch rows")
+    return t.to(device=device, dtype=torch.int32).contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def window_fwd(q, k, v, n_head, window, n_sink, scale, start, ctxlen=None, q_start=None, want_lse=False):
+    """Returns (y, lse or None); lse (opaque) goes to window_bwd."""
+    lib = _lib.load()
+    _check_qkv(q, k, v, n_head)
+    (B, Nq, E), (_, Nk, Ek) = q.shape, k.shape
+    ctxlen, q_start = _per_row(ctxlen, "ctxlen", B, q.device), _per_row(q_start, "q_start", B, q.device)
+    (q, k, v), strides = _strided(q, k, v)
+    y = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty(lib.ncn_window_lse_bytes(B, Nq, n_head) // 4, dtype=torch.float32, device=q.device) if want_lse else None
+    with _on(q.device):
+        rc = lib.ncn_window_fwd(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(), _ptr(lse), _ptr(ctxlen), _ptr(q_start), strides, B, Nq, Nk, E, Ek,
+            n_head, window, n_sink, start, scale, _dtype_code(q), _stream(),
+        )
+    _lib.check("ncn_window_fwd", rc)
+    return y, lse
+
+
+def window_bwd(q, k, v, y, dy, lse, n_head, window, n_sink, scale, start, ctxlen=None, q_start=None):
+    """Returns (dq, dk, dv)."""
+    lib = _lib.load()
+    _check_qkv(q, k, v, n_head)
+    (B, Nq, E), (_, Nk, Ek) = q.shape, k.shape
+    ctxlen, q_start = _per_row(ctxlen, "ctxlen", B, q.device), _per_row(q_start, "q_start", B, q.device)
+    (q, k, v, dy), strides = _strided(q, k, v, dy)
+    y = y.contiguous()
+    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
+    if B == 0 or Nq == 0:
+        return dq, dk.zero_(), dv.zero_()
+    dt = _dtype_code(q)
+    with _on(q.device):
+        nbytes = lib.ncn_window_bwd_workspace_bytes(B, Nq, Nk, E, Ek, n_head, window, n_sink, dt)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        rc = lib.ncn_window_bwd(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(), dy.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+            dv.data_ptr(), _ptr(ctxlen), _ptr(q_start), strides, ws.data_ptr(), nbytes, B, Nq, Nk, E, Ek, n_head, window, n_sink, start,
+            scale, dt, _stream(),
+        )
+    _lib.check("ncn_window_bwd", rc)
+    return dq, dk, dv
+
+
+def _rotary_args(q, k, freqs, positions, n_head):
+    _check_inputs(q)
+    B, N, E = q.shape
+    if k is not None and (k.dim() != 3 or k.shape[:2] != q.shape[:2] or k.dtype != q.dtype or k.device != q.device):
+        raise ValueError("q and k must agree in batch size, positions, dtype and device")
+    if n_head < 1 or E % n_head:
+        raise ValueError(f"n_head = {n_head} does not divide the {E} features of the queries")
+    if freqs.dim() != 1 or 2 * freqs.numel() > E // n_head:
+        raise ValueError("freqs must hold one frequency for each rotated pair of a head")
+    freqs = freqs.detach().to(device=q.device, dtype=torch.float64).contiguous()
+    stride = 0
+    if positions is not None:
+        shared = positions.dim() == 1 or (positions.dim() == 2 and positions.shape[0] == 1)
+        if positions.dim() not in (1, 2) or positions.shape[-1] != N or (not shared and positions.shape[0] != B):
+            raise ValueError("positions must be [N] or [B, N] for tensors [B, N, E]")
+        positions = positions.to(device=q.device, dtype=torch.int64).contiguous()
+        stride = 0 if shared else N
+    return freqs, positions, stride
+
+
+def qk_rotary(q, k, wq, wk, freqs, positions, n_head, start, interleaved, eps, magnitude, inverse=False):
+    """Returns (q', k'): with weights the heads are normalised first."""
+    lib = _lib.load()
+    freqs, positions, pos_stride = _rotary_args(q, k, freqs, positions, n_head)
+    B, N, E = q.shape
+    ts, strides = _strided(*(t for t in (q, k) if t is not None))
+    q, k = ts[0], ts[1] if len(ts) > 1 else None
+    if k is None:
+        strides = (ctypes.c_int64 * 4)(*strides, 0, 0)
+    if wq is not None:
+        wq = _weights(wq, E // n_head, q.device)
+        wk = None if k is None else _weights(wk, E // n_head, q.device)
+    yq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    yk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
+    with _on(q.device):
+        rc = lib.ncn_qk_rotary(
+            q.data_ptr(), _ptr(k), _ptr(wq), _ptr(wk), freqs.data_ptr(), _ptr(positions), pos_stride, start, yq.data_ptr(), _ptr(yk),
+            strides, B, N, E, 0 if k is None else k.shape[2], n_head, 2 * freqs.numel(), int(interleaved), eps, magnitude, int(inverse),
+            _dtype_code(q), _stream(),
+        )
+    _lib.check("ncn_qk_rotary", rc)
+    return yq, yk
+
+
+def qk_norm_rotary_bwd(q, k, wq, wk, freqs, positions, dyq, dyk, n_head, start, interleaved, eps, magnitude):
+    """Returns (dq, dk, dwq, dwk); the weights' gradients are fp32 [E / n_head]."""
+    lib = _lib.load()
+    freqs, positions, pos_stride = _rotary_args(q, k, freqs, positions, n_head)
+    (B, N, E), d = q.shape, q.shape[2] // n_head
+    wq = _weights(wq, d, q.device)
+    dwq = torch.zeros(d, dtype=torch.float32, device=q.device)
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    dk = dwk = None
+    if k is None:
+        (q, dyq), s = _strided(q, dyq)
+        strides = (ctypes.c_int64 * 8)(s[0], s[1], 0, 0, s[2], s[3], 0, 0)
+    else:
+        wk, dwk = _weights(wk, d, q.device), torch.zeros(d, dtype=torch.float32, device=q.device)
+        dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+        (q, k, dyq, dyk), strides = _strided(q, k, dyq, dyk)
+    if B == 0 or N == 0:
+        return dq, dk, dwq, dwk
+    with _on(q.device):
+        nbytes = lib.ncn_qk_norm_rotary_workspace_bytes(B, N, E, n_head)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        rc = lib.ncn_qk_norm_rotary_bwd(
+            q.data_ptr(), _ptr(k), wq.data_ptr(), _ptr(wk), freqs.data_ptr(), _ptr(positions), pos_stride, start, dyq.data_ptr(),
+            _ptr(dyk), dq.data_ptr(), _ptr(dk), dwq.data_ptr(), _ptr(dwk), strides, ws.data_ptr(), nbytes, B, N, E,
+            0 if k is None else k.shape[2], n_head, 2 * freqs.numel(), int(interleaved), eps, magnitude, _dtype_code(q), _stream(),
+        )
+    _lib.check("ncn_qk_norm_rotary_bwd", rc)
+    return dq, dk, dwq, dwk
 
 
 def device_status() -> None:
