@@ -226,9 +226,10 @@ size_t ncn_ckpt_bytes(int64_t B, int64_t N, int64_t E, int L, int ckpt_every, in
  * key's v reaches, in the forward and backward, queries up to 256 positions from those that see it.)  ctxlen (int32 [B] on the device) null: Nk.
  * q_start (int32 [B] on the device) null: start for every row.  window >= 1, n_sink >= 0, scale > 0. */
 
-/* Forward.  lse: null, or ncn_window_lse_bytes(...) bytes that ncn_window_bwd takes (opaque). */
-size_t ncn_window_lse_bytes(int64_t B, int64_t Nq, int n_head);
-int ncn_window_fwd(const void* q, const void* k, const void* v, void* y, float* lse, const int* ctxlen, const int* q_start,
+/* Forward.  state: null, or ncn_window_state_bytes(...) bytes, 16-byte aligned, that ncn_window_bwd takes (opaque: the softmax's sums and, with
+ * bf16, what rounding took off y). */
+size_t ncn_window_state_bytes(int64_t B, int64_t Nq, int64_t E, int n_head, int dtype);
+int ncn_window_fwd(const void* q, const void* k, const void* v, void* y, void* state, const int* ctxlen, const int* q_start,
                    const int64_t* strides, int64_t B, int64_t Nq, int64_t Nk, int64_t E, int64_t Ek, int n_head, int64_t window,
                    int64_t n_sink, int64_t start, double scale, int dtype, void* stream);
 
@@ -236,7 +237,7 @@ int ncn_window_fwd(const void* q, const void* k, const void* v, void* y, float* 
  * bitwise reproducible for equal arguments on one device. */
 size_t ncn_window_bwd_workspace_bytes(int64_t B, int64_t Nq, int64_t Nk, int64_t E, int64_t Ek, int n_head, int64_t window, int64_t n_sink,
                                       int dtype);
-int ncn_window_bwd(const void* q, const void* k, const void* v, const void* y, const void* dy, const float* lse, void* dq, void* dk, void* dv,
+int ncn_window_bwd(const void* q, const void* k, const void* v, const void* y, const void* dy, const void* state, void* dq, void* dk, void* dv,
                    const int* ctxlen, const int* q_start, const int64_t* strides, void* workspace, size_t workspace_bytes, int64_t B,
                    int64_t Nq, int64_t Nk, int64_t E, int64_t Ek, int n_head, int64_t window, int64_t n_sink, int64_t start, double scale,
                    int dtype, void* stream);

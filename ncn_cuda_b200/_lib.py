@@ -78,7 +78,7 @@ SIGNATURES = {
     "ncn_last_cuda_error": (c_char_p, []),
     "ncn_version": (c_int, []),
     "ncn_reload_env": (None, []),
-    "ncn_window_lse_bytes": (c_size_t, [c_int64] * 2 + [c_int]),
+    "ncn_window_state_bytes": (c_size_t, [c_int64] * 3 + [c_int] * 2),
     "ncn_window_fwd": (
         c_int,
         [c_void_p] * 8 + [c_int64] * 5 + [c_int] + [c_int64] * 3 + [c_double, c_int, c_void_p],

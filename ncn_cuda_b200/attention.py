@@ -126,14 +126,14 @@ class WindowAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, n_head, window, n_sink, scale, ctxlen, q_start, start):
         ctx.cfg = (n_head, window, n_sink, scale, start)
-        y, lse = ops.window_fwd(q, k, v, *ctx.cfg, ctxlen=ctxlen, q_start=q_start, want_lse=True)
-        ctx.save_for_backward(q, k, v, y, lse, ctxlen, q_start)
+        y, state = ops.window_fwd(q, k, v, *ctx.cfg, ctxlen=ctxlen, q_start=q_start, want_state=True)
+        ctx.save_for_backward(q, k, v, y, state, ctxlen, q_start)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        q, k, v, y, lse, ctxlen, q_start = ctx.saved_tensors
-        dq, dk, dv = ops.window_bwd(q, k, v, y, dy, lse, *ctx.cfg, ctxlen=ctxlen, q_start=q_start)
+        q, k, v, y, state, ctxlen, q_start = ctx.saved_tensors
+        dq, dk, dv = ops.window_bwd(q, k, v, y, dy, state, *ctx.cfg, ctxlen=ctxlen, q_start=q_start)
         return dq, dk, dv, None, None, None, None, None, None, None
 
 

@@ -76,6 +76,11 @@ void bwd_tiles(const AttnParams& p, int dtype, int& T, int& TQ) {
   }
 }
 
+void set_state(AttnParams& p, void* state, int dtype) {
+  p.lse = static_cast<float*>(state);
+  p.rest = state && dtype == NCN_BF16 ? reinterpret_cast<__nv_bfloat16*>(p.lse + delta_floats(p)) : nullptr;
+}
+
 bool grid_ok(const AttnParams& p) {
   const long long tq = (p.Nq + 31) / 32, tk = (p.Nk + 31) / 32 + 64 * ((p.n_sink + 63) / 64);
   return tq * p.H <= kMaxGrid / p.B && (tk > p.n_sink ? tk : p.n_sink) * p.Hk <= kMaxGrid / p.B && 8ll * p.Hk * p.G * p.Nq <= kMaxGrid / p.B;
@@ -88,12 +93,12 @@ using namespace ncn;
 
 extern "C" {
 
-size_t ncn_window_lse_bytes(int64_t B, int64_t Nq, int n_head) {
-  if (B <= 0 || Nq <= 0 || n_head <= 0 || Nq > kMaxLength) return 0;
-  return (size_t)B * n_head * round_up(Nq, 128) * sizeof(float);
+size_t ncn_window_state_bytes(int64_t B, int64_t Nq, int64_t E, int n_head, int dtype) {
+  if (B <= 0 || Nq <= 0 || E <= 0 || n_head <= 0 || Nq > kMaxLength) return 0;
+  return (size_t)B * n_head * round_up(Nq, 128) * sizeof(float) + (dtype == NCN_BF16 ? (size_t)B * Nq * E * 2 : 0);
 }
 
-int ncn_window_fwd(const void* q, const void* k, const void* v, void* y, float* lse, const int* ctxlen, const int* q_start,
+int ncn_window_fwd(const void* q, const void* k, const void* v, void* y, void* state, const int* ctxlen, const int* q_start,
                    const int64_t* strides, int64_t B, int64_t Nq, int64_t Nk, int64_t E, int64_t Ek, int n_head, int64_t window,
                    int64_t n_sink, int64_t start, double scale, int dtype, void* stream) {
   AttnParams p{};
@@ -103,7 +108,8 @@ int ncn_window_fwd(const void* q, const void* k, const void* v, void* y, float* 
   if (!grid_ok(p)) return NCN_ERR_TOO_LARGE;
   DevInfo dev;
   if ((rc = get_dev(dev)) != NCN_OK) return rc;
-  p.y = y, p.lse = lse, p.status = dev.status;
+  p.y = y, p.status = dev.status;
+  set_state(p, state, dtype);
   cudaError_t e = attn_tensor_covers(p, dtype) ? launch_attn_tensor_fwd(p, (cudaStream_t)stream) : launch_attn_simt_fwd(p, dtype, (cudaStream_t)stream);
   return e == cudaSuccess ? NCN_OK : cuda_fail(e);
 }
@@ -124,18 +130,19 @@ size_t ncn_window_bwd_workspace_bytes(int64_t B, int64_t Nq, int64_t Nk, int64_t
   return most * sizeof(float);
 }
 
-int ncn_window_bwd(const void* q, const void* k, const void* v, const void* y, const void* dy, const float* lse, void* dq, void* dk, void* dv,
+int ncn_window_bwd(const void* q, const void* k, const void* v, const void* y, const void* dy, const void* state, void* dq, void* dk, void* dv,
                    const int* ctxlen, const int* q_start, const int64_t* strides, void* workspace, size_t workspace_bytes, int64_t B,
                    int64_t Nq, int64_t Nk, int64_t E, int64_t Ek, int n_head, int64_t window, int64_t n_sink, int64_t start, double scale,
                    int dtype, void* stream) {
   AttnParams p{};
   int rc = attn_params(p, q, k, v, ctxlen, q_start, strides, 8, B, Nq, Nk, E, Ek, n_head, window, n_sink, start, scale, dtype);
   if (rc != NCN_OK || B == 0 || Nq == 0) return rc;
-  if (!y || !dy || !lse || !dq || ((!dk || !dv) && Nk > 0)) return NCN_ERR_NULL;
+  if (!y || !dy || !state || !dq || ((!dk || !dv) && Nk > 0)) return NCN_ERR_NULL;
   if (!grid_ok(p)) return NCN_ERR_TOO_LARGE;
   DevInfo dev;
   if ((rc = get_dev(dev)) != NCN_OK) return rc;
-  p.y_in = y, p.dy = dy, p.lse = const_cast<float*>(lse), p.dq = dq, p.dk = dk, p.dv = dv, p.status = dev.status;
+  p.y_in = y, p.dy = dy, p.dq = dq, p.dk = dk, p.dv = dv, p.status = dev.status;
+  set_state(p, const_cast<void*>(state), dtype);
   if (!aligned16(dy)) p.vec = 0;
   int T, TQ;
   bwd_tiles(p, dtype, T, TQ);
@@ -223,7 +230,7 @@ int ncn_qk_rotary(const void* q, const void* k, const float* wq, const float* wk
 
 size_t ncn_qk_norm_rotary_workspace_bytes(int64_t B, int64_t N, int64_t E, int n_head) {
   if (B <= 0 || N <= 0 || E <= 0 || n_head <= 0 || E % n_head != 0) return 0;
-  // a row of sums per CTA, of which every warp's worth of heads has one at most
+  // a row of sums per CTA, of which there are no more than heads of queries
   const long long rows = B > kRotaryMostCtas || N > kRotaryMostCtas || B * N > kRotaryMostCtas ? kRotaryMostCtas : B * N;
   const long long ctas = rows * n_head > kRotaryMostCtas ? kRotaryMostCtas : rows * n_head;
   return (size_t)ctas * 2 * (E / n_head) * sizeof(float);

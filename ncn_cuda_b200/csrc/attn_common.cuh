@@ -16,6 +16,7 @@ struct AttnParams {
   const void *q, *k, *v;       // [B, N, heads * d] with the strides below, features of a position contiguous
   void* y;                     // [B, Nq, H * d], contiguous
   float* lse;                  // [B, H, Nqp], log2 of the softmax sums; +inf where nothing is seen.  May be null in the forward
+  __nv_bfloat16* rest;         // bf16, kept with lse: what rounding took off y, itself rounded to bf16, [B, Nq, H * d].  May be null
   const void *dy, *y_in;       // backward: cotangent (strides) and output
   void *dq, *dk, *dv;          // contiguous
   float* delta;                // [B, H, Nqp]: sum(dy * y)
@@ -131,6 +132,14 @@ __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
+// A result and what rounding it takes off.  The backward's delta = sum(dy * y) is taken from every dP of a row: with the 8 bits of a bf16
+// y it would bring an error as large as dS's own rounding where a query sees few keys (2 visible keys: 1.5 times the error of dq).
+__device__ __forceinline__ void put_rest(float* p, float*, float v) { *p = v; }
+__device__ __forceinline__ void put_rest(__nv_bfloat16* p, __nv_bfloat16* rest, float v) {
+  const __nv_bfloat16 r = __float2bfloat16(v);
+  *p = r;
+  if (rest) *rest = __float2bfloat16(v - __bfloat162float(r));
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

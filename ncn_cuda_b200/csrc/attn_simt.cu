@@ -180,11 +180,12 @@ __global__ void __launch_bounds__(256) attn_simt_fwd_kernel(const AttnParams p) 
     const int qi = i0 + 4 * ty + i;
     if (qi >= p.Nq) continue;
     const float inv = l[i] > 0.f || l[i] != l[i] ? 1.f / l[i] : 0.f;
-    T* y = static_cast<T*>(p.y) + ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
+    const long long at = ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
+    T *y = static_cast<T*>(p.y) + at, *rest = sizeof(T) == 2 && p.rest ? reinterpret_cast<T*>(p.rest) + at : nullptr;
 #pragma unroll
     for (int e = 0; e < DP / 16; ++e) {
       const int c = feature_of<DP>(e);
-      if (c < p.d) put(y + c, o[i][e] * inv);
+      if (c < p.d) put_rest(y + c, rest ? rest + c : nullptr, o[i][e] * inv);
     }
     if (p.lse && tx == 0)
       p.lse[((long long)b * p.H + h) * p.Nqp + qi] = l[i] == 0.f ? INFINITY : m[i] * p.scale_log2 + log2f(l[i]);
@@ -220,8 +221,12 @@ __global__ void __launch_bounds__(256) attn_simt_dq_kernel(const AttnParams p) {
     lse[i] = live ? p.lse[at] : INFINITY;
     float sum = 0.f;
     if (live) {
-      const T* y = static_cast<const T*>(p.y_in) + ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
-      for (int c = tx; c < p.d; c += 16) sum = fmaf(dO[r * (DP + 4) + c], to_f(y[c]), sum);
+      const long long row = ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
+      const T* y = static_cast<const T*>(p.y_in) + row;
+      for (int c = tx; c < p.d; c += 16) {
+        const float rest = sizeof(T) == 2 ? to_f(p.rest[row + c]) : 0.f;
+        sum = fmaf(dO[r * (DP + 4) + c], to_f(y[c]) + rest, sum);
+      }
     }
     delta[i] = sum16(sum);
     if (tx == 0 && qi < p.Nq) p.delta[at] = delta[i];

@@ -183,6 +183,17 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// what the rounding in store_row takes off, rounded itself
+__device__ __forceinline__ void store_rest(__nv_bfloat16* row, const float (&x)[32], float f, int c0, int d) {
+  float r[32];
+#pragma unroll
+  for (int e = 0; e < 32; ++e) r[e] = x[e] * f - __bfloat162float(__float2bfloat16(x[e] * f));
+#pragma unroll
+  for (int e = 0; e < 32; e += 8)
+    if (c0 + e < d)
+      *reinterpret_cast<uint4*>(row + c0 + e) =
+          make_uint4(pack(r[e], r[e + 1]), pack(r[e + 2], r[e + 3]), pack(r[e + 4], r[e + 5]), pack(r[e + 6], r[e + 7]));
+}
 // 32 features of a row to global memory, c0 .. c0 + 31 of d (a multiple of 8)
 __device__ __forceinline__ void store_row(__nv_bfloat16* row, const float (&x)[32], float f, int c0, int d) {
 #pragma unroll
@@ -395,9 +406,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_fwd_kernel(const __gr
     if (mine > 0 && ok) ok = wait(o_full + x, 0);
     tmem_after();
     if (ok) {
-      const bool some = mine > 0 && !(l == 0.f);
+      // (padding between rows that see a whole tile has had no mask)
+      const bool some = mine > 0 && pos >= 0 && pos < end && !(l == 0.f);
       const float inv = some ? 1.f / l : 0.f;
-      __nv_bfloat16* const row = static_cast<__nv_bfloat16*>(p.y) + ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
+      const long long row = ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
 #pragma unroll 1
       for (int c = 0; c < DP; c += 32) {
         float o[32];
@@ -409,7 +421,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_fwd_kernel(const __gr
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0.f;
         }
-        if (qi < p.Nq) store_row(row, o, inv, c, p.d);
+        if (qi < p.Nq) {
+          store_row(static_cast<__nv_bfloat16*>(p.y) + row, o, inv, c, p.d);
+          if (p.rest) store_rest(p.rest + row, o, inv, c, p.d);
+        }
       }
       if (p.lse && qi < p.Nq) p.lse[((long long)b * p.H + h) * p.Nqp + qi] = some ? ref + log2f(l) : INFINITY;
     }
@@ -531,15 +546,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
     // delta: half of the features each
     float sum = 0.f;
     if (live) {
-      const __nv_bfloat16* y = static_cast<const __nv_bfloat16*>(p.y_in) + ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
+      const long long y_row = ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
+      const __nv_bfloat16 *y = static_cast<const __nv_bfloat16*>(p.y_in) + y_row, *rest = p.rest + y_row;
       const __nv_bfloat16* dy = static_cast<const __nv_bfloat16*>(p.dy) + b * p.sdy_b + qi * p.sdy_n + (long long)h * p.d;
       for (int c = half * (DP / 2); c < min((half + 1) * (DP / 2), p.d); c += 8) {
-        const uint4 u = *reinterpret_cast<const uint4*>(y + c), w = *reinterpret_cast<const uint4*>(dy + c);
-        const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, ww[4] = {w.x, w.y, w.z, w.w};
+        const uint4 u = *reinterpret_cast<const uint4*>(y + c), w = *reinterpret_cast<const uint4*>(dy + c),
+                    t = *reinterpret_cast<const uint4*>(rest + c);
+        const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, ww[4] = {w.x, w.y, w.z, w.w}, tt[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          sum = fmaf(__uint_as_float(uu[e] << 16), __uint_as_float(ww[e] << 16), sum);
-          sum = fmaf(__uint_as_float(uu[e] & 0xffff0000u), __uint_as_float(ww[e] & 0xffff0000u), sum);
+          sum = fmaf(__uint_as_float(uu[e] << 16) + __uint_as_float(tt[e] << 16), __uint_as_float(ww[e] << 16), sum);
+          sum = fmaf(__uint_as_float(uu[e] & 0xffff0000u) + __uint_as_float(tt[e] & 0xffff0000u), __uint_as_float(ww[e] & 0xffff0000u), sum);
         }
       }
     }
@@ -857,6 +874,22 @@ EncodeFn encode_fn() {
   }();
   return fn;
 }
+// Tensor maps are encoded by the driver, which wants a context current in the calling thread; a thread of the autograd engine that has
+// made no runtime call yet has none.
+cudaError_t bind_context() {
+  static const auto current = [] {
+    void* at = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &at, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+      at = nullptr;
+    return reinterpret_cast<CUresult (*)(CUcontext*)>(at);
+  }();
+  CUcontext ctx = nullptr;
+  if (current && current(&ctx) == CUDA_SUCCESS && ctx) return cudaSuccess;
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  return e == cudaSuccess ? cudaSetDevice(dev) : e;
+}
 // [B, N, heads, d] with boxes of 128 positions x 64 features
 cudaError_t encode(CUtensorMap& m, const void* at, int d, int heads, int N, int B, long long sn, long long sb) {
   const EncodeFn fn = encode_fn();
@@ -892,7 +925,8 @@ cudaError_t run_bwd(const AttnParams& p, const Maps& maps, cudaStream_t st) {
   return launch_behind(attn_tensor_dkv_kernel<DP, SLOTS>, dim3((unsigned)(items * p.Hk * p.B)), kThreads, smem, st, p, maps);
 }
 cudaError_t encode_all(Maps& m, const AttnParams& p, bool bwd) {
-  cudaError_t e = encode(m.q, p.q, p.d, p.H, p.Nq, p.B, p.sq_n, p.sq_b);
+  cudaError_t e = bind_context();
+  if (e == cudaSuccess) e = encode(m.q, p.q, p.d, p.H, p.Nq, p.B, p.sq_n, p.sq_b);
   if (e == cudaSuccess) e = encode(m.k, p.k, p.d, p.Hk, p.Nk, p.B, p.sk_n, p.sk_b);
   if (e == cudaSuccess) e = encode(m.v, p.v, p.d, p.Hk, p.Nk, p.B, p.sv_n, p.sv_b);
   if (e == cudaSuccess && bwd) e = encode(m.dy, p.dy, p.d, p.H, p.Nq, p.B, p.sdy_n, p.sdy_b);
@@ -907,7 +941,7 @@ bool attn_tensor_covers(const AttnParams& p, int dtype) {
   const long long s[8] = {p.sq_b, p.sq_n, p.sk_b, p.sk_n, p.sv_b, p.sv_n, p.sdy_b, p.sdy_n};
   for (const long long x : s)
     if (x < 8 || x >= (1ll << 38)) return false;
-  const void* const out[5] = {p.y, p.y_in, p.dq, p.dk, p.dv};
+  const void* const out[6] = {p.y, p.y_in, p.dq, p.dk, p.dv, p.lse};  // (rest lies a multiple of 512 bytes behind lse)
   for (const void* o : out)
     if (reinterpret_cast<uintptr_t>(o) & 15u) return false;
   return true;

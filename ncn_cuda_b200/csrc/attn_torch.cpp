@@ -96,19 +96,19 @@ struct WindowCfg {
 
 struct WindowNode : public Node {
   WindowCfg c{};
-  SavedVariable q, k, v, y, lse, ctxlen, q_start;
+  SavedVariable q, k, v, y, state, ctxlen, q_start;
   bool has_ctx = false, has_start = false;
 
   std::string name() const override { return "NCNWindowAttentionBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    for (SavedVariable* s : {&q, &k, &v, &y, &lse, &ctxlen, &q_start}) s->reset_data();
+    for (SavedVariable* s : {&q, &k, &v, &y, &state, &ctxlen, &q_start}) s->reset_data();
   }
   variable_list apply(variable_list&& g) override {
     std::lock_guard<std::mutex> lock(mutex_);
     at::NoGradGuard no_grad;
     if (!g[0].defined()) return variable_list(3);
-    const Tensor Q = q.unpack(), K = k.unpack(), V = v.unpack(), Y = y.unpack(shared_from_this()), L = lse.unpack();
+    const Tensor Q = q.unpack(), K = k.unpack(), V = v.unpack(), Y = y.unpack(shared_from_this()), L = state.unpack();
     const Tensor ctx = has_ctx ? ctxlen.unpack() : Tensor(), st = has_start ? q_start.unpack() : Tensor();
     const c10::cuda::OptionalCUDAGuard guard(Q.device());
     const Tensor dy = readable(g[0]), y_c = Y.contiguous();
@@ -124,7 +124,7 @@ struct WindowNode : public Node {
     strides_of(qr, s), strides_of(kr, s + 2), strides_of(vr, s + 4), strides_of(dy, s + 6);
     check_status("ncn_window_bwd",
                  ncn_window_bwd(qr.const_data_ptr(), kr.const_data_ptr(), vr.const_data_ptr(), y_c.const_data_ptr(), dy.const_data_ptr(),
-                                L.const_data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), int_ptr(ctx), int_ptr(st), s,
+                                L.const_data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), int_ptr(ctx), int_ptr(st), s,
                                 ws.data_ptr(), bytes, B, Nq, Nk, E, Ek, (int)c.n_head, c.window, c.n_sink, c.start, c.scale, dt,
                                 stream_of(Q)));
     return {dq, dk, dv};
@@ -153,17 +153,17 @@ std::optional<Tensor> py_window(const Tensor& q, const Tensor& k, const Tensor& 
     const Tensor ctx = per_row(ctxlen, "ctxlen", B, q.device()), st = per_row(q_start, "q_start", B, q.device());
     const Tensor qr = readable(q), kr = readable(k), vr = readable(v);
     y = at::empty(q.sizes(), qr.options());
-    Tensor lse;
-    if (grad) lse = at::empty({(int64_t)(ncn_window_lse_bytes(B, Nq, (int)n_head) / 4)}, qr.options().dtype(at::kFloat));
+    Tensor state;
+    if (grad) state = at::empty({(int64_t)ncn_window_state_bytes(B, Nq, E, (int)n_head, dtype_code(q))}, qr.options().dtype(at::kByte));
     int64_t s[6];
     strides_of(qr, s), strides_of(kr, s + 2), strides_of(vr, s + 4);
     check_status("ncn_window_fwd",
                  ncn_window_fwd(qr.const_data_ptr(), kr.const_data_ptr(), vr.const_data_ptr(), y.data_ptr(),
-                                grad ? lse.mutable_data_ptr<float>() : nullptr, int_ptr(ctx), int_ptr(st), s, B, Nq, Nk, E, Ek, (int)n_head,
+                                grad ? state.data_ptr() : nullptr, int_ptr(ctx), int_ptr(st), s, B, Nq, Nk, E, Ek, (int)n_head,
                                 window, n_sink, start, scale, dtype_code(q), stream_of(q)));
     if (grad) {
       node->q = SavedVariable(q, false), node->k = SavedVariable(k, false), node->v = SavedVariable(v, false);
-      node->lse = SavedVariable(lse, false);
+      node->state = SavedVariable(state, false);
       if (ctx.defined()) node->ctxlen = SavedVariable(ctx, false), node->has_ctx = true;
       if (st.defined()) node->q_start = SavedVariable(st, false), node->has_start = true;
     }

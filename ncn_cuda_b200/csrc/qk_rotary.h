@@ -20,12 +20,14 @@ struct RotaryParams {
   long long pos_b, start;   // stride of a row of positions (0: the same for all)
   float* partial;           // backward of the norm: [grid][2][d]
   int B, N, d, R;
-  int interleaved, backward, vec, teams;  // teams: how many share the heads of one position
+  int interleaved, backward, vec;
+  int span, parts;          // positions that a CTA takes at a time, CTAs that share their heads
   float eps, magnitude;
 };
 
+constexpr int kRotarySpan = 16, kRotaryTable = 1024;  // most positions of a span; its pairs of sines
 constexpr long long kRotaryMostCtas = 8192;  // of a launch: rows of partial sums
-int rotary_plan(RotaryParams& p, int sms);  // sets teams; returns the CTAs of a launch
+int rotary_plan(RotaryParams& p, int sms);  // sets span and parts; returns the CTAs of a launch
 cudaError_t launch_rotary(const RotaryParams& p, int dtype, int grid, cudaStream_t st);
 
 }  // namespace ncn

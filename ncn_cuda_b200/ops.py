@@ -347,25 +347,25 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def window_fwd(q, k, v, n_head, window, n_sink, scale, start, ctxlen=None, q_start=None, want_lse=False):
-    """Returns (y, lse or None); lse (opaque) goes to window_bwd."""
+def window_fwd(q, k, v, n_head, window, n_sink, scale, start, ctxlen=None, q_start=None, want_state=False):
+    """Returns (y, state or None); state (opaque) goes to window_bwd."""
     lib = _lib.load()
     _check_qkv(q, k, v, n_head)
     (B, Nq, E), (_, Nk, Ek) = q.shape, k.shape
     ctxlen, q_start = _per_row(ctxlen, "ctxlen", B, q.device), _per_row(q_start, "q_start", B, q.device)
     (q, k, v), strides = _strided(q, k, v)
     y = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty(lib.ncn_window_lse_bytes(B, Nq, n_head) // 4, dtype=torch.float32, device=q.device) if want_lse else None
+    state = torch.empty(lib.ncn_window_state_bytes(B, Nq, E, n_head, _dtype_code(q)), dtype=torch.uint8, device=q.device) if want_state else None
     with _on(q.device):
         rc = lib.ncn_window_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(), _ptr(lse), _ptr(ctxlen), _ptr(q_start), strides, B, Nq, Nk, E, Ek,
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(), _ptr(state), _ptr(ctxlen), _ptr(q_start), strides, B, Nq, Nk, E, Ek,
             n_head, window, n_sink, start, scale, _dtype_code(q), _stream(),
         )
     _lib.check("ncn_window_fwd", rc)
-    return y, lse
+    return y, state
 
 
-def window_bwd(q, k, v, y, dy, lse, n_head, window, n_sink, scale, start, ctxlen=None, q_start=None):
+def window_bwd(q, k, v, y, dy, state, n_head, window, n_sink, scale, start, ctxlen=None, q_start=None):
     """Returns (dq, dk, dv)."""
     lib = _lib.load()
     _check_qkv(q, k, v, n_head)
@@ -381,7 +381,7 @@ def window_bwd(q, k, v, y, dy, lse, n_head, window, n_sink, scale, start, ctxlen
         nbytes = lib.ncn_window_bwd_workspace_bytes(B, Nq, Nk, E, Ek, n_head, window, n_sink, dt)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         rc = lib.ncn_window_bwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(), dy.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(), dy.data_ptr(), state.data_ptr(), dq.data_ptr(), dk.data_ptr(),
             dv.data_ptr(), _ptr(ctxlen), _ptr(q_start), strides, ws.data_ptr(), nbytes, B, Nq, Nk, E, Ek, n_head, window, n_sink, start,
             scale, dt, _stream(),
         )

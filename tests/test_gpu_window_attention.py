@@ -1,12 +1,14 @@
 """Windowed attention with sinks: training, chunks of a prompt, padded batches, single tokens over a cache; against 64 bits."""
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
 
 import ncn_cuda_b200 as ncn
 from ncn_cuda_b200 import ops
-from tests import attention_oracle as O
+from tests import window_oracle as O
 from tests.kernels_util import kernels_of, launched
 
 pytestmark = pytest.mark.gpu
@@ -91,6 +93,33 @@ def test_padded_rows_hold_anything(dtype, d, N, ctx):
     for b, n in enumerate(ctx):
         for t in (y, dq, dk, dv):
             assert (t[b, n:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [64, 128, 20])
+@pytest.mark.parametrize("window", [300, 600, None])
+def test_padding_behind_tiles_that_all_see(dtype, d, window):
+    """Contexts that end inside a tile of queries whose other rows see whole tiles of keys."""
+    ctx = [700, 390, 513, 640]
+    q, k, v, dy = make(d, 4, 700, 700, 2, 1, d, dtype)
+    y, grads = check(q, k, v, dy, 2, window, 2, ctxlen=torch.tensor(ctx))
+    for b, n in enumerate(ctx):
+        for t in (y, *grads):
+            assert (t[b, n:] == 0).all()
+
+
+def test_backward_first_in_a_new_thread():
+    """The first CUDA call that a thread of the autograd engine makes may be a backward."""
+    code = """
+import torch, ncn_cuda_b200 as ncn
+q, k, v = (torch.randn(1, 200, n * 64, device='cuda').bfloat16().requires_grad_(True) for n in (2, 1, 1))
+y = ncn.fused_window_attention(q, k, v, 2, 50, n_sink=1)
+y.backward(torch.ones_like(y))
+torch.cuda.synchronize()
+print('done', bool(torch.isfinite(q.grad).all()))
+"""
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "done True" in out.stdout, out.stderr[-2000:]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -6,7 +6,7 @@ import torch
 
 import ncn_cuda_b200 as ncn
 from ncn_cuda_b200 import ops
-from tests import attention_oracle as O
+from tests import window_oracle as O
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16

@@ -68,7 +68,7 @@ def attention(q, k, v, n_head, window, n_sink, scale, ctxlen, start, dy=None):
     dP = dO @ V.mT
     D = (dO * Y).sum(-1, keepdim=True)
     dS = P * (dP - D)
-    e_delta = (dO.abs() * (ey + half * (Y.abs() + ey))).sum(-1, keepdim=True) + (d + 2) * u * (dO * Y).abs().sum(-1, keepdim=True)
+    e_delta = (dO.abs() * (ey + half * half * (Y.abs() + ey))).sum(-1, keepdim=True) + (d + 2) * u * (dO * Y).abs().sum(-1, keepdim=True)
     e_dp = (d + 2) * u * (dO.abs() @ V.abs().mT)
     e_ds = dS.abs() * (w32 + rounded) + P * (e_dp + e_delta) * (1 + rounded)
     acc_q, acc_k = (2 * math.sqrt(count) + 32) * u, (2 * math.sqrt(float(G * Nq)) + 32) * u
