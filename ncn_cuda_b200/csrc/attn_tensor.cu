@@ -82,15 +82,29 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
-               "l"(b), "r"(idesc), "r"((int)add)
-               : "memory");
+// One instruction's products.  Operands in shared memory are given by the low halves of their descriptors, the high half is the same for
+// all: what the issuing thread computes per instruction is two 32-bit additions.  (With whole descriptors formed for each, an instruction
+// took 90 to 130 cycles to issue, and 64 to execute: heads of 128 in windows of 2048, 4300 cycles per pair of tiles.)
+constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);  // rows of 8 x 128 bytes 1024 apart, version 1, 128-byte swizzle
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((int)add), "n"(kDescHigh)
+      : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
-               "l"(b), "r"(idesc), "r"((int)add)
-               : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((int)add), "n"(kDescHigh)
+      : "memory");
+}
+// one lane of a warp whose lanes are all here
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
 }
 __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int c, int head, int row, int b, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
@@ -104,11 +118,9 @@ __device__ __forceinline__ uint64_t now_ns() {
   return t;
 }
 
-// Operand descriptors: 128-byte swizzle, groups of 8 rows 1024 bytes apart.  Along the features ("k-major") the 16 features of an
-// instruction are 32 bytes on; along the positions ("mn-major") the 64-feature blocks are kBlockBytes apart, 16 positions 2048 on.
-__device__ __forceinline__ uint64_t desc_of(uint32_t smem, uint32_t lead) {
-  return ((smem & 0x3ffffu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
+// Operand descriptors.  Along the features ("k-major") the 16 features of an instruction are 32 bytes on; along the positions
+// ("mn-major") the 64-feature blocks are kBlockBytes apart, 16 positions 2048 bytes on.  Addresses and distances in units of 16 bytes.
+__device__ __forceinline__ uint32_t desc_low(uint32_t smem, uint32_t lead) { return ((smem & 0x3ffffu) >> 4) | ((lead >> 4) << 16); }
 template <int N, bool MN>
 __device__ __forceinline__ constexpr uint32_t idesc_of() {  // fp32 sums, bf16 operands, 128 x N
   return (1u << 4) | (1u << 7) | (1u << 10) | (MN ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kT >> 4) << 24);
@@ -116,18 +128,20 @@ __device__ __forceinline__ constexpr uint32_t idesc_of() {  // fp32 sums, bf16 o
 // D[128 x 128] = A B^T over DP features; A, B tiles
 template <int DP>
 __device__ __forceinline__ void product_scores(uint32_t d, uint32_t a, uint32_t b) {
+  const uint32_t la = desc_low(a, 16), lb = desc_low(b, 16);
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k) {
-    const uint32_t off = (k / 4) * kBlockBytes + (k % 4) * 32;
-    mma_ss(d, desc_of(a + off, 16), desc_of(b + off, 16), idesc_of<kT, false>(), k > 0);
+    const uint32_t off = ((k / 4) * kBlockBytes + (k % 4) * 32) >> 4;
+    mma_ss(d, la + off, lb + off, idesc_of<kT, false>(), k > 0);
   }
 }
 // D[128 x DP] (+)= W V over 128 positions; W bf16 in tensor memory, positions 64 .. 127 `upper` columns on; V a tile
 template <int DP>
 __device__ __forceinline__ void product_sums(uint32_t d, uint32_t w, uint32_t upper, uint32_t v, bool add) {
+  const uint32_t lv = desc_low(v, kBlockBytes);
 #pragma unroll
   for (int k = 0; k < kT / 16; ++k)
-    mma_ts(d, w + (k / 4) * upper + (k % 4) * 8, desc_of(v + k * 2048, kBlockBytes), idesc_of<DP, true>(), add || k > 0);
+    mma_ts(d, w + (k / 4) * upper + (k % 4) * 8, lv + k * (2048 >> 4), idesc_of<DP, true>(), add || k > 0);
 }
 
 // A wait that gives up: the kernel then leaves an error in the status word, and its other warps stop waiting too.
@@ -291,13 +305,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_fwd_kernel(const __gr
       }
     }
   } else if (warp == 8) {
+    const bool leader = elect_one();
     const KeyTiles kt[2] = {key_tiles<kT>(p, g, i0, i0 + kT), key_tiles<kT>(p, g, i0 + kT, i0 + 2 * kT)};
     const uint32_t qs = smem_u32(Q);
     int left[2] = {kt[0].count(), kt[1].count()};
     bool begun[2] = {false, false};
     uint32_t phase[2] = {0, 0};
     bool ok = n == 0 || (wait(q_full, 0) && ring.wait_full(wait, 0));
-    if (ok && n > 0 && lane == 0) {
+    if (ok && n > 0 && leader) {
       const uint32_t ks = smem_u32(ring.at(0));
       for (int x = 0; x < 2; ++x)
         if (kt[x].needs(all.tile(0)) && left[x]) {
@@ -317,16 +332,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_fwd_kernel(const __gr
           if (!(ok = wait(p_ready + x, phase[x]))) break;
           phase[x] ^= 1;
           tmem_after();
-          if (lane == 0) product_sums<DP>(tmem + 2 * kT + x * 128, tmem + x * kT, 32, vs, begun[x]);
+          if (leader) product_sums<DP>(tmem + 2 * kT + x * 128, tmem + x * kT, 32, vs, begun[x]);
           begun[x] = true;
-          if (--left[x] == 0 && lane == 0) mma_commit(o_full + x);
+          if (--left[x] == 0 && leader) mma_commit(o_full + x);
         }
-        if (next >= 0 && left[x] > 0 && kt[x].needs(next) && lane == 0) {
+        if (next >= 0 && left[x] > 0 && kt[x].needs(next) && leader) {
           product_scores<DP>(tmem + x * kT, qs + x * TILE, ks);
           mma_commit(s_full + x);
         }
       }
-      if (lane == 0 && ok) {
+      if (leader && ok) {
         ring.release(2 * j + 1);
         if (next >= 0) ring.release(2 * j + 2);
       }
@@ -503,13 +518,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
       }
     }
   } else if (warp == 8) {
+    const bool leader = elect_one();
     const uint32_t qs = smem_u32(Q), dys = smem_u32(dY);
     // scores of tile j into buffer j % 2
     auto scores = [&](int j) {
       if (!ring.wait_full(wait, 2 * j)) return false;
       const int k0 = kt.tile(j) * kT;
       if (k0 + kT > g.ctx && g.ctx < p.Nk) clear_rows<DP>(ring.at(2 * j), 0, g.ctx - k0);
-      if (lane == 0) {
+      if (leader) {
         product_scores<DP>(tmem + (j & 1) * kT, qs, smem_u32(ring.at(2 * j)));
         mma_commit(s_full + (j & 1));
       }
@@ -517,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
     };
     auto grads = [&](int j) {
       if (!ring.wait_full(wait, 2 * j + 1)) return false;
-      if (lane == 0) {
+      if (leader) {
         product_scores<DP>(t_dp, dys, smem_u32(ring.at(2 * j + 1)));
         mma_commit(dp_full);
         ring.release(2 * j + 1);
@@ -529,13 +545,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
       if (!(ok = wait(ds_ready, j & 1))) break;
       tmem_after();
       if (j + 1 < n && !(ok = grads(j + 1))) break;
-      if (lane == 0) {
+      if (leader) {
         product_sums<DP>(t_dq, tmem + (j & 1) * kT, 64, smem_u32(ring.at(2 * j)), j > 0);
         ring.release(2 * j);
       }
       if (j + 2 < n) ok = scores(j + 2);
     }
-    if (ok && n > 0 && lane == 0) mma_commit(done);
+    if (ok && n > 0 && leader) mma_commit(done);
   } else {
     const int half = warp / 4, r = warp % 4 * 32 + lane, qi = i0 + r, pos = g.start + qi;
     const int end = min(g.ctx, g.start + p.Nq);
@@ -711,6 +727,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
       }
     }
   } else if (warp == 8) {
+    const bool leader = elect_one();
     const uint32_t ks = smem_u32(K), vs = smem_u32(V);
     // waits for a tile of queries (or their cotangents) and clears its rows of padding
     auto arrived = [&](int load) {
@@ -721,7 +738,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
     };
     auto scores = [&](int i) {
       if (!arrived(2 * i)) return false;
-      if (lane == 0) {
+      if (leader) {
         product_scores<DP>(tmem, ks, smem_u32(ring.at(2 * i)));
         mma_commit(s_full);
       }
@@ -729,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
     };
     auto grads = [&](int i) {
       if (!arrived(2 * i + 1)) return false;
-      if (lane == 0) {
+      if (leader) {
         product_scores<DP>(t_dp, vs, smem_u32(ring.at(2 * i + 1)));
         mma_commit(dp_full);
       }
@@ -739,20 +756,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
     for (int i = 0; ok && i < n; ++i) {
       if (!(ok = wait(p_ready, i & 1))) break;
       tmem_after();
-      if (lane == 0) {
+      if (leader) {
         product_sums<DP>(t_dv, tmem, 64, smem_u32(ring.at(2 * i + 1)), i > 0);
         ring.release(2 * i + 1);
       }
       if (i + 1 < n && !(ok = scores(i + 1))) break;
       if (!(ok = wait(ds_ready, i & 1))) break;
       tmem_after();
-      if (lane == 0) {
+      if (leader) {
         product_sums<DP>(t_dk, t_dp, 64, smem_u32(ring.at(2 * i)), i > 0);
         ring.release(2 * i);
       }
       if (i + 1 < n) ok = grads(i + 1);
     }
-    if (ok && n > 0 && lane == 0) mma_commit(done);
+    if (ok && n > 0 && leader) mma_commit(done);
   } else {
     const int half = warp / 4, r = warp % 4 * 32 + lane, key = k0 + r;
     const int end = min(g.ctx, g.start + p.Nq);

@@ -74,133 +74,169 @@ __device__ __forceinline__ float team_sum(float x) {
 }
 
 // Heads of d = 16 m features with R a multiple of 16: a team of W >= d / 16 lanes per head, 16 features per lane in two chunks of 8.
-// Lane i < R / 16 holds the pairs 8 i .. 8 i + 7 (half layout: chunks i and i + R / 2 / 8; interleaved: chunks 2 i, 2 i + 1), the
-// lanes behind it two chunks of the features that are not rotated.  A CTA takes p.span positions at a time, their heads dealt out to its
-// teams (and to p.parts CTAs, where there are few positions); the next head is fetched while one is worked on.
+// Lane i < R / 16 holds the pairs 8 i .. 8 i + 7 (half layout: features 8 i .. and R / 2 + 8 i ..; interleaved: 16 i ..), the
+// lanes behind it features that are not rotated.  A CTA takes p.span positions at a time; the heads of all of them, those of the
+// queries first, are dealt out to its teams (and to p.parts CTAs, where there are few positions).  The first head is under way while
+// the sines are formed, the next one while one is worked on.
 enum Mode : int { PLAIN = 0, NORM = 1, NORM_BWD = 2 };  // PLAIN: either direction
 template <typename T, int W, int MODE>
 __global__ void __launch_bounds__(256, MODE == NORM_BWD ? 2 : 4) rotary_kernel(const __grid_constant__ RotaryParams p) {
   wait_for_inputs();
   constexpr bool norm = MODE != PLAIN, norm_bwd = MODE == NORM_BWD;
   constexpr int TEAMS = 256 / W;
-  __shared__ long long offs[4][kRotarySpan];  // of the span's positions in q, k and their cotangents
   __shared__ __align__(16) float2 table[kRotaryTable];
+  __shared__ __align__(16) float weight[norm ? 2 * 16 * W : 4];  // W <= 16: the first 2 W threads fill it
   const int lane = threadIdx.x % W, team = threadIdx.x / W, half = p.R / 2;
-  const bool active = lane < p.d / 16, turn = lane < p.R / 16;
+  const int turning = p.R / 16;
+  const bool active = lane < p.d / 16, turn = lane < turning;
   const int c0 = turn && !p.interleaved ? 8 * lane : 16 * lane, c1 = turn && !p.interleaved ? 8 * lane + half : c0 + 8;
-  const int part = blockIdx.x % p.parts;
+  const int part = blockIdx.x % p.parts, step = p.parts * TEAMS, first = part * TEAMS + team;
+  const uint32_t N = (uint32_t)p.N;
   const long long rows = (long long)p.B * p.N, stride = (long long)(gridDim.x / p.parts) * p.span;
-  float dw[2][16];  // (NORM_BWD)
+  const float inv[2] = {1.f / p.t[0].heads, p.t[1].heads ? 1.f / p.t[1].heads : 0.f}, inv_d = 1.f / p.d;
+  // position of a row of all of them (32-bit divisions where the batch allows)
+  auto split = [&](long long row, long long& b, long long& n) {
+    if (rows <= 0xffffffffll) {
+      const uint32_t q = (uint32_t)row / N;
+      b = q, n = (uint32_t)row - q * N;
+    } else {
+      b = row / p.N, n = row - b * p.N;
+    }
+  };
+  if (norm && threadIdx.x < 2 * W && active && p.t[team].heads) {  // entry j of a lane: four weights of its features
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) weight[((team * 4 + j) * W + lane) * 4 + e] = p.t[team].w[(j < 2 ? c0 : c1) + j % 2 * 4 + e];
+  }
+  float dw[2][16];  // (NORM_BWD)  of the tensor that is being worked on, of the other
 #pragma unroll
   for (int e = 0; e < 16; ++e) dw[0][e] = dw[1][e] = 0.f;
+  int of = 0;  // the former
   for (long long row0 = (long long)(blockIdx.x / p.parts) * p.span; row0 < rows; row0 += stride) {
-    const int span = (int)min((long long)p.span, rows - row0);
-    __syncthreads();
+    const int span = (int)min((long long)p.span, rows - row0), of_q = span * p.t[0].heads, count = of_q + span * p.t[1].heads;
+    const int turns = (count + step - 1) / step;  // the same for every lane: shuffles
+    Chunks<T> x_next, g_next;
+    auto place = [&](int i, int& which, int& at, int& h) {  // (i < 2^20: the product is off by less than what 0.5 leaves)
+      which = i >= of_q;
+      const int j = which ? i - of_q : i, heads = which ? p.t[1].heads : p.t[0].heads;
+      at = (int)((j + 0.5f) * (which ? inv[1] : inv[0]));
+      h = j - at * heads;
+    };
+    auto fetch = [&](int i) {
+      x_next.clear();
+      if (norm_bwd) g_next.clear();
+      if (active && i < count) {
+        int which, at, h;
+        long long b, n;
+        place(i, which, at, h);
+        split(row0 + at, b, n);
+        const RotaryTensor& t = p.t[which];
+        x_next.load(static_cast<const T*>(t.x) + b * t.sb + n * t.sn + (long long)h * p.d, c0, c1);
+        if (norm_bwd) g_next.load(static_cast<const T*>(t.dy) + b * t.gb + n * t.gn + (long long)h * p.d, c0, c1);
+      }
+    };
+    fetch(first);
+    __syncthreads();  // (the span before is done with the sines)
     for (int e = threadIdx.x; e < span * half; e += 256) {
-      const long long row = row0 + e / half, b = row / p.N, n = row - b * p.N;
-      table[e] = cos_sin(p, p.pos ? p.pos[b * p.pos_b + n] : p.start + n, e % half);
-    }
-    if (threadIdx.x < span) {
-      const long long row = row0 + threadIdx.x, b = row / p.N, n = row - b * p.N;
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        offs[which][threadIdx.x] = b * p.t[which].sb + n * p.t[which].sn;
-        offs[2 + which][threadIdx.x] = b * p.t[which].gb + n * p.t[which].gn;
-      }
+      const int at = e / half;
+      long long b, n;
+      split(row0 + at, b, n);
+      const int pair = e - at * half;
+      table[at * half + (pair % 8 / 2 * turning + pair / 8) * 2 + pair % 2] = cos_sin(p, p.pos ? p.pos[b * p.pos_b + n] : p.start + n, pair);
     }
     __syncthreads();
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const RotaryTensor& t = p.t[which];
-      if (!t.heads) continue;
-      float w[16];
-      if (norm && active) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = t.w[c0 + e], w[8 + e] = t.w[c1 + e];
+    for (int k = 0; k < turns; ++k) {
+      const int i = first + k * step;
+      const bool here = active && i < count;
+      int which, at, h;
+      place(i, which, at, h);
+      const float4* w = reinterpret_cast<const float4*>(weight) + which * 4 * W + lane;
+      float a[8], c[8], ga[8], gc[8];
+      Chunks<T>::widen(x_next.a, a);
+      Chunks<T>::widen(x_next.c, c);
+      if (norm_bwd) {
+        Chunks<T>::widen(g_next.a, ga);
+        Chunks<T>::widen(g_next.c, gc);
       }
-      const int count = span * t.heads, step = p.parts * TEAMS, first = part * TEAMS + team;
-      const int turns = (count + step - 1) / step;  // the same for every lane: shuffles
-      auto fetch = [&](int i, Chunks<T>& x, Chunks<T>& g) {
-        const bool here = active && i < count;
-        x.clear();
-        if (norm_bwd) g.clear();
-        if (here) {
-          const int at = i / t.heads, h = i - at * t.heads;
-          x.load(static_cast<const T*>(t.x) + offs[which][at] + h * p.d, c0, c1);
-          if (norm_bwd) g.load(static_cast<const T*>(t.dy) + offs[2 + which][at] + h * p.d, c0, c1);
-        }
-      };
-      Chunks<T> x_next, g_next;
-      fetch(first, x_next, g_next);
-      for (int k = 0; k < turns; ++k) {
-        const int i = first + k * step, at = i / t.heads;
-        const bool here = active && i < count;
-        float a[8], c[8], ga[8], gc[8];
-        Chunks<T>::widen(x_next.a, a);
-        Chunks<T>::widen(x_next.c, c);
-        if (norm_bwd) {
-          Chunks<T>::widen(g_next.a, ga);
-          Chunks<T>::widen(g_next.c, gc);
-        }
-        if (k + 1 < turns) fetch(i + step, x_next, g_next);
-        float r = 1.f;
-        if (norm) {
-          float sq = 0.f;
+      if (k + 1 < turns) fetch(i + step);
+      float r = 1.f;
+      if (norm) {
+        float sq = 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sq = fmaf(a[e], a[e], fmaf(c[e], c[e], sq));
-          r = rsqrtf(team_sum<W>(sq) / p.d + p.eps);
-        }
-        if (!norm_bwd) {
+        for (int e = 0; e < 8; ++e) sq = fmaf(a[e], a[e], fmaf(c[e], c[e], sq));
+        r = rsqrtf(team_sum<W>(sq) * inv_d + p.eps);
+        if (!here) r = 0.f;  // (infinite where eps is 0)
+      }
+      float wa[8], wc[8];
+      if (norm) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            ga[e] = norm ? a[e] * r * w[e] : a[e];
-            gc[e] = norm ? c[e] * r * w[8 + e] : c[e];
+        for (int e = 0; e < 8; e += 4) {
+          const float4 u = here ? w[e / 4 * W] : make_float4(0, 0, 0, 0), v = here ? w[(2 + e / 4) * W] : make_float4(0, 0, 0, 0);
+          wa[e] = u.x, wa[e + 1] = u.y, wa[e + 2] = u.z, wa[e + 3] = u.w;
+          wc[e] = v.x, wc[e + 1] = v.y, wc[e + 2] = v.z, wc[e + 3] = v.w;
+        }
+      }
+      if (!norm_bwd) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          ga[e] = norm ? a[e] * r * wa[e] : a[e];
+          gc[e] = norm ? c[e] * r * wc[e] : c[e];
+        }
+      }
+      if (turn && here) {
+        const float4* tab = reinterpret_cast<const float4*>(table + at * half) + lane;  // (entry e: the lane's pairs 2 e, 2 e + 1)
+        if (p.interleaved) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float4 s = tab[e * turning], u = tab[(2 + e) * turning];
+            float y0 = ga[4 * e], y1 = ga[4 * e + 1];
+            ga[4 * e] = y0 * s.x - y1 * s.y, ga[4 * e + 1] = y1 * s.x + y0 * s.y;
+            y0 = ga[4 * e + 2], y1 = ga[4 * e + 3];
+            ga[4 * e + 2] = y0 * s.z - y1 * s.w, ga[4 * e + 3] = y1 * s.z + y0 * s.w;
+            y0 = gc[4 * e], y1 = gc[4 * e + 1];
+            gc[4 * e] = y0 * u.x - y1 * u.y, gc[4 * e + 1] = y1 * u.x + y0 * u.y;
+            y0 = gc[4 * e + 2], y1 = gc[4 * e + 3];
+            gc[4 * e + 2] = y0 * u.z - y1 * u.w, gc[4 * e + 3] = y1 * u.z + y0 * u.w;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const float4 s = tab[e / 2 * turning];
+            float a0 = ga[e], b0 = gc[e];
+            ga[e] = a0 * s.x - b0 * s.y, gc[e] = b0 * s.x + a0 * s.y;
+            a0 = ga[e + 1], b0 = gc[e + 1];
+            ga[e + 1] = a0 * s.z - b0 * s.w, gc[e + 1] = b0 * s.z + a0 * s.w;
           }
         }
-        if (turn && here) {
-          const float4* tab = reinterpret_cast<const float4*>(table + at * half + 8 * lane);  // (two pairs each; half is a multiple of 8)
-          if (p.interleaved) {
+      }
+      if (norm_bwd) {
+        if (here && which != of) {  // from the queries to the keys, or to the next span's queries
+          of = which;
 #pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-              const float4 s = tab[e / 2], u = tab[2 + e / 2];
-              float y0 = ga[2 * e], y1 = ga[2 * e + 1];
-              ga[2 * e] = y0 * s.x - y1 * s.y, ga[2 * e + 1] = y1 * s.x + y0 * s.y;
-              y0 = ga[2 * e + 2], y1 = ga[2 * e + 3];
-              ga[2 * e + 2] = y0 * s.z - y1 * s.w, ga[2 * e + 3] = y1 * s.z + y0 * s.w;
-              y0 = gc[2 * e], y1 = gc[2 * e + 1];
-              gc[2 * e] = y0 * u.x - y1 * u.y, gc[2 * e + 1] = y1 * u.x + y0 * u.y;
-              y0 = gc[2 * e + 2], y1 = gc[2 * e + 3];
-              gc[2 * e + 2] = y0 * u.z - y1 * u.w, gc[2 * e + 3] = y1 * u.z + y0 * u.w;
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const float4 s = tab[e / 2];
-              float a0 = ga[e], b0 = gc[e];
-              ga[e] = a0 * s.x - b0 * s.y, gc[e] = b0 * s.x + a0 * s.y;
-              a0 = ga[e + 1], b0 = gc[e + 1];
-              ga[e + 1] = a0 * s.z - b0 * s.w, gc[e + 1] = b0 * s.z + a0 * s.w;
-            }
+          for (int e = 0; e < 16; ++e) {
+            const float t = dw[0][e];
+            dw[0][e] = dw[1][e];
+            dw[1][e] = t;
           }
         }
-        if (norm_bwd) {
-          float dot = 0.f;
+        float dot = 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            a[e] *= r, c[e] *= r;  // x r
-            if (here) dw[which][e] = fmaf(ga[e], a[e], dw[which][e]), dw[which][8 + e] = fmaf(gc[e], c[e], dw[which][8 + e]);
-            ga[e] *= here ? w[e] : 0.f, gc[e] *= here ? w[8 + e] : 0.f;
-            dot = fmaf(ga[e], a[e], fmaf(gc[e], c[e], dot));
-          }
-          const float mean = team_sum<W>(dot) / p.d;
+        for (int e = 0; e < 8; ++e) {
+          a[e] *= r, c[e] *= r;  // x r
+          dw[0][e] = fmaf(ga[e], a[e], dw[0][e]), dw[0][8 + e] = fmaf(gc[e], c[e], dw[0][8 + e]);  // (zeros where nothing is)
+          ga[e] *= wa[e], gc[e] *= wc[e];
+          dot = fmaf(ga[e], a[e], fmaf(gc[e], c[e], dot));
+        }
+        const float mean = team_sum<W>(dot) * inv_d;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) ga[e] = r * (ga[e] - a[e] * mean), gc[e] = r * (gc[e] - c[e] * mean);
-        }
-        if (here) {
-          T* y = static_cast<T*>(t.out) + (row0 * t.heads + i) * p.d;
-          Chunks<T>::store(y + c0, ga);
-          Chunks<T>::store(y + c1, gc);
-        }
+        for (int e = 0; e < 8; ++e) ga[e] = r * (ga[e] - a[e] * mean), gc[e] = r * (gc[e] - c[e] * mean);
+      }
+      if (here) {
+        const RotaryTensor& t = p.t[which];
+        T* y = static_cast<T*>(t.out) + ((row0 + at) * t.heads + h) * p.d;
+        Chunks<T>::store(y + c0, ga);
+        Chunks<T>::store(y + c1, gc);
       }
     }
   }
@@ -211,7 +247,10 @@ __global__ void __launch_bounds__(256, MODE == NORM_BWD ? 2 : 4) rotary_kernel(c
       __syncthreads();
       if (active) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) red[team][c0 + e] = dw[which][e], red[team][c1 + e] = dw[which][8 + e];
+        for (int e = 0; e < 8; ++e) {
+          red[team][c0 + e] = which == of ? dw[0][e] : dw[1][e];
+          red[team][c1 + e] = which == of ? dw[0][8 + e] : dw[1][8 + e];
+        }
       }
       __syncthreads();
       for (int c = threadIdx.x; c < p.d; c += 256) {
@@ -316,7 +355,9 @@ __global__ void __launch_bounds__(256) rotary_any_kernel(const RotaryParams p) {
   }
 }
 
-bool in_chunks(const RotaryParams& p) { return p.vec && p.d % 16 == 0 && p.R % 16 == 0 && p.d <= 256; }
+bool in_chunks(const RotaryParams& p) {
+  return p.vec && p.d % 16 == 0 && p.R % 16 == 0 && p.d <= 256 && p.t[0].heads < 1 << 16 && p.t[1].heads < 1 << 16;
+}
 int team_width(const RotaryParams& p) {  // lanes per head
   int w = 1;
   while (w < p.d / 16) w *= 2;
@@ -343,7 +384,7 @@ cudaError_t by_width(const RotaryParams& p, int grid, cudaStream_t st) {
 
 }  // namespace
 
-// Positions that a CTA takes at a time, CTAs that share one position's heads, and CTAs.  A span is as long as leaves 16 CTAs per SM
+// Positions that a CTA takes at a time, CTAs that share one position's heads, and CTAs.  A span is as long as leaves 8 CTAs per SM
 // (the last ones are not waited for long), its sines are formed once; with few positions their heads are spread out, a team each.  The
 // backward of a norm takes 4 CTAs per SM at most, each with several spans: every CTA leaves a row of sums behind.
 int rotary_plan(RotaryParams& p, int sms) {
@@ -352,7 +393,7 @@ int rotary_plan(RotaryParams& p, int sms) {
   p.span = p.parts = 1;
   if (in_chunks(p)) {
     const int teams = 256 / team_width(p), most = p.R ? kRotaryTable / (p.R / 2) : kRotarySpan;
-    while (2 * p.span <= most && 2 * p.span <= kRotarySpan && rows / (2 * p.span) >= 16ll * sms) p.span *= 2;
+    while (2 * p.span <= most && 2 * p.span <= kRotarySpan && rows / (2 * p.span) >= 8ll * sms) p.span *= 2;
     const long long spans = (rows + p.span - 1) / p.span;
     while (p.parts * teams < heads && spans * p.parts < 4ll * sms) ++p.parts;
     ctas = spans * p.parts;

@@ -143,6 +143,20 @@ def test_a_row_of_zeros_and_values_that_are_not_finite():
     assert torch.equal(y, clean)
 
 
+@pytest.mark.parametrize("d,N", [(64, 100), (96, 37), (33, 37)])
+def test_eps_of_zero(d, N):
+    q, k, dq, dk, wq, wk = make(5, 3, N, 3, 1, d, F32)
+    freqs, _ = ncn.rotary_frequencies(32, device="cuda")
+    leaves = [t.requires_grad_(True) for t in (q, k, wq, wk)]
+    y = ncn.fused_qk_norm_rotary(*leaves, freqs, 3, eps=0.0)
+    grads = torch.autograd.grad(y, leaves, [dq, dk])
+    for i, (x, w, g, n) in enumerate(((q, wq, dq, 3), (k, wk, dk, 1))):
+        want = O.norm_rotary(x, w, n, grid_of(None, 3, N), freqs, False, 1.0, eps=0.0, dy=g)
+        O.close(f"y{i}", y[i].detach(), want["y"])
+        O.close(f"dx{i}", grads[i], want["dx"])
+        O.close(f"dw{i}", grads[2 + i], want["dw"])
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_same_bits_captured(dtype):
     q, k, dq, dk, wq, wk = make(8, 2, 500, 4, 2, 128, dtype)
