@@ -63,7 +63,7 @@ struct KeyTiles {
   int ns = 0, t0 = 0, t1 = -1, p_lo = 0, p_hi = -1;
   __device__ __forceinline__ int count() const { return ns + max(t1 - t0 + 1, 0); }
   __device__ __forceinline__ int tile(int i) const { return i < ns ? i : t0 + i - ns; }
-  __device__ __forceinline__ bool needs(int t) const { return t < ns || (t >= t0 && t <= t1); }
+  __device__ __forceinline__ int entry(int t) const { return t < ns ? t : t - t0 + ns; }  // the list's entry that tile t is
 };
 template <int T>
 __device__ __forceinline__ KeyTiles key_tiles(const AttnParams& p, const RowGeom& g, int i0, int i1) {

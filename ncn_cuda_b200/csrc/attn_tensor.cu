@@ -14,6 +14,8 @@
 // return no sum depends on the order in which CTAs finish.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "attn_tensor.h"
 #include "ncn_common.cuh"
 
@@ -21,7 +23,8 @@ namespace ncn {
 namespace {
 
 constexpr int kT = 128;               // positions of a tile
-constexpr int kThreads = 320;         // warps 0-7 scores, 8 products, 9 TMA
+constexpr int kThreads = 352;         // backward: warps 0-7 scores, 8 products, 9 TMA, 10 padding
+constexpr int kFwdThreads = 608;      // forward: warps 0-15 scores, 16 products, 17 TMA, 18 padding
 constexpr uint32_t kBlockBytes = kT * 128;
 constexpr uint64_t kWaitLimitNs = 4000000000ull;
 
@@ -59,10 +62,29 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&x)[32
 }
 __device__ __forceinline__ void tmem_load32f(uint32_t at, float (&x)[32]) { tmem_load32(at, reinterpret_cast<uint32_t(&)[32]>(x)); }
 __device__ __forceinline__ void tmem_store32f(uint32_t at, float (&x)[32]) { tmem_store32(at, reinterpret_cast<uint32_t(&)[32]>(x)); }
+__device__ __forceinline__ void tmem_load16f(uint32_t at, float (&x)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]), "=f"(x[8]), "=f"(x[9]),
+                 "=f"(x[10]), "=f"(x[11]), "=f"(x[12]), "=f"(x[13]), "=f"(x[14]), "=f"(x[15])
+               : "r"(at));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&x)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(x[0]), "r"(x[1]), "r"(x[2]),
+      "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]), "r"(x[11]), "r"(x[12]), "r"(x[13]), "r"(x[14]),
+      "r"(x[15]), "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t (&x)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]),
+               "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(at)
+               : "memory");
+}
 // Waits for the loads; the values are tied to it, so that nothing made of them is moved ahead of the wait.
-__device__ __forceinline__ void tmem_tie(float (&x)[32]) {
+template <int N>
+__device__ __forceinline__ void tmem_tie(float (&x)[N]) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 8)
+  for (int i = 0; i < N; i += 8)
     asm volatile("" : "+f"(x[i]), "+f"(x[i + 1]), "+f"(x[i + 2]), "+f"(x[i + 3]), "+f"(x[i + 4]), "+f"(x[i + 5]), "+f"(x[i + 6]), "+f"(x[i + 7]));
 }
 template <int N>
@@ -71,7 +93,8 @@ __device__ __forceinline__ void tmem_loaded(float (&x)[N][32]) {
 #pragma unroll
   for (int c = 0; c < N; ++c) tmem_tie(x[c]);
 }
-__device__ __forceinline__ void tmem_loaded(float (&x)[32]) {
+template <int N>
+__device__ __forceinline__ void tmem_loaded(float (&x)[N]) {
   tmem_wait_load();
   tmem_tie(x);
 }
@@ -106,9 +129,9 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
   return yes != 0;
 }
-__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int c, int head, int row, int b, uint64_t* bar) {
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int c, int head, int row, int b, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-                   smem_u32(dst)),
+                   dst),
                "l"(map), "r"(c), "r"(head), "r"(row), "r"(b), "r"(smem_u32(bar))
                : "memory");
 }
@@ -135,20 +158,24 @@ __device__ __forceinline__ void product_scores(uint32_t d, uint32_t a, uint32_t 
     mma_ss(d, la + off, lb + off, idesc_of<kT, false>(), k > 0);
   }
 }
-// D[128 x DP] (+)= W V over 128 positions; W bf16 in tensor memory, positions 64 .. 127 `upper` columns on; V a tile
-template <int DP>
-__device__ __forceinline__ void product_sums(uint32_t d, uint32_t w, uint32_t upper, uint32_t v, bool add) {
+// D[128 x DP] (+)= W V over 64 of 128 positions: 0 .. 31 and 64 .. 95 (HALF 0) or the others.  W bf16 in tensor memory, two positions per
+// column, positions 64 .. 127 64 columns on; V a tile.  Two threads share a row of weights, and each hands in its first 32 before it
+// makes the others.
+template <int DP, int HALF>
+__device__ __forceinline__ void product_sums(uint32_t d, uint32_t w, uint32_t v, bool add) {
   const uint32_t lv = desc_low(v, kBlockBytes);
 #pragma unroll
-  for (int k = 0; k < kT / 16; ++k)
-    mma_ts(d, w + (k / 4) * upper + (k % 4) * 8, lv + k * (2048 >> 4), idesc_of<DP, true>(), add || k > 0);
+  for (int i = 0; i < 4; ++i) {
+    const int k = i / 2 * 4 + i % 2 + 2 * HALF;
+    mma_ts(d, w + (k / 4) * 64 + (k % 4) * 8, lv + k * (2048 >> 4), idesc_of<DP, true>(), add || i > 0 || HALF > 0);
+  }
 }
 
 // A wait that gives up: the kernel then leaves an error in the status word, and its other warps stop waiting too.
 struct Waiter {
   volatile int* stop;
   int* status;
-  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
+  __device__ __forceinline__ bool one(uint64_t* bar, uint32_t parity) const {
     for (int i = 0; i < 64; ++i)
       if (mbar_try_wait(bar, parity)) return true;
     const uint64_t begin = now_ns();
@@ -162,40 +189,92 @@ struct Waiter {
     }
     return true;
   }
+  // a whole warp: one answer for all of its lanes
+  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const { return __all_sync(~0u, one(bar, parity)); }
 };
 
-// A ring of tile slots: loads 0, 1, 2, ... in order, slot i % SLOTS
+// A ring of tile slots, and a place in it that moves on by one
 template <int SLOTS>
 struct Ring {
   uint64_t *full, *empty;
-  uint8_t* mem;
-  uint32_t bytes;
-  __device__ __forceinline__ uint8_t* at(int i) const { return mem + (i % SLOTS) * bytes; }
-  __device__ __forceinline__ bool wait_full(const Waiter& w, int i) const { return w(full + i % SLOTS, (i / SLOTS) & 1); }
-  __device__ __forceinline__ bool wait_empty(const Waiter& w, int i) const { return i < SLOTS || w(empty + i % SLOTS, (i / SLOTS + 1) & 1); }
-  __device__ __forceinline__ void release(int i) const { mma_commit(empty + i % SLOTS); }
+  uint32_t mem, bytes;
+  struct Place {
+    int slot = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next() {
+      if (++slot == SLOTS) slot = 0, parity ^= 1;
+    }
+  };
+  __device__ __forceinline__ Place place(int i) const {
+    Place p;
+    p.slot = i % SLOTS;
+    p.parity = (i / SLOTS) & 1;
+    return p;
+  }
+  __device__ __forceinline__ uint32_t at(const Place& p) const { return mem + p.slot * bytes; }
+  __device__ __forceinline__ uint64_t* arrived(const Place& p) const { return full + p.slot; }
+  __device__ __forceinline__ bool wait_full(const Waiter& w, const Place& p) const { return w.one(full + p.slot, p.parity); }
+  __device__ __forceinline__ bool wait_empty(const Waiter& w, const Place& p) const { return w.one(empty + p.slot, p.parity ^ 1); }  // (free at first)
+  __device__ __forceinline__ void release(const Place& p) const { mma_commit(empty + p.slot); }
 };
 
 template <int DP>
-__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, int head, int row, int b, uint64_t* bar) {
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int head, int row, int b, uint64_t* bar) {
 #pragma unroll
   for (int c = 0; c < DP / 64; ++c) tma_load(dst + c * kBlockBytes, map, c * 64, head, row, b, bar);
 }
-// Clears the rows outside [lo, hi) of a tile that has arrived; a whole warp.
+// Clears the rows outside [lo, hi) of a tile; a whole warp.  The thread that issues the products has seen the tile arrive, asks for it
+// (`go`) and waits (`cleared`) before it goes on: one tile at a time, so neither can be a phase ahead.
 template <int DP>
-__device__ __forceinline__ void clear_rows(uint8_t* tile, int lo, int hi) {
+__device__ __forceinline__ void clear_rows(uint32_t tile, int lo, int hi, uint64_t* cleared) {
   const int lane = threadIdx.x % 32;
   for (int e = lane; e < kT * DP / 8; e += 32) {
     const int r = e % (kT * 8) / 8;
-    if (r < lo || r >= hi) *reinterpret_cast<uint4*>(tile + e / (kT * 8) * kBlockBytes + e % (kT * 8) * 16) = make_uint4(0, 0, 0, 0);
+    if (r < lo || r >= hi)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + e / (kT * 8) * kBlockBytes + e % (kT * 8) * 16), "r"(0) : "memory");
   }
   fence_proxy_async();
   __syncwarp();
+  if (lane == 0) mbar_arrive(cleared);
+}
+__device__ __forceinline__ bool have_cleared(const Waiter& wait, uint64_t* go, uint64_t* cleared, uint32_t phase) {
+  mbar_arrive(go);
+  return wait.one(cleared, phase);
 }
 
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Exponentials.  The special-function pipe gives 16 per SM and cycle, 1024 cycles per tile of 128 x 128, as long as both products of heads
+// of 128 take; so some pairs (kOnFma of 8) are computed on the FMA pipe instead, two at a time: 2^x = 2^n 2^f, n the nearest whole number,
+// |f| <= 1/2, 2^f by the polynomial of degree 4 of least relative error (Remez exchange; 2.6e-6 = 2^-18.6, a thousandth of the weights'
+// rounding to bf16).  Below 2^-120 the result is 2^-120 rather than less, so masked scores (-inf) go to the other pipe: tiles with a mask
+// do entirely.  NaN stays NaN.
+constexpr int kOnFma = 3;
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-120.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-120.f));
+  constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it leaves the nearest whole number in the low bits
+  const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
+  const float2 n = __fadd2_rn(t, make_float2(-kRound, -kRound));
+  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+  float2 p = __ffma2_rn(f, make_float2(0.009570101911f, 0.009570101911f), make_float2(0.05591786032f, 0.05591786032f));
+  p = __ffma2_rn(p, f, make_float2(0.2402474483f, 0.2402474483f));
+  p = __ffma2_rn(p, f, make_float2(0.6931218147f, 0.6931218147f));
+  p = __ffma2_rn(p, f, make_float2(0.9999992614f, 0.9999992614f));
+  const float2 two_n = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000));
+  return __fmul2_rn(p, two_n);
+}
+// s[e] = 2^(s[e] * scale + bias)
+template <bool MIX>
+__device__ __forceinline__ void exp2_pair(float& a, float& b, float2 scale, float2 bias, int pair) {
+  float2 x = __ffma2_rn(make_float2(a, b), scale, bias);
+  if (MIX && pair % 8 < kOnFma)
+    x = exp2_fma(x);
+  else
+    x = make_float2(ex2(x.x), ex2(x.y));
+  a = x.x, b = x.y;
 }
 // what the rounding in store_row takes off, rounded itself
 __device__ __forceinline__ void store_rest(__nv_bfloat16* row, const float (&x)[32], float f, int c0, int d) {
@@ -217,6 +296,15 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* row, const float (&x)[3
                                                            pack(x[e + 4] * f, x[e + 5] * f), pack(x[e + 6] * f, x[e + 7] * f));
 }
 
+// After a wait that gave up: what is on its way to the last loads' slots arrives before the memory is given up.
+template <int SLOTS>
+__device__ __forceinline__ void settle(const Ring<SLOTS>& ring, int loads) {
+  for (int e = loads > SLOTS ? loads - SLOTS : 0; e < loads; ++e) {
+    const auto at = ring.place(e);
+    mbar_wait_bounded(ring.full + at.slot, at.parity, 1u << 16);
+  }
+}
+
 struct Maps {
   CUtensorMap q, k, v, dy;
 };
@@ -236,8 +324,11 @@ __device__ __forceinline__ Columns columns_of(const AttnParams& p, int pos, int 
 __device__ __forceinline__ bool visible(const Columns& c, int x) { return x < c.hi && (x >= c.lo || x < c.sink); }
 
 // ------------------------------------------------------------------ forward
-// Two tiles of 128 queries per CTA, four warps each: while one's scores are exponentiated, the other's products run.  A thread owns a
-// row.  Tensor memory: scores of both (128 columns each; the weights over them), sums of both (DP each).
+// Two tiles of 128 queries per CTA, eight warps each: while one's scores are exponentiated, the other's products run.  Two threads own a
+// row, 64 keys each (with one, the single warp that a tile then has on each of the SM's four parts waits for its own instructions: 2000
+// cycles per tile, and 3400 per pair of tiles where heads of 128 need 2048 for their products).  They agree on the largest score through
+// shared memory, read the scores twice from tensor memory rather than keep them, and rescale and write half of the features each.
+// Tensor memory: scores of both tiles (128 columns each; the weights over them), sums of both (DP each).
 // The running maximum is followed lazily: sums are rescaled only where it has grown by 2^8 since, which bf16 weights and
 // fp32 sums carry without loss.
 constexpr float kLazy = 8.f;
@@ -245,29 +336,30 @@ constexpr float kLazy = 8.f;
 template <int DP, int SLOTS>
 struct FwdSmem {
   static constexpr uint32_t tile = kT * DP * 2;
-  static constexpr uint32_t bytes = (2 + SLOTS) * tile + 256;
+  static constexpr uint32_t bytes = (2 + SLOTS) * tile + 2048 + 512;
 };
 
 template <int DP, int SLOTS>
-__global__ void __launch_bounds__(kThreads, 1) attn_tensor_fwd_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ Maps maps) {
   constexpr uint32_t TILE = FwdSmem<DP, SLOTS>::tile;
   extern __shared__ __align__(1024) uint8_t base[];
   if (smem_u32(base) & 1023) {  // (the swizzle goes by the address)
     if (threadIdx.x == 0 && p.status) atomicExch(p.status, (int)DEV_WAIT_TIMEOUT);
     return;
   }
-  uint8_t* const Q = base;
-  uint64_t* const bars = reinterpret_cast<uint64_t*>(base + (2 + SLOTS) * TILE);
-  uint64_t *const q_full = bars, *const s_full = bars + 1, *const p_ready = bars + 3, *const o_full = bars + 5;
-  const Ring<SLOTS> ring{bars + 7, bars + 7 + SLOTS, base + 2 * TILE, TILE};
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 7 + 2 * SLOTS);
+  const uint32_t qs = smem_u32(base);
+  float* const shared_row = reinterpret_cast<float*>(base + (2 + SLOTS) * TILE);  // [tile][half][row]
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(shared_row + 4 * kT);
+  uint64_t *const q_full = bars, *const s_full = bars + 1, *const p_half = bars + 3, *const p_ready = bars + 5, *const o_full = bars + 7, *const go = bars + 9, *const cleared = bars + 10;
+  const Ring<SLOTS> ring{bars + 11, bars + 11 + SLOTS, qs + 2 * TILE, TILE};
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 11 + 2 * SLOTS);
   volatile int* const stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
-  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  if (warp == 16) tmem_alloc(tmem_slot, 512);
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    for (int x = 0; x < 2; ++x) mbar_init(s_full + x, 1), mbar_init(p_ready + x, kT), mbar_init(o_full + x, 1);
+    mbar_init(q_full, 1), mbar_init(go, 1), mbar_init(cleared, 1);
+    for (int x = 0; x < 2; ++x) mbar_init(s_full + x, 1), mbar_init(p_half + x, 2 * kT), mbar_init(p_ready + x, 2 * kT), mbar_init(o_full + x, 1);
     for (int i = 0; i < SLOTS; ++i) mbar_init(ring.full + i, 1), mbar_init(ring.empty + i, 1);
     fence_mbar_init();
     *stop = 0;
@@ -284,109 +376,137 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_fwd_kernel(const __gr
   const KeyTiles all = key_tiles<kT>(p, g, i0, i0 + 2 * kT);
   const int n = all.count();
   const Waiter wait{stop, p.status};
+  // the last tile may end in padding, whose values would meet weights of zero
+  const bool clear = n > 0 && g.ctx < p.Nk && all.tile(n - 1) * kT + kT > g.ctx;
 
-  if (warp == 9) {
-    if (lane == 0 && n > 0) {
+  if (warp == 17) {
+    if (n > 0 && elect_one()) {
       const int queries = i0 + kT < p.Nq ? 2 : 1;
       mbar_expect_tx(q_full, queries * TILE);
-      for (int x = 0; x < queries; ++x) load_tile<DP>(Q + x * TILE, &maps.q, h, i0 + x * kT, b, q_full);
-      bool ok = true;
-      int i = 0;
-      for (; i < 2 * n && ok; ++i) {
-        ok = ring.wait_empty(wait, i);
-        if (!ok) break;
-        uint64_t* const bar = ring.full + i % SLOTS;
-        mbar_expect_tx(bar, TILE);
-        load_tile<DP>(ring.at(i), i % 2 ? &maps.v : &maps.k, hk, all.tile(i / 2) * kT, b, bar);
-      }
-      if (!ok) {  // what is on its way arrives before the memory is given up
-        mbar_wait_bounded(q_full, 0);
-        for (int e = i > SLOTS ? i - SLOTS : 0; e < i; ++e) mbar_wait_bounded(ring.full + e % SLOTS, (e / SLOTS) & 1);
-      }
-    }
-  } else if (warp == 8) {
-    const bool leader = elect_one();
-    const KeyTiles kt[2] = {key_tiles<kT>(p, g, i0, i0 + kT), key_tiles<kT>(p, g, i0 + kT, i0 + 2 * kT)};
-    const uint32_t qs = smem_u32(Q);
-    int left[2] = {kt[0].count(), kt[1].count()};
-    bool begun[2] = {false, false};
-    uint32_t phase[2] = {0, 0};
-    bool ok = n == 0 || (wait(q_full, 0) && ring.wait_full(wait, 0));
-    if (ok && n > 0 && leader) {
-      const uint32_t ks = smem_u32(ring.at(0));
-      for (int x = 0; x < 2; ++x)
-        if (kt[x].needs(all.tile(0)) && left[x]) {
-          product_scores<DP>(tmem + x * kT, qs + x * TILE, ks);
-          mma_commit(s_full + x);
+      for (int x = 0; x < queries; ++x) load_tile<DP>(qs + x * TILE, &maps.q, h, i0 + x * kT, b, q_full);
+      typename Ring<SLOTS>::Place to;
+      for (int i = 0; i < 2 * n; ++i) {
+        if (!ring.wait_empty(wait, to)) {
+          mbar_wait_bounded(q_full, 0, 1u << 16);
+          settle(ring, i);
+          break;
         }
-      ring.release(0);
+        mbar_expect_tx(ring.arrived(to), TILE);
+        load_tile<DP>(ring.at(to), i & 1 ? &maps.v : &maps.k, hk, all.tile(i >> 1) * kT, b, ring.arrived(to));
+        to.next();
+      }
     }
-    for (int j = 0; ok && j < n; ++j) {
-      const int t = all.tile(j), next = j + 1 < n ? all.tile(j + 1) : -1;
-      if (!(ok = ring.wait_full(wait, 2 * j + 1) && (next < 0 || ring.wait_full(wait, 2 * j + 2)))) break;
-      if (t * kT + kT > g.ctx && g.ctx < p.Nk) clear_rows<DP>(ring.at(2 * j + 1), 0, g.ctx - t * kT);
-      const uint32_t vs = smem_u32(ring.at(2 * j + 1)), ks = smem_u32(ring.at(2 * j + 2));
+  } else if (warp == 18) {
+    if (clear && wait(go, 0)) clear_rows<DP>(ring.at(ring.place(2 * n - 1)), 0, g.ctx - all.tile(n - 1) * kT, cleared);
+  } else if (warp == 16) {
+    if (n > 0 && elect_one()) {
+      // what tile x needs of the list: entries below ns, and lo .. hi
+      int ns[2], lo[2], hi[2], last[2];
       for (int x = 0; x < 2; ++x) {
-        const bool mine = left[x] > 0 && kt[x].needs(t);
-        if (mine) {
-          if (!(ok = wait(p_ready + x, phase[x]))) break;
-          phase[x] ^= 1;
-          tmem_after();
-          if (leader) product_sums<DP>(tmem + 2 * kT + x * 128, tmem + x * kT, 32, vs, begun[x]);
-          begun[x] = true;
-          if (--left[x] == 0 && leader) mma_commit(o_full + x);
-        }
-        if (next >= 0 && left[x] > 0 && kt[x].needs(next) && leader) {
-          product_scores<DP>(tmem + x * kT, qs + x * TILE, ks);
-          mma_commit(s_full + x);
-        }
+        const KeyTiles kt = key_tiles<kT>(p, g, i0 + x * kT, i0 + x * kT + kT);
+        ns[x] = kt.ns;
+        lo[x] = all.entry(kt.t0);
+        hi[x] = kt.t1 >= kt.t0 ? all.entry(kt.t1) : -1;
+        last[x] = max(ns[x] - 1, hi[x]);
       }
-      if (leader && ok) {
-        ring.release(2 * j + 1);
-        if (next >= 0) ring.release(2 * j + 2);
+      uint32_t phase[2] = {0, 0};
+      bool begun[2] = {false, false};
+      typename Ring<SLOTS>::Place k_at, v_at;
+      v_at.next();
+      auto needs = [&](int x, int j) { return j < ns[x] || (j >= lo[x] && j <= hi[x]); };
+      auto scores = [&](int x) {
+        product_scores<DP>(tmem + x * kT, qs + x * TILE, ring.at(k_at));
+        mma_commit(s_full + x);
+      };
+      bool ok = wait.one(q_full, 0) && ring.wait_full(wait, k_at);
+      if (ok) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (needs(x, 0)) scores(x);
+        ring.release(k_at);
+        k_at.next(), k_at.next();
+      }
+#pragma unroll 1
+      for (int j = 0; ok && j < n; ++j) {
+        ok = ring.wait_full(wait, v_at) && (j + 1 < n ? ring.wait_full(wait, k_at) : !clear || have_cleared(wait, go, cleared, 0));
+        if (!ok) break;
+        const uint32_t vs = ring.at(v_at);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (needs(x, j)) {
+            if (!(ok = wait.one(p_half + x, phase[x]))) break;
+            tmem_after();
+            product_sums<DP, 0>(tmem + 2 * kT + x * 128, tmem + x * kT, vs, begun[x]);
+            if (!(ok = wait.one(p_ready + x, phase[x]))) break;
+            tmem_after();
+            product_sums<DP, 1>(tmem + 2 * kT + x * 128, tmem + x * kT, vs, true);
+            phase[x] ^= 1;
+            begun[x] = true;
+            if (j == last[x]) mma_commit(o_full + x);
+          }
+          if (j + 1 < n && needs(x, j + 1)) scores(x);
+        }
+        if (!ok) break;
+        ring.release(v_at);
+        v_at.next(), v_at.next();
+        if (j + 1 < n) {
+          ring.release(k_at);
+          k_at.next(), k_at.next();
+        }
       }
     }
+    __syncwarp();
   } else {
-    const int x = warp / 4, r = threadIdx.x % kT, qi = i0 + x * kT + r, pos = g.start + qi;
+    const int x = warp / 8, half = warp / 4 % 2, r = threadIdx.x % kT, qi = i0 + x * kT + r, pos = g.start + qi;
     const int end = min(g.ctx, g.start + p.Nq);
     const KeyTiles kt = key_tiles<kT>(p, g, i0 + x * kT, i0 + x * kT + kT);
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
-    const uint32_t ts = tmem + x * kT + lanes, to = tmem + 2 * kT + x * 128 + lanes;
+    const uint32_t ts = tmem + x * kT + half * 64 + lanes, to = tmem + 2 * kT + x * 128 + lanes;
     const int p_lo = g.start + i0 + x * kT, p_hi = p_lo + kT - 1;  // positions of the tile, padding included
-    const int mine = kt.count();
+    const int mine = kt.count(), pair_bar = 1 + x * 4 + warp % 4;  // the barrier of the two warps that share rows
+    float *const my_row = shared_row + (2 * x + half) * kT + r, *const other_row = shared_row + (2 * x + 1 - half) * kT + r;
+    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
     float ref = -INFINITY, l = 0.f;  // (ref in log2 units)
     bool ok = true;
     for (int j = 0; j < mine; ++j) {
+      const int k0 = kt.tile(j) * kT + half * 64;
+      const bool whole = k0 + 63 <= p_lo && k0 + 64 <= g.ctx && (k0 > p_hi - p.window || k0 + 64 <= p.n_sink);
+      const Columns col = columns_of(p, pos, end, k0);
       if (!(ok = wait(s_full + x, j & 1))) break;
       tmem_after();
-      const int k0 = kt.tile(j) * kT;
-      float s[4][32];
+      float top;
+      {
+        float s[2][32];
+        tmem_load32f(ts, s[0]);
+        tmem_load32f(ts + 32, s[1]);
+        tmem_loaded(s);
+        if (!whole) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_load32f(ts + 32 * c, s[c]);
-      tmem_loaded(s);
-      const bool whole = k0 + kT - 1 <= p_lo && k0 + kT <= g.ctx && (k0 > p_hi - p.window || k0 + kT <= p.n_sink);
-      if (!whole) {
-        const Columns col = columns_of(p, pos, end, k0);
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+            for (int e = 0; e < 32; ++e)
+              if (!visible(col, 32 * c + e)) s[c][e] = -INFINITY;
+        }
+        float mx[4];
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!visible(col, 32 * c + e)) s[c][e] = -INFINITY;
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            mx[2 * c + u] = fmaxf(s[c][u], s[c][u + 2]);
+#pragma unroll
+            for (int e = u + 4; e < 32; e += 4) mx[2 * c + u] = fmaxf(fmaxf(mx[2 * c + u], s[c][e]), s[c][e + 2]);
+          }
+        top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
       }
-      float mx[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mx[c] = s[c][0];
-#pragma unroll
-        for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], s[c][e]);
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+      *my_row = top;
+      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+      top = fmaxf(top, *other_row);  // (written again only when both have handed in this tile's weights)
       const bool grown = top > ref + kLazy;  // (also the first score of a row: ref is -inf)
       if (__any_sync(~0u, grown && ref != -INFINITY)) {  // the sums that the products so far have left: they are done, the scores came after them
         const float keep = grown ? ex2(ref - top) : 1.f;
         l *= keep;
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
+        for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
           float o[32];
           tmem_load32f(to + c, o);
           tmem_loaded(o);
@@ -397,36 +517,56 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_fwd_kernel(const __gr
       }
       if (grown) ref = top;
       const float bias = ref == -INFINITY ? 0.f : ref;
-      float sum[4];
+      const float2 bias2 = make_float2(-bias, -bias);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      auto weights = [&](auto mix) {
+        float s[2][16];
+        tmem_load16f(ts, s[0]);
 #pragma unroll
-      for (int c = 0; c < 4; c += 2) {
-        uint32_t w[32];
+        for (int c = 0; c < 4; ++c) {  // the weights of scores 16 c .. lie over scores 8 c .., which have been used
+          tmem_loaded(s[c % 2]);
+          if (c < 3) tmem_load16f(ts + 16 * (c + 1), s[(c + 1) % 2]);
+          uint32_t w[8];
+          float(&t)[16] = s[c % 2];
+          if (!decltype(mix)::value) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          sum[c + u] = 0.f;
+            for (int e = 0; e < 16; ++e)
+              if (!visible(col, 16 * c + e)) t[e] = -INFINITY;
+          }
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float a = ex2(fmaf(s[c + u][e], p.scale_log2, -bias)), bb = ex2(fmaf(s[c + u][e + 1], p.scale_log2, -bias));
-            sum[c + u] += a + bb;
-            w[16 * u + e / 2] = pack(a, bb);
+          for (int e = 0; e < 16; e += 2) {
+            exp2_pair<decltype(mix)::value>(t[e], t[e + 1], scale2, bias2, e / 2);
+            sum[e / 2 % 2] = __fadd2_rn(sum[e / 2 % 2], make_float2(t[e], t[e + 1]));
+            w[e / 2] = pack(t[e], t[e + 1]);
+          }
+          tmem_store8(ts + 8 * c, w);
+          if (c == 1) {
+            tmem_stored();
+            tmem_before();
+            mbar_arrive(p_half + x);
           }
         }
-        tmem_store32(ts + 16 * c, w);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      };
+      if (whole) weights(std::true_type());
+      else weights(std::false_type());
+      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       tmem_stored();
       tmem_before();
       mbar_arrive(p_ready + x);
     }
     if (mine > 0 && ok) ok = wait(o_full + x, 0);
     tmem_after();
+    if (!ok) asm volatile("bar.arrive %0, 64;" ::"r"(pair_bar) : "memory");  // given up: the warp that shares the rows does not wait for this one
     if (ok) {
+      *my_row = l;
+      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+      l += *other_row;
       // (padding between rows that see a whole tile has had no mask)
       const bool some = mine > 0 && pos >= 0 && pos < end && !(l == 0.f);
       const float inv = some ? 1.f / l : 0.f;
       const long long row = ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
 #pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
+      for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
         float o[32];
         if (mine > 0) {
           tmem_load32f(to + c, o);
@@ -441,12 +581,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_fwd_kernel(const __gr
           if (p.rest) store_rest(p.rest + row, o, inv, c, p.d);
         }
       }
-      if (p.lse && qi < p.Nq) p.lse[((long long)b * p.H + h) * p.Nqp + qi] = some ? ref + log2f(l) : INFINITY;
+      if (p.lse && half == 0 && qi < p.Nq) p.lse[((long long)b * p.H + h) * p.Nqp + qi] = some ? ref + log2f(l) : INFINITY;
     }
     tmem_before();
   }
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tmem_after();
     tmem_free(tmem, 512);
   }
@@ -458,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_fwd_kernel(const __gr
 template <int DP, int SLOTS>
 struct BwdSmem {
   static constexpr uint32_t tile = kT * DP * 2;
-  static constexpr uint32_t bytes = (2 + SLOTS) * tile + 2048 + 256;
+  static constexpr uint32_t bytes = (2 + SLOTS) * tile + 2048 + 512;
 };
 
 template <int DP, int SLOTS>
@@ -469,18 +609,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
     if (threadIdx.x == 0 && p.status) atomicExch(p.status, (int)DEV_WAIT_TIMEOUT);
     return;
   }
-  uint8_t *const Q = base, *const dY = base + TILE;
+  const uint32_t qs = smem_u32(base), dys = qs + TILE;
   float* const halves = reinterpret_cast<float*>(base + (2 + SLOTS) * TILE);  // [2][128]
   uint64_t* const bars = reinterpret_cast<uint64_t*>(halves + 512);
-  uint64_t *const q_full = bars, *const s_full = bars + 1, *const dp_full = bars + 3, *const ds_ready = bars + 4, *const done = bars + 5;
-  const Ring<SLOTS> ring{bars + 6, bars + 6 + SLOTS, base + 2 * TILE, TILE};
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 6 + 2 * SLOTS);
+  uint64_t *const q_full = bars, *const s_full = bars + 1, *const dp_full = bars + 3, *const ds_half = bars + 4, *const ds_ready = bars + 5, *const done = bars + 6,
+           *const go = bars + 7, *const cleared = bars + 8;
+  const Ring<SLOTS> ring{bars + 9, bars + 9 + SLOTS, qs + 2 * TILE, TILE};
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 9 + 2 * SLOTS);
   volatile int* const stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (warp == 8) tmem_alloc(tmem_slot, 512);
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1), mbar_init(s_full, 1), mbar_init(s_full + 1, 1), mbar_init(dp_full, 1), mbar_init(ds_ready, 256), mbar_init(done, 1);
+    mbar_init(q_full, 1), mbar_init(s_full, 1), mbar_init(s_full + 1, 1), mbar_init(dp_full, 1), mbar_init(ds_half, 256), mbar_init(ds_ready, 256);
+    mbar_init(done, 1), mbar_init(go, 1), mbar_init(cleared, 1);
     for (int i = 0; i < SLOTS; ++i) mbar_init(ring.full + i, 1), mbar_init(ring.empty + i, 1);
     fence_mbar_init();
     *stop = 0;
@@ -498,60 +640,65 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
   const int n = kt.count();
   const Waiter wait{stop, p.status};
 
+  // the last tile may end in padding: keys that would meet a dS of zero
+  const bool clear = n > 0 && g.ctx < p.Nk && kt.tile(n - 1) * kT + kT > g.ctx;
+
   if (warp == 9) {
-    if (lane == 0 && n > 0) {
+    if (n > 0 && elect_one()) {
       mbar_expect_tx(q_full, 2 * TILE);
-      load_tile<DP>(Q, &maps.q, h, i0, b, q_full);
-      load_tile<DP>(dY, &maps.dy, h, i0, b, q_full);
-      bool ok = true;
-      int i = 0;
-      for (; i < 2 * n && ok; ++i) {
-        ok = ring.wait_empty(wait, i);
-        if (!ok) break;
-        uint64_t* const bar = ring.full + i % SLOTS;
-        mbar_expect_tx(bar, TILE);
-        load_tile<DP>(ring.at(i), i % 2 ? &maps.v : &maps.k, hk, kt.tile(i / 2) * kT, b, bar);
-      }
-      if (!ok) {
-        mbar_wait_bounded(q_full, 0);
-        for (int e = i > SLOTS ? i - SLOTS : 0; e < i; ++e) mbar_wait_bounded(ring.full + e % SLOTS, (e / SLOTS) & 1);
+      load_tile<DP>(qs, &maps.q, h, i0, b, q_full);
+      load_tile<DP>(dys, &maps.dy, h, i0, b, q_full);
+      typename Ring<SLOTS>::Place to;
+      for (int i = 0; i < 2 * n; ++i) {
+        if (!ring.wait_empty(wait, to)) {
+          mbar_wait_bounded(q_full, 0, 1u << 16);
+          settle(ring, i);
+          break;
+        }
+        mbar_expect_tx(ring.arrived(to), TILE);
+        load_tile<DP>(ring.at(to), i & 1 ? &maps.v : &maps.k, hk, kt.tile(i >> 1) * kT, b, ring.arrived(to));
+        to.next();
       }
     }
+  } else if (warp == 10) {
+    if (clear && wait(go, 0)) clear_rows<DP>(ring.at(ring.place(2 * n - 2)), 0, g.ctx - kt.tile(n - 1) * kT, cleared);
   } else if (warp == 8) {
-    const bool leader = elect_one();
-    const uint32_t qs = smem_u32(Q), dys = smem_u32(dY);
-    // scores of tile j into buffer j % 2
-    auto scores = [&](int j) {
-      if (!ring.wait_full(wait, 2 * j)) return false;
-      const int k0 = kt.tile(j) * kT;
-      if (k0 + kT > g.ctx && g.ctx < p.Nk) clear_rows<DP>(ring.at(2 * j), 0, g.ctx - k0);
-      if (leader) {
-        product_scores<DP>(tmem + (j & 1) * kT, qs, smem_u32(ring.at(2 * j)));
+    if (n > 0 && elect_one()) {
+      typename Ring<SLOTS>::Place k_at, v_at, old_k;  // of the next scores, the next dP, the next dS
+      v_at.next();
+      auto scores = [&](int j) {  // of tile j into buffer j % 2
+        if (!(ring.wait_full(wait, k_at) && (j + 1 < n || !clear || have_cleared(wait, go, cleared, 0)))) return false;
+        product_scores<DP>(tmem + (j & 1) * kT, qs, ring.at(k_at));
         mma_commit(s_full + (j & 1));
-      }
-      return true;
-    };
-    auto grads = [&](int j) {
-      if (!ring.wait_full(wait, 2 * j + 1)) return false;
-      if (leader) {
-        product_scores<DP>(t_dp, dys, smem_u32(ring.at(2 * j + 1)));
+        k_at.next(), k_at.next();
+        return true;
+      };
+      auto grads = [&]() {
+        if (!ring.wait_full(wait, v_at)) return false;
+        product_scores<DP>(t_dp, dys, ring.at(v_at));
         mma_commit(dp_full);
-        ring.release(2 * j + 1);
+        ring.release(v_at);
+        v_at.next(), v_at.next();
+        return true;
+      };
+      bool ok = wait.one(q_full, 0) && scores(0) && grads() && (n < 2 || scores(1));
+#pragma unroll 1
+      for (int j = 0; ok && j < n; ++j) {
+        const uint32_t ds = tmem + (j & 1) * kT, ks = ring.at(old_k);
+        if (!(ok = wait.one(ds_half, j & 1))) break;
+        tmem_after();
+        product_sums<DP, 0>(t_dq, ds, ks, j > 0);
+        if (!(ok = wait.one(ds_ready, j & 1))) break;
+        tmem_after();
+        if (j + 1 < n && !(ok = grads())) break;
+        product_sums<DP, 1>(t_dq, ds, ks, true);
+        ring.release(old_k);
+        old_k.next(), old_k.next();
+        if (j + 2 < n) ok = scores(j + 2);
       }
-      return true;
-    };
-    bool ok = n == 0 || (wait(q_full, 0) && scores(0) && grads(0) && (n < 2 || scores(1)));
-    for (int j = 0; ok && j < n; ++j) {
-      if (!(ok = wait(ds_ready, j & 1))) break;
-      tmem_after();
-      if (j + 1 < n && !(ok = grads(j + 1))) break;
-      if (leader) {
-        product_sums<DP>(t_dq, tmem + (j & 1) * kT, 64, smem_u32(ring.at(2 * j)), j > 0);
-        ring.release(2 * j);
-      }
-      if (j + 2 < n) ok = scores(j + 2);
+      if (ok) mma_commit(done);
     }
-    if (ok && n > 0 && leader) mma_commit(done);
+    __syncwarp();
   } else {
     const int half = warp / 4, r = warp % 4 * 32 + lane, qi = i0 + r, pos = g.start + qi;
     const int end = min(g.ctx, g.start + p.Nq);
@@ -593,32 +740,40 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
       tmem_loaded(s);
       const bool whole = k0 + 63 <= p_lo && p_hi < end && k0 + 64 <= g.ctx && (k0 > p_hi - p.window || k0 + 64 <= p.n_sink);
       const Columns col = columns_of(p, pos, end, k0);
+      const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), bias2 = make_float2(-lse, -lse);
+      auto weights = [&](auto mix) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int e = 0; e < 32; ++e) s[c][e] = ex2(fmaf(s[c][e], p.scale_log2, -lse));
+          for (int e = 0; e < 32; e += 2) exp2_pair<decltype(mix)::value>(s[c][e], s[c][e + 1], scale2, bias2, e / 2);
+      };
+      if (whole) weights(std::true_type());
+      else weights(std::false_type());
       if (!(ok = wait(dp_full, j & 1))) break;
       tmem_after();
-      uint32_t w[32];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float dp[32];
+        uint32_t w[16];
         tmem_load32f(t_dp + half * 64 + 32 * c + lanes, dp);
         tmem_loaded(dp);
         if (whole) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) dp[e] = s[c][e] * (dp[e] - delta);
+          for (int e = 0; e < 32; e += 2) {
+            const float2 t = __fmul2_rn(make_float2(s[c][e], s[c][e + 1]), __fadd2_rn(make_float2(dp[e], dp[e + 1]), make_float2(-delta, -delta)));
+            dp[e] = t.x, dp[e + 1] = t.y;
+          }
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) dp[e] = visible(col, 32 * c + e) ? s[c][e] * (dp[e] - delta) : 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) w[16 * c + e / 2] = pack(dp[e], dp[e + 1]);
+        for (int e = 0; e < 32; e += 2) w[e / 2] = pack(dp[e], dp[e + 1]);
+        tmem_store16(ts + 16 * c, w);
+        tmem_stored();
+        tmem_before();
+        mbar_arrive(c ? ds_ready : ds_half);
       }
-      tmem_store32(ts, w);
-      tmem_stored();
-      tmem_before();
-      mbar_arrive(ds_ready);
     }
     if (n > 0 && ok) ok = wait(done, 0);
     tmem_after();
@@ -660,19 +815,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
     if (threadIdx.x == 0 && p.status) atomicExch(p.status, (int)DEV_WAIT_TIMEOUT);
     return;
   }
-  uint8_t *const K = base, *const V = base + TILE;
+  const uint32_t ks = smem_u32(base), vs = ks + TILE;
   float* const stats = reinterpret_cast<float*>(base + (2 + SLOTS) * TILE);  // [STATS][2][128]
   uint64_t* const bars = reinterpret_cast<uint64_t*>(stats + STATS * 2 * kT);
-  uint64_t *const kv_full = bars, *const s_full = bars + 1, *const dp_full = bars + 2, *const p_ready = bars + 3, *const ds_ready = bars + 4,
-           *const done = bars + 5, *const st_full = bars + 6, *const st_empty = bars + 6 + STATS;
-  const Ring<SLOTS> ring{bars + 6 + 2 * STATS, bars + 6 + 2 * STATS + SLOTS, base + 2 * TILE, TILE};
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 6 + 2 * STATS + 2 * SLOTS);
+  uint64_t *const kv_full = bars, *const s_full = bars + 1, *const dp_full = bars + 2, *const p_half = bars + 3, *const p_ready = bars + 4, *const ds_half = bars + 5,
+           *const ds_ready = bars + 6, *const done = bars + 7, *const go = bars + 8, *const cleared = bars + 9, *const st_full = bars + 10,
+           *const st_empty = bars + 10 + STATS;
+  const Ring<SLOTS> ring{bars + 10 + 2 * STATS, bars + 10 + 2 * STATS + SLOTS, ks + 2 * TILE, TILE};
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 10 + 2 * STATS + 2 * SLOTS);
   volatile int* const stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (warp == 8) tmem_alloc(tmem_slot, 512);
   if (threadIdx.x == 0) {
-    mbar_init(kv_full, 1), mbar_init(s_full, 1), mbar_init(dp_full, 1), mbar_init(p_ready, 256), mbar_init(ds_ready, 256), mbar_init(done, 1);
+    mbar_init(kv_full, 1), mbar_init(s_full, 1), mbar_init(dp_full, 1), mbar_init(done, 1), mbar_init(go, 1), mbar_init(cleared, 1);
+    mbar_init(p_half, 256), mbar_init(p_ready, 256), mbar_init(ds_half, 256), mbar_init(ds_ready, 256);
     for (int i = 0; i < STATS; ++i) mbar_init(st_full + i, 1), mbar_init(st_empty + i, 8);
     for (int i = 0; i < SLOTS; ++i) mbar_init(ring.full + i, 1), mbar_init(ring.empty + i, 1);
     fence_mbar_init();
@@ -693,22 +850,28 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
   auto head_of = [&](int i) { return hk * p.G + (it.begin + i) / it.tiles; };
   auto first_of = [&](int i) { return (it.first + (it.begin + i) % it.tiles) * kT; };
 
+  // tiles of queries that reach into padding: their rows there would meet weights of zero
+  auto padded = [&](int i) {
+    const int first = g.start + first_of(i);
+    return first < 0 || (first + kT > g.ctx && g.start + p.Nq > g.ctx);
+  };
+
   if (warp == 9) {
-    if (lane == 0 && n > 0) {
+    if (n > 0 && elect_one()) {
       mbar_expect_tx(kv_full, 2 * TILE);
-      load_tile<DP>(K, &maps.k, hk, k0, b, kv_full);
-      load_tile<DP>(V, &maps.v, hk, k0, b, kv_full);
+      load_tile<DP>(ks, &maps.k, hk, k0, b, kv_full);
+      load_tile<DP>(vs, &maps.v, hk, k0, b, kv_full);
+      typename Ring<SLOTS>::Place to;
       bool ok = true;
       int i = 0, held = 0;  // tiles and stats under way
-      for (; i < 2 * n && ok; ++i) {
-        ok = ring.wait_empty(wait, i);
-        if (!ok) break;
-        const int u = i / 2, h = head_of(u), i0 = first_of(u);
-        uint64_t* const bar = ring.full + i % SLOTS;
-        mbar_expect_tx(bar, TILE);
-        load_tile<DP>(ring.at(i), i % 2 ? &maps.dy : &maps.q, h, i0, b, bar);
-        if (i % 2 == 1) {  // the stats last: their place is free only when tile u - STATS is done with
-          if (u >= STATS && !(ok = wait(st_empty + u % STATS, (u / STATS + 1) & 1))) {
+      for (; i < 2 * n; ++i) {
+        if (!(ok = ring.wait_empty(wait, to))) break;
+        const int u = i >> 1, h = head_of(u), i0 = first_of(u);
+        mbar_expect_tx(ring.arrived(to), TILE);
+        load_tile<DP>(ring.at(to), i & 1 ? &maps.dy : &maps.q, h, i0, b, ring.arrived(to));
+        to.next();
+        if (i & 1) {  // the stats last: their place is free only when tile u - STATS is done with
+          if (!(ok = wait.one(st_empty + u % STATS, (u / STATS & 1) ^ 1))) {
             ++i;
             break;
           }
@@ -721,55 +884,67 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
         }
       }
       if (!ok) {
-        mbar_wait_bounded(kv_full, 0);
-        for (int e = held > STATS ? held - STATS : 0; e < held; ++e) mbar_wait_bounded(st_full + e % STATS, (e / STATS) & 1);
-        for (int e = i > SLOTS ? i - SLOTS : 0; e < i; ++e) mbar_wait_bounded(ring.full + e % SLOTS, (e / SLOTS) & 1);
+        mbar_wait_bounded(kv_full, 0, 1u << 16);
+        for (int e = held > STATS ? held - STATS : 0; e < held; ++e) mbar_wait_bounded(st_full + e % STATS, (e / STATS) & 1, 1u << 16);
+        settle(ring, i);
       }
+    }
+  } else if (warp == 10) {
+    uint32_t clears = 0;
+    for (int i = 0; i < 2 * n; ++i) {
+      if (!padded(i >> 1)) continue;
+      if (!wait(go, clears++ & 1)) break;
+      const int first = g.start + first_of(i >> 1);
+      clear_rows<DP>(ring.at(ring.place(i)), -first, g.ctx - first, cleared);
     }
   } else if (warp == 8) {
-    const bool leader = elect_one();
-    const uint32_t ks = smem_u32(K), vs = smem_u32(V);
-    // waits for a tile of queries (or their cotangents) and clears its rows of padding
-    auto arrived = [&](int load) {
-      if (!ring.wait_full(wait, load)) return false;
-      const int first = g.start + first_of(load / 2);
-      if (first < 0 || (first + kT > g.ctx && g.start + p.Nq > g.ctx)) clear_rows<DP>(ring.at(load), -first, g.ctx - first);
-      return true;
-    };
-    auto scores = [&](int i) {
-      if (!arrived(2 * i)) return false;
-      if (leader) {
-        product_scores<DP>(tmem, ks, smem_u32(ring.at(2 * i)));
+    if (n > 0 && elect_one()) {
+      typename Ring<SLOTS>::Place q_at, dy_at, old_q, old_dy;  // of the next scores, the next dP; of the next dk, the next dv
+      dy_at.next(), old_dy.next();
+      uint32_t clears = 0;
+      auto arrived = [&](const typename Ring<SLOTS>::Place& at, int i) {
+        if (!ring.wait_full(wait, at)) return false;
+        return !padded(i) || have_cleared(wait, go, cleared, clears++ & 1);  // (in the order of the loads)
+      };
+      auto scores = [&](int i) {
+        if (!arrived(q_at, i)) return false;
+        product_scores<DP>(tmem, ks, ring.at(q_at));
         mma_commit(s_full);
-      }
-      return true;
-    };
-    auto grads = [&](int i) {
-      if (!arrived(2 * i + 1)) return false;
-      if (leader) {
-        product_scores<DP>(t_dp, vs, smem_u32(ring.at(2 * i + 1)));
+        q_at.next(), q_at.next();
+        return true;
+      };
+      auto grads = [&](int i) {
+        if (!arrived(dy_at, i)) return false;
+        product_scores<DP>(t_dp, vs, ring.at(dy_at));
         mma_commit(dp_full);
+        dy_at.next(), dy_at.next();
+        return true;
+      };
+      bool ok = wait.one(kv_full, 0) && scores(0) && grads(0);
+#pragma unroll 1
+      for (int i = 0; ok && i < n; ++i) {
+        if (!(ok = wait.one(p_half, i & 1))) break;
+        tmem_after();
+        product_sums<DP, 0>(t_dv, tmem, ring.at(old_dy), i > 0);
+        if (!(ok = wait.one(p_ready, i & 1))) break;
+        tmem_after();
+        product_sums<DP, 1>(t_dv, tmem, ring.at(old_dy), true);
+        ring.release(old_dy);
+        old_dy.next(), old_dy.next();
+        if (i + 1 < n && !(ok = scores(i + 1))) break;
+        if (!(ok = wait.one(ds_half, i & 1))) break;
+        tmem_after();
+        product_sums<DP, 0>(t_dk, t_dp, ring.at(old_q), i > 0);
+        if (!(ok = wait.one(ds_ready, i & 1))) break;
+        tmem_after();
+        product_sums<DP, 1>(t_dk, t_dp, ring.at(old_q), true);
+        ring.release(old_q);
+        old_q.next(), old_q.next();
+        if (i + 1 < n) ok = grads(i + 1);
       }
-      return true;
-    };
-    bool ok = n == 0 || (wait(kv_full, 0) && scores(0) && grads(0));
-    for (int i = 0; ok && i < n; ++i) {
-      if (!(ok = wait(p_ready, i & 1))) break;
-      tmem_after();
-      if (leader) {
-        product_sums<DP>(t_dv, tmem, 64, smem_u32(ring.at(2 * i + 1)), i > 0);
-        ring.release(2 * i + 1);
-      }
-      if (i + 1 < n && !(ok = scores(i + 1))) break;
-      if (!(ok = wait(ds_ready, i & 1))) break;
-      tmem_after();
-      if (leader) {
-        product_sums<DP>(t_dk, t_dp, 64, smem_u32(ring.at(2 * i)), i > 0);
-        ring.release(2 * i);
-      }
-      if (i + 1 < n) ok = grads(i + 1);
+      if (ok) mma_commit(done);
     }
-    if (ok && n > 0 && leader) mma_commit(done);
+    __syncwarp();
   } else {
     const int half = warp / 4, r = warp % 4 * 32 + lane, key = k0 + r;
     const int end = min(g.ctx, g.start + p.Nq);
@@ -787,43 +962,46 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
       // queries key .. last of the columns see the key
       const int lo = key - first, hi = min(end, key < p.n_sink ? end : key + p.window) - first;
       const bool whole = k0 + kT - 1 <= first && first + 64 <= end && (first + 63 < k0 + p.window || k0 + kT <= p.n_sink);
-      uint32_t w[32];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
+        uint32_t w[16];
+        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+        auto weights = [&](auto mix) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 ls = *reinterpret_cast<const float4*>(lse + 32 * c + e);
-          s[c][e] = ex2(fmaf(s[c][e], p.scale_log2, -ls.x));
-          s[c][e + 1] = ex2(fmaf(s[c][e + 1], p.scale_log2, -ls.y));
-          s[c][e + 2] = ex2(fmaf(s[c][e + 2], p.scale_log2, -ls.z));
-          s[c][e + 3] = ex2(fmaf(s[c][e + 3], p.scale_log2, -ls.w));
-        }
+          for (int e = 0; e < 32; e += 4) {
+            const float4 ls = *reinterpret_cast<const float4*>(lse + 32 * c + e);
+            exp2_pair<decltype(mix)::value>(s[c][e], s[c][e + 1], scale2, make_float2(-ls.x, -ls.y), e / 2);
+            exp2_pair<decltype(mix)::value>(s[c][e + 2], s[c][e + 3], scale2, make_float2(-ls.z, -ls.w), e / 2 + 1);
+          }
+        };
+        if (whole) weights(std::true_type());
+        else weights(std::false_type());
         if (!whole) {
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (32 * c + e < lo || 32 * c + e >= hi) s[c][e] = 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) w[16 * c + e / 2] = pack(s[c][e], s[c][e + 1]);
+        for (int e = 0; e < 32; e += 2) w[e / 2] = pack(s[c][e], s[c][e + 1]);
+        tmem_store16(ts + 16 * c, w);
+        tmem_stored();
+        tmem_before();
+        mbar_arrive(c ? p_ready : p_half);
       }
-      tmem_store32(ts, w);
-      tmem_stored();
-      tmem_before();
-      mbar_arrive(p_ready);
       if (!(ok = wait(dp_full, i & 1))) break;
       tmem_after();
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float dp[32];
+        uint32_t w[16];
         tmem_load32f(td + 32 * c, dp);
         tmem_loaded(dp);
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           const float4 de = *reinterpret_cast<const float4*>(delta + 32 * c + e);
-          dp[e] = s[c][e] * (dp[e] - de.x);
-          dp[e + 1] = s[c][e + 1] * (dp[e + 1] - de.y);
-          dp[e + 2] = s[c][e + 2] * (dp[e + 2] - de.z);
-          dp[e + 3] = s[c][e + 3] * (dp[e + 3] - de.w);
+          const float2 t = __fmul2_rn(make_float2(s[c][e], s[c][e + 1]), __fadd2_rn(make_float2(dp[e], dp[e + 1]), make_float2(-de.x, -de.y)));
+          const float2 u = __fmul2_rn(make_float2(s[c][e + 2], s[c][e + 3]), __fadd2_rn(make_float2(dp[e + 2], dp[e + 3]), make_float2(-de.z, -de.w)));
+          dp[e] = t.x, dp[e + 1] = t.y, dp[e + 2] = u.x, dp[e + 3] = u.y;
         }
         if (!whole) {
 #pragma unroll
@@ -831,12 +1009,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
             if (32 * c + e < lo || 32 * c + e >= hi) dp[e] = 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) w[16 * c + e / 2] = pack(dp[e], dp[e + 1]);
+        for (int e = 0; e < 32; e += 2) w[e / 2] = pack(dp[e], dp[e + 1]);
+        tmem_store16(td + 16 * c, w);
+        tmem_stored();
+        tmem_before();
+        mbar_arrive(c ? ds_ready : ds_half);
       }
-      tmem_store32(td, w);
-      tmem_stored();
-      tmem_before();
-      mbar_arrive(ds_ready);
       __syncwarp();
       if (lane == 0) mbar_arrive(st_empty + i % STATS);
     }
@@ -927,7 +1105,7 @@ cudaError_t run_fwd(const AttnParams& p, const Maps& maps, cudaStream_t st) {
   const cudaError_t e = grant_smem(grant, attn_tensor_fwd_kernel<DP, SLOTS>, smem);
   if (e != cudaSuccess) return e;
   const int tiles = (p.Nq + 2 * kT - 1) / (2 * kT);
-  return launch_behind(attn_tensor_fwd_kernel<DP, SLOTS>, dim3((unsigned)(tiles * p.H * p.B)), kThreads, smem, st, p, maps);
+  return launch_behind(attn_tensor_fwd_kernel<DP, SLOTS>, dim3((unsigned)(tiles * p.H * p.B)), kFwdThreads, smem, st, p, maps);
 }
 template <int DP, int SLOTS>
 cudaError_t run_bwd(const AttnParams& p, const Maps& maps, cudaStream_t st) {
