@@ -135,6 +135,12 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
                "l"(map), "r"(c), "r"(head), "r"(row), "r"(b), "r"(smem_u32(bar))
                : "memory");
 }
+__device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int c, int head, int row, int b) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(src), "r"(c), "r"(head),
+               "r"(row), "r"(b)
+               : "memory");
+}
 __device__ __forceinline__ uint64_t now_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
@@ -276,16 +282,30 @@ __device__ __forceinline__ void exp2_pair(float& a, float& b, float2 scale, floa
     x = make_float2(ex2(x.x), ex2(x.y));
   a = x.x, b = x.y;
 }
-// what the rounding in store_row takes off, rounded itself
-__device__ __forceinline__ void store_rest(__nv_bfloat16* row, const float (&x)[32], float f, int c0, int d) {
-  float r[32];
+// Results leave through shared memory and the TMA unit: rows written by their threads straight to global memory, 16 bytes per lane and
+// row, took a third of the forward's time in windows of 1024 (15000 of 51000 cycles; now 4000).  32 features of row r, c0 .. c0 + 31,
+// into a tile laid out as the TMA unit has it.
+__device__ __forceinline__ void stage_row(uint32_t tile, int r, const float (&x)[32], float f, int c0) {
 #pragma unroll
-  for (int e = 0; e < 32; ++e) r[e] = x[e] * f - __bfloat162float(__float2bfloat16(x[e] * f));
+  for (int e = 0; e < 32; e += 8) {
+    const int c = c0 + e;
+    const uint32_t at = tile + (c / 64) * kBlockBytes + r * 128 + ((c % 64 / 8 ^ (r & 7)) << 4);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(pack(x[e] * f, x[e + 1] * f)), "r"(pack(x[e + 2] * f, x[e + 3] * f)),
+                 "r"(pack(x[e + 4] * f, x[e + 5] * f)), "r"(pack(x[e + 6] * f, x[e + 7] * f))
+                 : "memory");
+  }
+}
+// what the rounding in stage_row takes off, to be staged itself
+__device__ __forceinline__ void keep_rest(float (&x)[32], float f) {
 #pragma unroll
-  for (int e = 0; e < 32; e += 8)
-    if (c0 + e < d)
-      *reinterpret_cast<uint4*>(row + c0 + e) =
-          make_uint4(pack(r[e], r[e + 1]), pack(r[e + 2], r[e + 3]), pack(r[e + 4], r[e + 5]), pack(r[e + 6], r[e + 7]));
+  for (int e = 0; e < 32; ++e) x[e] = x[e] * f - __bfloat162float(__float2bfloat16(x[e] * f));
+}
+// A staged tile (written, fenced and handed in by its threads) to global memory; rows and features beyond the tensor are left out.
+template <int DP>
+__device__ __forceinline__ void send_tile(const CUtensorMap* map, uint32_t tile, int head, int row, int b) {
+#pragma unroll
+  for (int c = 0; c < DP / 64; ++c) tma_store(map, tile + c * kBlockBytes, c * 64, head, row, b);
+  bulk_commit();
 }
 // 32 features of a row to global memory, c0 .. c0 + 31 of d (a multiple of 8)
 __device__ __forceinline__ void store_row(__nv_bfloat16* row, const float (&x)[32], float f, int c0, int d) {
@@ -306,7 +326,7 @@ __device__ __forceinline__ void settle(const Ring<SLOTS>& ring, int loads) {
 }
 
 struct Maps {
-  CUtensorMap q, k, v, dy;
+  CUtensorMap q, k, v, dy, y, rest, dq, dk, dv;  // (the direction's own)
 };
 
 // The keys of tile k0 that a query at `pos` sees, as columns: [lo, hi), and those below `sink`
@@ -350,16 +370,19 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
   const uint32_t qs = smem_u32(base);
   float* const shared_row = reinterpret_cast<float*>(base + (2 + SLOTS) * TILE);  // [tile][half][row]
   uint64_t* const bars = reinterpret_cast<uint64_t*>(shared_row + 4 * kT);
-  uint64_t *const q_full = bars, *const s_full = bars + 1, *const p_half = bars + 3, *const p_ready = bars + 5, *const o_full = bars + 7, *const go = bars + 9, *const cleared = bars + 10;
-  const Ring<SLOTS> ring{bars + 11, bars + 11 + SLOTS, qs + 2 * TILE, TILE};
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 11 + 2 * SLOTS);
+  uint64_t *const q_full = bars, *const s_full = bars + 1, *const p_half = bars + 3, *const p_ready = bars + 5, *const o_full = bars + 7, *const go = bars + 9, *const cleared = bars + 10,
+           *const staged = bars + 11, *const sent = bars + 13;
+  const Ring<SLOTS> ring{bars + 15, bars + 15 + SLOTS, qs + 2 * TILE, TILE};
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 15 + 2 * SLOTS);
   volatile int* const stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
+  if (warp == 17 && elect_one()) tma_prefetch(&maps.q), tma_prefetch(&maps.k), tma_prefetch(&maps.v), tma_prefetch(&maps.y);
   if (warp == 16) tmem_alloc(tmem_slot, 512);
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1), mbar_init(go, 1), mbar_init(cleared, 1);
     for (int x = 0; x < 2; ++x) mbar_init(s_full + x, 1), mbar_init(p_half + x, 2 * kT), mbar_init(p_ready + x, 2 * kT), mbar_init(o_full + x, 1);
+    for (int x = 0; x < 2; ++x) mbar_init(staged + x, 2 * kT), mbar_init(sent + x, 1);
     for (int i = 0; i < SLOTS; ++i) mbar_init(ring.full + i, 1), mbar_init(ring.empty + i, 1);
     fence_mbar_init();
     *stop = 0;
@@ -564,24 +587,39 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
       // (padding between rows that see a whole tile has had no mask)
       const bool some = mine > 0 && pos >= 0 && pos < end && !(l == 0.f);
       const float inv = some ? 1.f / l : 0.f;
-      const long long row = ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
+      if (p.lse && half == 0 && qi < p.Nq) p.lse[((long long)b * p.H + h) * p.Nqp + qi] = some ? ref + log2f(l) : INFINITY;
+      // the tile's queries have been read by the last of its products (with no products, they may still be arriving)
+      const uint32_t tile = qs + x * TILE;
+      const int first = i0 + x * kT;
+      if (n > 0 && first < p.Nq) ok = wait(q_full, 0);
+      for (int pass = 0; ok && first < p.Nq && pass < (p.rest ? 2 : 1); ++pass) {
+        if (pass && !(ok = wait(sent + x, 0))) break;
 #pragma unroll 1
-      for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
-        float o[32];
-        if (mine > 0) {
-          tmem_load32f(to + c, o);
-          tmem_loaded(o);
-        }
-        if (!some) {
+        for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
+          float o[32];
+          if (mine > 0) {
+            tmem_load32f(to + c, o);
+            tmem_loaded(o);
+          }
+          if (!some) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          }
+          if (pass) keep_rest(o, inv);
+          stage_row(tile, r, o, pass ? 1.f : inv, c);
         }
-        if (qi < p.Nq) {
-          store_row(static_cast<__nv_bfloat16*>(p.y) + row, o, inv, c, p.d);
-          if (p.rest) store_rest(p.rest + row, o, inv, c, p.d);
+        fence_proxy_async();
+        mbar_arrive(staged + x);
+        if (warp % 8 == 0) {
+          if (!(ok = wait(staged + x, pass))) break;
+          if (lane == 0) {
+            send_tile<DP>(pass ? &maps.rest : &maps.y, tile, h, first, b);
+            bulk_wait_read0();
+            mbar_arrive(sent + x);
+          }
+          __syncwarp();
         }
       }
-      if (p.lse && half == 0 && qi < p.Nq) p.lse[((long long)b * p.H + h) * p.Nqp + qi] = some ? ref + log2f(l) : INFINITY;
     }
     tmem_before();
   }
@@ -610,19 +648,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
     return;
   }
   const uint32_t qs = smem_u32(base), dys = qs + TILE;
-  float* const halves = reinterpret_cast<float*>(base + (2 + SLOTS) * TILE);  // [2][128]
-  uint64_t* const bars = reinterpret_cast<uint64_t*>(halves + 512);
+  float* const deltas = reinterpret_cast<float*>(base + (2 + SLOTS) * TILE);  // [128]
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(deltas + 512);
   uint64_t *const q_full = bars, *const s_full = bars + 1, *const dp_full = bars + 3, *const ds_half = bars + 4, *const ds_ready = bars + 5, *const done = bars + 6,
-           *const go = bars + 7, *const cleared = bars + 8;
-  const Ring<SLOTS> ring{bars + 9, bars + 9 + SLOTS, qs + 2 * TILE, TILE};
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 9 + 2 * SLOTS);
+           *const go = bars + 7, *const cleared = bars + 8, *const staged = bars + 9;
+  const Ring<SLOTS> ring{bars + 10, bars + 10 + SLOTS, qs + 2 * TILE, TILE};
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 10 + 2 * SLOTS);
   volatile int* const stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
+  if (warp == 9 && elect_one()) tma_prefetch(&maps.q), tma_prefetch(&maps.dy), tma_prefetch(&maps.k), tma_prefetch(&maps.v), tma_prefetch(&maps.dq);
   if (warp == 8) tmem_alloc(tmem_slot, 512);
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1), mbar_init(s_full, 1), mbar_init(s_full + 1, 1), mbar_init(dp_full, 1), mbar_init(ds_half, 256), mbar_init(ds_ready, 256);
-    mbar_init(done, 1), mbar_init(go, 1), mbar_init(cleared, 1);
+    mbar_init(done, 1), mbar_init(go, 1), mbar_init(cleared, 1), mbar_init(staged, 256);
     for (int i = 0; i < SLOTS; ++i) mbar_init(ring.full + i, 1), mbar_init(ring.empty + i, 1);
     fence_mbar_init();
     *stop = 0;
@@ -706,26 +745,45 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
     const int p_lo = g.start + i0, p_hi = p_lo + kT - 1;
     const bool live = pos >= 0 && pos < end;
     const long long head_row = ((long long)b * p.H + h) * p.Nqp + qi;
-    // delta: half of the features each
-    float sum = 0.f;
-    if (live) {
-      const long long y_row = ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
-      const __nv_bfloat16 *y = static_cast<const __nv_bfloat16*>(p.y_in) + y_row, *rest = p.rest + y_row;
-      const __nv_bfloat16* dy = static_cast<const __nv_bfloat16*>(p.dy) + b * p.sdy_b + qi * p.sdy_n + (long long)h * p.d;
-      for (int c = half * (DP / 2); c < min((half + 1) * (DP / 2), p.d); c += 8) {
-        const uint4 u = *reinterpret_cast<const uint4*>(y + c), w = *reinterpret_cast<const uint4*>(dy + c),
-                    t = *reinterpret_cast<const uint4*>(rest + c);
-        const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, ww[4] = {w.x, w.y, w.z, w.w}, tt[4] = {t.x, t.y, t.z, t.w};
+    // delta = sum(dy * y) of every row: DP / 8 lanes read a row, so that a load takes whole rows; all of a thread's loads are under way at
+    // once (one after the other they took 17000 cycles, as long as eight tiles of keys).  dy is in shared memory already.
+    {
+      constexpr int LANES = DP / 8, ROWS = 32 / LANES, PASSES = 16 / ROWS;
+      const int c = lane % LANES * 8, row0 = warp * 16 + lane / LANES;
+      uint4 u[PASSES], t[PASSES];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sum = fmaf(__uint_as_float(uu[e] << 16) + __uint_as_float(tt[e] << 16), __uint_as_float(ww[e] << 16), sum);
-          sum = fmaf(__uint_as_float(uu[e] & 0xffff0000u) + __uint_as_float(tt[e] & 0xffff0000u), __uint_as_float(ww[e] & 0xffff0000u), sum);
+      for (int pass = 0; pass < PASSES; ++pass) {
+        const int i = i0 + row0 + pass * ROWS;
+        const bool here = c < p.d && g.start + i >= 0 && g.start + i < end;
+        const long long y_row = ((long long)b * p.Nq + (here ? i : 0)) * p.H * p.d + (long long)h * p.d + (here ? c : 0);  // (in bounds)
+        u[pass] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.y_in) + y_row);
+        t[pass] = *reinterpret_cast<const uint4*>(p.rest + y_row);
+      }
+      if (n > 0) wait(q_full, 0);  // (given up: the waits that follow give up too)
+#pragma unroll
+      for (int pass = 0; pass < PASSES; ++pass) {
+        const int row = row0 + pass * ROWS, i = i0 + row;
+        float sum = 0.f;
+        if (n > 0 && c < p.d && g.start + i >= 0 && g.start + i < end) {
+          uint4 w;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                       : "r"(dys + (c / 64) * kBlockBytes + row * 128 + ((c % 64 / 8 ^ (row & 7)) << 4)));
+          const uint32_t uu[4] = {u[pass].x, u[pass].y, u[pass].z, u[pass].w}, ww[4] = {w.x, w.y, w.z, w.w},
+                         tt[4] = {t[pass].x, t[pass].y, t[pass].z, t[pass].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sum = fmaf(__uint_as_float(uu[e] << 16) + __uint_as_float(tt[e] << 16), __uint_as_float(ww[e] << 16), sum);
+            sum = fmaf(__uint_as_float(uu[e] & 0xffff0000u) + __uint_as_float(tt[e] & 0xffff0000u), __uint_as_float(ww[e] & 0xffff0000u), sum);
+          }
         }
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        if (c == 0) deltas[row] = sum;
       }
     }
-    halves[half * kT + r] = sum;
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    const float delta = halves[r] + halves[kT + r];
+    const float delta = deltas[r];
     if (half == 0 && qi < p.Nq) p.delta[head_row] = delta;
     const float lse = live ? p.lse[head_row] : INFINITY;
     bool ok = true;
@@ -778,9 +836,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
     if (n > 0 && ok) ok = wait(done, 0);
     tmem_after();
     if (ok) {
-      __nv_bfloat16* const row = static_cast<__nv_bfloat16*>(p.dq) + ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
+      if (n > 0) ok = wait(q_full, 0);
 #pragma unroll 1
-      for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
+      for (int c = half * (DP / 2); ok && c < (half + 1) * (DP / 2); c += 32) {
         float o[32];
         if (n > 0) {
           tmem_load32f(t_dq + c + lanes, o);
@@ -789,8 +847,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0.f;
         }
-        if (qi < p.Nq) store_row(row, o, p.scale, c, p.d);
+        stage_row(qs, r, o, p.scale, c);  // (over the queries, which the last product has read)
       }
+      fence_proxy_async();
+      if (ok) mbar_arrive(staged);
+      if (ok && warp == 0 && wait(staged, 0) && lane == 0) {
+        send_tile<DP>(&maps.dq, qs, h, i0, b);
+        bulk_wait_read0();
+      }
+      __syncwarp();
     }
     tmem_before();
   }
@@ -820,15 +885,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
   uint64_t* const bars = reinterpret_cast<uint64_t*>(stats + STATS * 2 * kT);
   uint64_t *const kv_full = bars, *const s_full = bars + 1, *const dp_full = bars + 2, *const p_half = bars + 3, *const p_ready = bars + 4, *const ds_half = bars + 5,
            *const ds_ready = bars + 6, *const done = bars + 7, *const go = bars + 8, *const cleared = bars + 9, *const st_full = bars + 10,
-           *const st_empty = bars + 10 + STATS;
-  const Ring<SLOTS> ring{bars + 10 + 2 * STATS, bars + 10 + 2 * STATS + SLOTS, ks + 2 * TILE, TILE};
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 10 + 2 * STATS + 2 * SLOTS);
+           *const st_empty = bars + 10 + STATS, *const staged = bars + 10 + 2 * STATS;
+  const Ring<SLOTS> ring{bars + 11 + 2 * STATS, bars + 11 + 2 * STATS + SLOTS, ks + 2 * TILE, TILE};
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 11 + 2 * STATS + 2 * SLOTS);
   volatile int* const stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
+  if (warp == 9 && elect_one()) tma_prefetch(&maps.k), tma_prefetch(&maps.v), tma_prefetch(&maps.q), tma_prefetch(&maps.dy), tma_prefetch(&maps.dk);
   if (warp == 8) tmem_alloc(tmem_slot, 512);
   if (threadIdx.x == 0) {
-    mbar_init(kv_full, 1), mbar_init(s_full, 1), mbar_init(dp_full, 1), mbar_init(done, 1), mbar_init(go, 1), mbar_init(cleared, 1);
+    mbar_init(kv_full, 1), mbar_init(s_full, 1), mbar_init(dp_full, 1), mbar_init(done, 1), mbar_init(go, 1), mbar_init(cleared, 1), mbar_init(staged, 256);
     mbar_init(p_half, 256), mbar_init(p_ready, 256), mbar_init(ds_half, 256), mbar_init(ds_ready, 256);
     for (int i = 0; i < STATS; ++i) mbar_init(st_full + i, 1), mbar_init(st_empty + i, 8);
     for (int i = 0; i < SLOTS; ++i) mbar_init(ring.full + i, 1), mbar_init(ring.empty + i, 1);
@@ -847,12 +913,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
   const KeyItem it = key_item<kT, kT>(p, g, at.first_last);
   const int k0 = it.tile * kT, n = it.end - it.begin;
   const Waiter wait{stop, p.status};
-  auto head_of = [&](int i) { return hk * p.G + (it.begin + i) / it.tiles; };
-  auto first_of = [&](int i) { return (it.first + (it.begin + i) % it.tiles) * kT; };
+  // an entry of the list of the item's heads and tiles of queries, and the next one (each role walks the list by itself)
+  struct Entry {
+    int head, tile, first, end;  // tile: first <= tile < end
+    __device__ __forceinline__ int row() const { return tile * kT; }
+    __device__ __forceinline__ void next() {
+      if (++tile == end) tile = first, ++head;
+    }
+  };
+  Entry entry{hk * p.G, it.first, it.first, it.first + it.tiles};
+  if (it.begin > 0 && n > 0) entry.head += it.begin / it.tiles, entry.tile += it.begin % it.tiles;
 
   // tiles of queries that reach into padding: their rows there would meet weights of zero
-  auto padded = [&](int i) {
-    const int first = g.start + first_of(i);
+  auto padded = [&](const Entry& e) {
+    const int first = g.start + e.row();
     return first < 0 || (first + kT > g.ctx && g.start + p.Nq > g.ctx);
   };
 
@@ -866,7 +940,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
       int i = 0, held = 0;  // tiles and stats under way
       for (; i < 2 * n; ++i) {
         if (!(ok = ring.wait_empty(wait, to))) break;
-        const int u = i >> 1, h = head_of(u), i0 = first_of(u);
+        const int u = i >> 1, h = entry.head, i0 = entry.row();
         mbar_expect_tx(ring.arrived(to), TILE);
         load_tile<DP>(ring.at(to), i & 1 ? &maps.dy : &maps.q, h, i0, b, ring.arrived(to));
         to.next();
@@ -881,6 +955,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
           bulk_g2s(st, p.lse + row, kT * 4, st_full + u % STATS);
           bulk_g2s(st + kT, p.delta + row, kT * 4, st_full + u % STATS);
           held = u + 1;
+          entry.next();
         }
       }
       if (!ok) {
@@ -892,35 +967,38 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
   } else if (warp == 10) {
     uint32_t clears = 0;
     for (int i = 0; i < 2 * n; ++i) {
-      if (!padded(i >> 1)) continue;
-      if (!wait(go, clears++ & 1)) break;
-      const int first = g.start + first_of(i >> 1);
-      clear_rows<DP>(ring.at(ring.place(i)), -first, g.ctx - first, cleared);
+      if (padded(entry)) {
+        if (!wait(go, clears++ & 1)) break;
+        const int first = g.start + entry.row();
+        clear_rows<DP>(ring.at(ring.place(i)), -first, g.ctx - first, cleared);
+      }
+      if (i & 1) entry.next();
     }
   } else if (warp == 8) {
     if (n > 0 && elect_one()) {
       typename Ring<SLOTS>::Place q_at, dy_at, old_q, old_dy;  // of the next scores, the next dP; of the next dk, the next dv
       dy_at.next(), old_dy.next();
       uint32_t clears = 0;
-      auto arrived = [&](const typename Ring<SLOTS>::Place& at, int i) {
+      auto arrived = [&](const typename Ring<SLOTS>::Place& at) {
         if (!ring.wait_full(wait, at)) return false;
-        return !padded(i) || have_cleared(wait, go, cleared, clears++ & 1);  // (in the order of the loads)
+        return !padded(entry) || have_cleared(wait, go, cleared, clears++ & 1);  // (in the order of the loads)
       };
-      auto scores = [&](int i) {
-        if (!arrived(q_at, i)) return false;
+      auto scores = [&]() {
+        if (!arrived(q_at)) return false;
         product_scores<DP>(tmem, ks, ring.at(q_at));
         mma_commit(s_full);
         q_at.next(), q_at.next();
         return true;
       };
-      auto grads = [&](int i) {
-        if (!arrived(dy_at, i)) return false;
+      auto grads = [&]() {  // (moves on to the next entry)
+        if (!arrived(dy_at)) return false;
         product_scores<DP>(t_dp, vs, ring.at(dy_at));
         mma_commit(dp_full);
         dy_at.next(), dy_at.next();
+        entry.next();
         return true;
       };
-      bool ok = wait.one(kv_full, 0) && scores(0) && grads(0);
+      bool ok = wait.one(kv_full, 0) && scores() && grads();
 #pragma unroll 1
       for (int i = 0; ok && i < n; ++i) {
         if (!(ok = wait.one(p_half, i & 1))) break;
@@ -931,7 +1009,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
         product_sums<DP, 1>(t_dv, tmem, ring.at(old_dy), true);
         ring.release(old_dy);
         old_dy.next(), old_dy.next();
-        if (i + 1 < n && !(ok = scores(i + 1))) break;
+        if (i + 1 < n && !(ok = scores())) break;
         if (!(ok = wait.one(ds_half, i & 1))) break;
         tmem_after();
         product_sums<DP, 0>(t_dk, t_dp, ring.at(old_q), i > 0);
@@ -940,7 +1018,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
         product_sums<DP, 1>(t_dk, t_dp, ring.at(old_q), true);
         ring.release(old_q);
         old_q.next(), old_q.next();
-        if (i + 1 < n) ok = grads(i + 1);
+        if (i + 1 < n) ok = grads();
       }
       if (ok) mma_commit(done);
     }
@@ -951,7 +1029,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16, ts = tmem + half * 64 + lanes, td = t_dp + half * 64 + lanes;
     bool ok = true;
     for (int i = 0; i < n; ++i) {
-      const int first = g.start + first_of(i) + half * 64;  // position of column 0
+      const int first = g.start + entry.row() + half * 64;  // position of column 0
+      entry.next();
       const float *lse = stats + i % STATS * 2 * kT + half * 64, *delta = lse + kT;
       if (!(ok = wait(st_full + i % STATS, (i / STATS) & 1) && wait(s_full, i & 1))) break;
       tmem_after();
@@ -1024,8 +1103,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
     if (ok) {
       float* const part = sinks ? part_of(p, b, hk, it.tile, it.chunk < 0 ? p.chunks : it.chunk) : nullptr;
       const long long row = ((long long)b * p.Nk + key) * p.Hk * p.d + (long long)hk * p.d;
+      if (n > 0) ok = wait(kv_full, 0);
 #pragma unroll 1
-      for (int which = 0; which < 2; ++which)
+      for (int which = 0; ok && which < 2; ++which)
 #pragma unroll 1
         for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
           float o[32];
@@ -1042,10 +1122,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
               if (c + e < p.d) *reinterpret_cast<float4*>(at_part + e) = make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
-          } else if (it.chunk < 0 && key < p.Nk) {
-            store_row(static_cast<__nv_bfloat16*>(which ? p.dv : p.dk) + row, o, f, c, p.d);
+          } else if (sinks) {  // (a tile whose rows go two ways)
+            if (it.chunk < 0 && key < p.Nk) store_row(static_cast<__nv_bfloat16*>(which ? p.dv : p.dk) + row, o, f, c, p.d);
+          } else {
+            stage_row(which ? vs : ks, r, o, f, c);  // (over the keys and values, which the last products have read)
           }
         }
+      if (!sinks) {
+        fence_proxy_async();
+        if (ok) mbar_arrive(staged);
+        if (ok && warp == 0 && wait(staged, 0) && lane == 0) {
+          send_tile<DP>(&maps.dk, ks, hk, k0, b);
+          send_tile<DP>(&maps.dv, vs, hk, k0, b);
+          bulk_wait_read0();
+        }
+        __syncwarp();
+      }
     }
     tmem_before();
   }
@@ -1124,7 +1216,16 @@ cudaError_t encode_all(Maps& m, const AttnParams& p, bool bwd) {
   if (e == cudaSuccess) e = encode(m.q, p.q, p.d, p.H, p.Nq, p.B, p.sq_n, p.sq_b);
   if (e == cudaSuccess) e = encode(m.k, p.k, p.d, p.Hk, p.Nk, p.B, p.sk_n, p.sk_b);
   if (e == cudaSuccess) e = encode(m.v, p.v, p.d, p.Hk, p.Nk, p.B, p.sv_n, p.sv_b);
-  if (e == cudaSuccess && bwd) e = encode(m.dy, p.dy, p.d, p.H, p.Nq, p.B, p.sdy_n, p.sdy_b);
+  const long long En = (long long)p.H * p.d, Ek = (long long)p.Hk * p.d;  // results are contiguous
+  if (!bwd) {
+    if (e == cudaSuccess) e = encode(m.y, p.y, p.d, p.H, p.Nq, p.B, En, En * p.Nq);
+    if (e == cudaSuccess && p.rest) e = encode(m.rest, p.rest, p.d, p.H, p.Nq, p.B, En, En * p.Nq);
+    return e;
+  }
+  if (e == cudaSuccess) e = encode(m.dy, p.dy, p.d, p.H, p.Nq, p.B, p.sdy_n, p.sdy_b);
+  if (e == cudaSuccess) e = encode(m.dq, p.dq, p.d, p.H, p.Nq, p.B, En, En * p.Nq);
+  if (e == cudaSuccess) e = encode(m.dk, p.dk, p.d, p.Hk, p.Nk, p.B, Ek, Ek * p.Nk);
+  if (e == cudaSuccess) e = encode(m.dv, p.dv, p.d, p.Hk, p.Nk, p.B, Ek, Ek * p.Nk);
   return e;
 }
 
