@@ -101,16 +101,25 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// bf16, heads of a multiple of 8 features.  Blocks of 16 keys go from global memory straight into the operands of the matrix
-// instructions (m16n8k16: 16 query rows, 8 keys or features, 16 features or keys), 16 bytes per lane and load, without shared
-// memory: the order of a sum's terms is free, so the lane that loads features 8 c .. 8 c + 7 of a key uses them as its four
-// pairs of two products' terms, with the queries laid out the same way; for the values, the lane's eight features belong to eight
-// products' columns, and pairs of keys are put together by byte permutes.  The products take a fraction of the time of
-// the loads; their formats ask for 16 rows, however few there are (WIDE: the upper 8 are there).
-template <int DP, bool WIDE>
-__global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const AttnParams p) {
+// a pair of bf16 per lane as an 8 x 8 matrix (lane / 4: row): its transpose
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// bf16, heads of a multiple of 8 features.  Blocks of 16 keys go from global memory straight into the left operands of the matrix
+// instructions (m16n8k16), 16 bytes per lane and load, without shared memory; 8 query rows are the columns (TILES of them).
+//   scores^T = keys . queries^T    16 keys, 16 features a time
+//   sums^T  += values^T . weights^T  16 features, 16 keys a time
+// The order of a sum's terms is free: the lane that loads features 8 c .. 8 c + 7 of two keys uses them as its pairs of two products'
+// terms, the queries laid out the same way.  For the values the lane's eight features belong to four products' rows, and pairs of keys
+// are put together by byte permutes.  (With the queries as left operand, whose 16 rows are half empty, a step took twice the
+// instructions and 32 registers more, and one CTA less fitted on an SM.)
+template <int DP, int TILES>
+__global__ void __launch_bounds__(kWarps * 32, TILES == 1 ? 2 : 1) attn_decode_kernel(const __grid_constant__ AttnParams p) {
   wait_for_inputs();
-  constexpr int R = WIDE ? 16 : 8, TK = DP / 32, TV = DP / 64;
+  constexpr int R = 8 * TILES, TK = DP / 32, TV = DP / 64;
   extern __shared__ float sm[];
   float *Os = sm, *ms = Os + kWarps * R * DP, *ls = ms + kWarps * R;
   const int ranks = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
@@ -122,24 +131,33 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const AttnP
   const KeyBlocks kb = key_blocks(p, g, 16);
   using bf16 = __nv_bfloat16;
 
-  uint4 q[WIDE ? 2 : 1][TK];
-  int pos[WIDE ? 2 : 1];
+  uint4 q[TILES][TK];
+  int pos[TILES][2];  // of the lane's columns 2 c4, 2 c4 + 1
 #pragma unroll
-  for (int u = 0; u < (WIDE ? 2 : 1); ++u) {
+  for (int u = 0; u < TILES; ++u) {
     const int r = g8 + 8 * u, row = row0 + r, i = row % p.Nq, h = hk * p.G + row / p.Nq;
-    pos[u] = r < rows ? g.start + i : -1;
 #pragma unroll
     for (int t = 0; t < TK; ++t) {
       const int c = (4 * t + c4) * 8;
       q[u][t] = load16(static_cast<const bf16*>(p.q) + b * p.sq_b + i * p.sq_n + (long long)h * p.d + c, r < rows && c < p.d);
     }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int column = 2 * c4 + x + 8 * u;
+      pos[u][x] = column < rows ? g.start + (row0 + column) % p.Nq : -1;
+    }
   }
   const bf16* kp = static_cast<const bf16*>(p.k) + b * p.sk_b + (long long)hk * p.d + c4 * 8;
   const bf16* vp = static_cast<const bf16*>(p.v) + b * p.sv_b + (long long)hk * p.d + g8 * 8;
 
-  float o[TV * 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float o[TILES][TV * 4][4], m[TILES][2], l[TILES][2];
 #pragma unroll
-  for (int e = 0; e < TV * 8; ++e) o[e][0] = o[e][1] = o[e][2] = o[e][3] = 0.f;
+  for (int u = 0; u < TILES; ++u) {
+    m[u][0] = m[u][1] = -INFINITY;
+    l[u][0] = l[u][1] = 0.f;
+#pragma unroll
+    for (int e = 0; e < TV * 4; ++e) o[u][e][0] = o[u][e][1] = o[u][e][2] = o[u][e][3] = 0.f;
+  }
 
   for (int i = rank * kWarps + warp; i < kb.count; i += ranks * kWarps) {
     int limit;
@@ -157,69 +175,63 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attn_decode_kernel(const AttnP
 #pragma unroll
       for (int t = 0; t < TV; ++t) vf[n][t] = load16(vp + key * p.sv_n + 64 * t, key < limit && 64 * t + 8 * g8 < p.d);
     }
-    float s[2][4] = {};
+    uint32_t w[TILES][2];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int u = 0; u < TILES; ++u) {
+      float s[4] = {};  // keys g8 (0, 1) and g8 + 8 (2, 3), columns 2 c4 and 2 c4 + 1
 #pragma unroll
       for (int t = 0; t < TK; ++t)
 #pragma unroll
         for (int half = 0; half < 4; half += 2) {
-          const uint32_t a[4] = {word(q[0][t], half), WIDE ? word(q[WIDE ? 1 : 0][t], half) : 0u, word(q[0][t], half + 1),
-                                 WIDE ? word(q[WIDE ? 1 : 0][t], half + 1) : 0u};
-          mma_bf16(s[n], a, word(kf[n][t], half), word(kf[n][t], half + 1));
+          const uint32_t a[4] = {word(kf[0][t], half), word(kf[1][t], half), word(kf[0][t], half + 1), word(kf[1][t], half + 1)};
+          mma_bf16(s, a, word(q[u][t], half), word(q[u][t], half + 1));
         }
-    uint32_t a[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int u = 0; u < (WIDE ? 2 : 1); ++u) {
-      float mx = -INFINITY;
+      for (int x = 0; x < 2; ++x) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = key0 + 8 * n + 2 * c4 + e;
-          float& x = s[n][2 * u + e];
-          x = key < limit && sees(p, g.ctx, pos[u], key) ? x * p.scale_log2 : -INFINITY;
-          mx = fmaxf(mx, x);
+        for (int n = 0; n < 2; ++n) {
+          const int key = key0 + 8 * n + g8;
+          s[2 * n + x] = key < limit && sees(p, g.ctx, pos[u][x], key) ? s[2 * n + x] * p.scale_log2 : -INFINITY;
         }
-      mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-      const float now = fmaxf(m[u], mx), ref = now == -INFINITY ? 0.f : now, keep = ex2(m[u] - ref);
-      m[u] = now;
-      l[u] *= keep;
+        float mx = fmaxf(s[x], s[2 + x]);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float w0 = ex2(s[n][2 * u] - ref), w1 = ex2(s[n][2 * u + 1] - ref);
-        l[u] += w0 + w1;
-        a[2 * n + u] = pack(w0, w1);
+        for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, d));
+        const float now = fmaxf(m[u][x], mx), ref = now == -INFINITY ? 0.f : now, keep = ex2(m[u][x] - ref);
+        m[u][x] = now;
+        s[x] = ex2(s[x] - ref), s[2 + x] = ex2(s[2 + x] - ref);
+        l[u][x] = fmaf(l[u][x], keep, s[x] + s[2 + x]);
+#pragma unroll
+        for (int e = 0; e < TV * 4; ++e) o[u][e][x] *= keep, o[u][e][2 + x] *= keep;
       }
-#pragma unroll
-      for (int e = 0; e < TV * 8; ++e) o[e][2 * u] *= keep, o[e][2 * u + 1] *= keep;
+      w[u][0] = transpose8(pack(s[0], s[1]));
+      w[u][1] = transpose8(pack(s[2], s[3]));
     }
 #pragma unroll
     for (int t = 0; t < TV; ++t)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
-        mma_bf16(o[t * 8 + e], a, __byte_perm(word(vf[0][t], e / 2), word(vf[1][t], e / 2), sel),
-                 __byte_perm(word(vf[2][t], e / 2), word(vf[3][t], e / 2), sel));
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t a[4] = {__byte_perm(word(vf[0][t], e), word(vf[1][t], e), 0x5410), __byte_perm(word(vf[0][t], e), word(vf[1][t], e), 0x7632),
+                               __byte_perm(word(vf[2][t], e), word(vf[3][t], e), 0x5410), __byte_perm(word(vf[2][t], e), word(vf[3][t], e), 0x7632)};
+#pragma unroll
+        for (int u = 0; u < TILES; ++u) mma_bf16(o[u][t * 4 + e], a, w[u][0], w[u][1]);
       }
   }
-  // column 2 c4 + x of product (t, e) is feature (8 t + 2 c4 + x) * 8 + e
+  // row g8 and g8 + 8 of product (t, e) are features 64 t + 8 g8 + 2 e and the next one
 #pragma unroll
-  for (int u = 0; u < (WIDE ? 2 : 1); ++u) {
-    const int r = g8 + 8 * u;
-    l[u] += __shfl_xor_sync(~0u, l[u], 1);
-    l[u] += __shfl_xor_sync(~0u, l[u], 2);
-    if (c4 == 0) ms[warp * R + r] = m[u], ls[warp * R + r] = l[u];
+  for (int u = 0; u < TILES; ++u)
 #pragma unroll
-    for (int t = 0; t < TV; ++t)
+    for (int x = 0; x < 2; ++x) {
+      const int r = 2 * c4 + x + 8 * u;
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+      for (int d = 4; d < 32; d *= 2) l[u][x] += __shfl_xor_sync(~0u, l[u][x], d);
+      if (g8 == 0) ms[warp * R + r] = m[u][x], ls[warp * R + r] = l[u][x];
 #pragma unroll
-        for (int e = 0; e < 8; e += 4)
-          *reinterpret_cast<float4*>(Os + (warp * R + r) * DP + (8 * t + 2 * c4 + x) * 8 + e) =
-              make_float4(o[t * 8 + e][2 * u + x], o[t * 8 + e + 1][2 * u + x], o[t * 8 + e + 2][2 * u + x], o[t * 8 + e + 3][2 * u + x]);
-  }
+      for (int t = 0; t < TV; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2)
+          *reinterpret_cast<float4*>(Os + (warp * R + r) * DP + 64 * t + 8 * g8 + 2 * e) =
+              make_float4(o[u][t * 4 + e][x], o[u][t * 4 + e][2 + x], o[u][t * 4 + e + 1][x], o[u][t * 4 + e + 1][2 + x]);
+    }
   join<bf16, R, DP>(p, Os, ms, ls, rows, row0, hk, b);
 }
 
@@ -316,7 +328,9 @@ __global__ void __launch_bounds__(kWarps * 32) attn_decode_any_kernel(const Attn
   join<T, R, DP>(p, Os, ms, ls, rows, row0, hk, b);
 }
 
-// CTAs of a cluster: enough that the SMs have a CTA each, no more than the keys feed, blocks of `size` keys to a warp.
+// CTAs of a cluster: enough that the SMs have a CTA each, no more than the keys feed, blocks of `size` keys to a warp.  (64 rows of a cache
+// of 8192, windows of 4096, 8 heads of keys of 128: 184 us with clusters of 1 and 2, 197 of 4, 242 of 8; one row, windows of 1024: 16.7 us
+// with one CTA per head, 7.3 with clusters of 8.)
 template <typename K>
 cudaError_t launch(K kernel, const AttnParams& p, int R, int DP, int size, int sms, SmemGrant& grant, cudaStream_t st) {
   const size_t smem = sizeof(float) * kWarps * R * (DP + 2);
@@ -345,8 +359,8 @@ cudaError_t launch(K kernel, const AttnParams& p, int R, int DP, int size, int s
 template <int DP>
 cudaError_t run_bf16(const AttnParams& p, int sms, cudaStream_t st) {
   static SmemGrant g8, g16;
-  return p.G * p.Nq > 8 ? launch(attn_decode_kernel<DP, true>, p, 16, DP, 16, sms, g16, st)
-                        : launch(attn_decode_kernel<DP, false>, p, 8, DP, 16, sms, g8, st);
+  return p.G * p.Nq > 8 ? launch(attn_decode_kernel<DP, 2>, p, 16, DP, 16, sms, g16, st)
+                        : launch(attn_decode_kernel<DP, 1>, p, 8, DP, 16, sms, g8, st);
 }
 template <typename T, int DP>
 cudaError_t run_any(const AttnParams& p, int sms, cudaStream_t st) {
