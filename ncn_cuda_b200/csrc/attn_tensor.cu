@@ -248,6 +248,9 @@ __device__ __forceinline__ bool have_cleared(const Waiter& wait, uint64_t* go, u
   return wait.one(cleared, phase);
 }
 
+__device__ __forceinline__ void lds128(uint32_t at, uint32_t (&x)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at));
+}
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -283,7 +286,7 @@ __device__ __forceinline__ void exp2_pair(float& a, float& b, float2 scale, floa
   a = x.x, b = x.y;
 }
 // Results leave through shared memory and the TMA unit: rows written by their threads straight to global memory, 16 bytes per lane and
-// row, took a third of the forward's time in windows of 1024 (15000 of 51000 cycles; now 4000).  32 features of row r, c0 .. c0 + 31,
+// row, took a third of the forward's time in windows of 1024 (15000 of 51000 cycles).  32 features of row r, c0 .. c0 + 31,
 // into a tile laid out as the TMA unit has it.
 __device__ __forceinline__ void stage_row(uint32_t tile, int r, const float (&x)[32], float f, int c0) {
 #pragma unroll
@@ -293,6 +296,25 @@ __device__ __forceinline__ void stage_row(uint32_t tile, int r, const float (&x)
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(pack(x[e] * f, x[e + 1] * f)), "r"(pack(x[e + 2] * f, x[e + 3] * f)),
                  "r"(pack(x[e + 4] * f, x[e + 5] * f)), "r"(pack(x[e + 6] * f, x[e + 7] * f))
                  : "memory");
+  }
+}
+// The same for a warp's 32 rows by themselves (rows of 64 bytes), on their way when its lanes are done: no other warp is waited for.  Rows
+// and features beyond the tensor are left out.
+__device__ __forceinline__ void send_rows(const CUtensorMap* map, uint32_t at, const float (&x)[32], float f, int c, int head, int row, int b) {
+  const int lane = threadIdx.x % 32;
+  if (lane == 0) bulk_wait_read0();  // the place is free again
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 32; e += 8)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + lane * 64 + ((e / 8 ^ (lane >> 1 & 3)) << 4)),
+                 "r"(pack(x[e] * f, x[e + 1] * f)), "r"(pack(x[e + 2] * f, x[e + 3] * f)), "r"(pack(x[e + 4] * f, x[e + 5] * f)),
+                 "r"(pack(x[e + 6] * f, x[e + 7] * f))
+                 : "memory");
+  fence_proxy_async();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store(map, at, c, head, row, b);
+    bulk_commit();
   }
 }
 // what the rounding in stage_row takes off, to be staged itself
@@ -370,10 +392,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
   const uint32_t qs = smem_u32(base);
   float* const shared_row = reinterpret_cast<float*>(base + (2 + SLOTS) * TILE);  // [tile][half][row]
   uint64_t* const bars = reinterpret_cast<uint64_t*>(shared_row + 4 * kT);
-  uint64_t *const q_full = bars, *const s_full = bars + 1, *const p_half = bars + 3, *const p_ready = bars + 5, *const o_full = bars + 7, *const go = bars + 9, *const cleared = bars + 10,
-           *const staged = bars + 11, *const sent = bars + 13;
-  const Ring<SLOTS> ring{bars + 15, bars + 15 + SLOTS, qs + 2 * TILE, TILE};
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 15 + 2 * SLOTS);
+  uint64_t *const q_full = bars, *const s_full = bars + 1, *const p_half = bars + 3, *const p_ready = bars + 5, *const o_full = bars + 7, *const go = bars + 9, *const cleared = bars + 10;
+  const Ring<SLOTS> ring{bars + 11, bars + 11 + SLOTS, qs + 2 * TILE, TILE};
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 11 + 2 * SLOTS);
   volatile int* const stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
@@ -382,7 +403,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1), mbar_init(go, 1), mbar_init(cleared, 1);
     for (int x = 0; x < 2; ++x) mbar_init(s_full + x, 1), mbar_init(p_half + x, 2 * kT), mbar_init(p_ready + x, 2 * kT), mbar_init(o_full + x, 1);
-    for (int x = 0; x < 2; ++x) mbar_init(staged + x, 2 * kT), mbar_init(sent + x, 1);
     for (int i = 0; i < SLOTS; ++i) mbar_init(ring.full + i, 1), mbar_init(ring.empty + i, 1);
     fence_mbar_init();
     *stop = 0;
@@ -588,14 +608,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
       const bool some = mine > 0 && pos >= 0 && pos < end && !(l == 0.f);
       const float inv = some ? 1.f / l : 0.f;
       if (p.lse && half == 0 && qi < p.Nq) p.lse[((long long)b * p.H + h) * p.Nqp + qi] = some ? ref + log2f(l) : INFINITY;
-      // the tile's queries have been read by the last of its products (with no products, they may still be arriving)
-      const uint32_t tile = qs + x * TILE;
-      const int first = i0 + x * kT;
-      if (n > 0 && first < p.Nq) ok = wait(q_full, 0);
-      for (int pass = 0; ok && first < p.Nq && pass < (p.rest ? 2 : 1); ++pass) {
-        if (pass && !(ok = wait(sent + x, 0))) break;
+      // through the place of the tile's queries, 2 KB of it to a warp: the last of its products has read them (with no
+      // products, they may still be arriving)
+      const int row0 = i0 + x * kT + warp % 4 * 32;
+      if (n > 0 && i0 + x * kT < p.Nq) ok = wait(q_full, 0);
+      if (ok && row0 < p.Nq) {
+        const uint32_t place = qs + x * TILE + warp % 8 * 2048;
 #pragma unroll 1
-        for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
+        for (int c = half * (DP / 2); c < (half + 1) * (DP / 2) && c < p.d; c += 32) {
           float o[32];
           if (mine > 0) {
             tmem_load32f(to + c, o);
@@ -605,20 +625,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0.f;
           }
-          if (pass) keep_rest(o, inv);
-          stage_row(tile, r, o, pass ? 1.f : inv, c);
-        }
-        fence_proxy_async();
-        mbar_arrive(staged + x);
-        if (warp % 8 == 0) {
-          if (!(ok = wait(staged + x, pass))) break;
-          if (lane == 0) {
-            send_tile<DP>(pass ? &maps.rest : &maps.y, tile, h, first, b);
-            bulk_wait_read0();
-            mbar_arrive(sent + x);
+          send_rows(&maps.y, place, o, inv, c, h, row0, b);
+          if (p.rest) {
+            keep_rest(o, inv);
+            send_rows(&maps.rest, place, o, 1.f, c, h, row0, b);
           }
-          __syncwarp();
         }
+        if (lane == 0) bulk_wait_read0();
+        __syncwarp();
       }
     }
     tmem_before();
@@ -688,10 +702,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
       load_tile<DP>(qs, &maps.q, h, i0, b, q_full);
       load_tile<DP>(dys, &maps.dy, h, i0, b, q_full);
       typename Ring<SLOTS>::Place to;
+      for (int which = 0; which < 2; ++which) {  // y and its rest, for delta, in the ring's first places
+        mbar_expect_tx(ring.arrived(to), TILE);
+        load_tile<DP>(ring.at(to), which ? &maps.rest : &maps.y, h, i0, b, ring.arrived(to));
+        to.next();
+      }
       for (int i = 0; i < 2 * n; ++i) {
         if (!ring.wait_empty(wait, to)) {
           mbar_wait_bounded(q_full, 0, 1u << 16);
-          settle(ring, i);
+          settle(ring, i + 2);
           break;
         }
         mbar_expect_tx(ring.arrived(to), TILE);
@@ -700,11 +719,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
       }
     }
   } else if (warp == 10) {
-    if (clear && wait(go, 0)) clear_rows<DP>(ring.at(ring.place(2 * n - 2)), 0, g.ctx - kt.tile(n - 1) * kT, cleared);
+    if (clear && wait(go, 0)) clear_rows<DP>(ring.at(ring.place(2 * n)), 0, g.ctx - kt.tile(n - 1) * kT, cleared);
   } else if (warp == 8) {
     if (n > 0 && elect_one()) {
       typename Ring<SLOTS>::Place k_at, v_at, old_k;  // of the next scores, the next dP, the next dS
-      v_at.next();
+      k_at = old_k = ring.place(2), v_at = ring.place(3);
       auto scores = [&](int j) {  // of tile j into buffer j % 2
         if (!(ring.wait_full(wait, k_at) && (j + 1 < n || !clear || have_cleared(wait, go, cleared, 0)))) return false;
         product_scores<DP>(tmem + (j & 1) * kT, qs, ring.at(k_at));
@@ -738,56 +757,43 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
       if (ok) mma_commit(done);
     }
     __syncwarp();
-  } else {
+  } else {  // warps 0-7
     const int half = warp / 4, r = warp % 4 * 32 + lane, qi = i0 + r, pos = g.start + qi;
     const int end = min(g.ctx, g.start + p.Nq);
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     const int p_lo = g.start + i0, p_hi = p_lo + kT - 1;
     const bool live = pos >= 0 && pos < end;
     const long long head_row = ((long long)b * p.H + h) * p.Nqp + qi;
-    // delta = sum(dy * y) of every row: DP / 8 lanes read a row, so that a load takes whole rows; all of a thread's loads are under way at
-    // once (one after the other they took 17000 cycles, as long as eight tiles of keys).  dy is in shared memory already.
-    {
-      constexpr int LANES = DP / 8, ROWS = 32 / LANES, PASSES = 16 / ROWS;
-      const int c = lane % LANES * 8, row0 = warp * 16 + lane / LANES;
-      uint4 u[PASSES], t[PASSES];
-#pragma unroll
-      for (int pass = 0; pass < PASSES; ++pass) {
-        const int i = i0 + row0 + pass * ROWS;
-        const bool here = c < p.d && g.start + i >= 0 && g.start + i < end;
-        const long long y_row = ((long long)b * p.Nq + (here ? i : 0)) * p.H * p.d + (long long)h * p.d + (here ? c : 0);  // (in bounds)
-        u[pass] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.y_in) + y_row);
-        t[pass] = *reinterpret_cast<const uint4*>(p.rest + y_row);
-      }
-      if (n > 0) wait(q_full, 0);  // (given up: the waits that follow give up too)
-#pragma unroll
-      for (int pass = 0; pass < PASSES; ++pass) {
-        const int row = row0 + pass * ROWS, i = i0 + row;
-        float sum = 0.f;
-        if (n > 0 && c < p.d && g.start + i >= 0 && g.start + i < end) {
-          uint4 w;
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                       : "r"(dys + (c / 64) * kBlockBytes + row * 128 + ((c % 64 / 8 ^ (row & 7)) << 4)));
-          const uint32_t uu[4] = {u[pass].x, u[pass].y, u[pass].z, u[pass].w}, ww[4] = {w.x, w.y, w.z, w.w},
-                         tt[4] = {t[pass].x, t[pass].y, t[pass].z, t[pass].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            sum = fmaf(__uint_as_float(uu[e] << 16) + __uint_as_float(tt[e] << 16), __uint_as_float(ww[e] << 16), sum);
-            sum = fmaf(__uint_as_float(uu[e] & 0xffff0000u) + __uint_as_float(tt[e] & 0xffff0000u), __uint_as_float(ww[e] & 0xffff0000u), sum);
-          }
-        }
-#pragma unroll
-        for (int o = LANES / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-        if (c == 0) deltas[row] = sum;
-      }
-    }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    const float delta = deltas[r];
-    if (half == 0 && qi < p.Nq) p.delta[head_row] = delta;
     const float lse = live ? p.lse[head_row] : INFINITY;
     bool ok = true;
-    for (int j = 0; j < n; ++j) {
+    float delta = 0.f;
+    if (n > 0) {
+      // delta = sum(dy * y), of half of the row's features each.  All three are tiles that the TMA unit has fetched: read by the threads
+      // themselves, y and its rest took 9000 cycles longer (the cache that is left next to this much shared memory has no room for them).
+      ok = wait(q_full, 0) && wait(ring.full, 0) && wait(ring.full + 1, 0);
+      const uint32_t ys = qs + 2 * TILE, rests = ys + TILE;
+      float sum = 0.f;
+      if (ok && live) {
+#pragma unroll
+        for (int e = 0; e < DP / 2; e += 8) {
+          const int c = half * (DP / 2) + e;
+          const uint32_t off = (c / 64) * kBlockBytes + r * 128 + ((c % 64 / 8 ^ (r & 7)) << 4);
+          uint32_t u[4], t[4], w[4];
+          lds128(ys + off, u), lds128(rests + off, t), lds128(dys + off, w);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            sum = fmaf(__uint_as_float(u[x] << 16) + __uint_as_float(t[x] << 16), __uint_as_float(w[x] << 16), sum);
+            sum = fmaf(__uint_as_float(u[x] & 0xffff0000u) + __uint_as_float(t[x] & 0xffff0000u), __uint_as_float(w[x] & 0xffff0000u), sum);
+          }
+        }
+      }
+      deltas[half * kT + r] = sum;
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // (every warp comes here, whatever became of its waits)
+      if (threadIdx.x == 0) mbar_arrive(ring.empty), mbar_arrive(ring.empty + 1);
+      delta = deltas[r] + deltas[kT + r];
+      if (half == 0 && qi < p.Nq) p.delta[head_row] = delta;
+    }
+    for (int j = 0; ok && j < n; ++j) {
       const int k0 = kt.tile(j) * kT + half * 64;
       const uint32_t ts = tmem + (j & 1) * kT + half * 64 + lanes;
       if (!(ok = wait(s_full + (j & 1), (j >> 1) & 1))) break;
@@ -1023,7 +1029,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
       if (ok) mma_commit(done);
     }
     __syncwarp();
-  } else {
+  } else if (warp < 8) {
     const int half = warp / 4, r = warp % 4 * 32 + lane, key = k0 + r;
     const int end = min(g.ctx, g.start + p.Nq);
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16, ts = tmem + half * 64 + lanes, td = t_dp + half * 64 + lanes;
@@ -1177,15 +1183,16 @@ cudaError_t bind_context() {
   const cudaError_t e = cudaGetDevice(&dev);
   return e == cudaSuccess ? cudaSetDevice(dev) : e;
 }
-// [B, N, heads, d] with boxes of 128 positions x 64 features
-cudaError_t encode(CUtensorMap& m, const void* at, int d, int heads, int N, int B, long long sn, long long sb) {
+// [B, N, heads, d] with boxes of 128 positions x 64 features, or (of_warp) 32 x 32
+cudaError_t encode(CUtensorMap& m, const void* at, int d, int heads, int N, int B, long long sn, long long sb, bool of_warp = false) {
   const EncodeFn fn = encode_fn();
   if (!fn) return cudaErrorNotSupported;
   const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)N, (cuuint64_t)B};
   const cuuint64_t strides[3] = {(cuuint64_t)d * 2, (cuuint64_t)sn * 2, (cuuint64_t)sb * 2};
-  const cuuint32_t box[4] = {64, 1, kT, 1}, step[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {of_warp ? 32u : 64u, 1, of_warp ? 32u : (cuuint32_t)kT, 1}, step[4] = {1, 1, 1, 1};
   return fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(at), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+            of_warp ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
              ? cudaSuccess
              : cudaErrorInvalidValue;
 }
@@ -1218,11 +1225,13 @@ cudaError_t encode_all(Maps& m, const AttnParams& p, bool bwd) {
   if (e == cudaSuccess) e = encode(m.v, p.v, p.d, p.Hk, p.Nk, p.B, p.sv_n, p.sv_b);
   const long long En = (long long)p.H * p.d, Ek = (long long)p.Hk * p.d;  // results are contiguous
   if (!bwd) {
-    if (e == cudaSuccess) e = encode(m.y, p.y, p.d, p.H, p.Nq, p.B, En, En * p.Nq);
-    if (e == cudaSuccess && p.rest) e = encode(m.rest, p.rest, p.d, p.H, p.Nq, p.B, En, En * p.Nq);
+    if (e == cudaSuccess) e = encode(m.y, p.y, p.d, p.H, p.Nq, p.B, En, En * p.Nq, true);
+    if (e == cudaSuccess && p.rest) e = encode(m.rest, p.rest, p.d, p.H, p.Nq, p.B, En, En * p.Nq, true);
     return e;
   }
   if (e == cudaSuccess) e = encode(m.dy, p.dy, p.d, p.H, p.Nq, p.B, p.sdy_n, p.sdy_b);
+  if (e == cudaSuccess) e = encode(m.y, p.y_in, p.d, p.H, p.Nq, p.B, En, En * p.Nq);
+  if (e == cudaSuccess) e = encode(m.rest, p.rest, p.d, p.H, p.Nq, p.B, En, En * p.Nq);
   if (e == cudaSuccess) e = encode(m.dq, p.dq, p.d, p.H, p.Nq, p.B, En, En * p.Nq);
   if (e == cudaSuccess) e = encode(m.dk, p.dk, p.d, p.Hk, p.Nk, p.B, Ek, Ek * p.Nk);
   if (e == cudaSuccess) e = encode(m.dv, p.dv, p.d, p.Hk, p.Nk, p.B, Ek, Ek * p.Nk);
