@@ -38,33 +38,33 @@ template <typename T> struct Chunks {
 #pragma unroll
     for (int i = 0; i < V; ++i) a[i] = c[i] = make_uint4(0, 0, 0, 0);
   }
-  static __device__ __forceinline__ void widen(const uint4 (&r)[V], float (&x)[8]) {
+  static __device__ __forceinline__ void widen(const uint4 (&r)[V], float2 (&x)[4]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+      if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (sizeof(T) == 2) {
-          x[2 * e] = __uint_as_float(w[e] << 16);
-          x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-        } else {
-          x[4 * i + e] = __uint_as_float(w[e]);
-        }
+        for (int e = 0; e < 4; ++e) x[e] = make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+      } else {
+        x[2 * i] = make_float2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        x[2 * i + 1] = make_float2(__uint_as_float(w[2]), __uint_as_float(w[3]));
       }
     }
   }
-  static __device__ __forceinline__ void store(T* at, const float (&x)[8]) {
+  static __device__ __forceinline__ void store(T* at, const float2 (&x)[4]) {
     if constexpr (sizeof(T) == 2) {
       __nv_bfloat162 h[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      for (int i = 0; i < 4; ++i) h[i] = __float22bfloat162_rn(x[i]);
       *reinterpret_cast<uint4*>(at) = *reinterpret_cast<uint4*>(h);
     } else {
-      reinterpret_cast<float4*>(at)[0] = make_float4(x[0], x[1], x[2], x[3]);
-      reinterpret_cast<float4*>(at)[1] = make_float4(x[4], x[5], x[6], x[7]);
+      reinterpret_cast<float4*>(at)[0] = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
+      reinterpret_cast<float4*>(at)[1] = make_float4(x[2].x, x[2].y, x[3].x, x[3].y);
     }
   }
 };
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 minus(float2 x) { return make_float2(-x.x, -x.y); }
 
 template <int W>
 __device__ __forceinline__ float team_sum(float x) {
@@ -84,7 +84,8 @@ __global__ void __launch_bounds__(256, MODE == NORM_BWD ? 2 : 4) rotary_kernel(c
   wait_for_inputs();
   constexpr bool norm = MODE != PLAIN, norm_bwd = MODE == NORM_BWD;
   constexpr int TEAMS = 256 / W;
-  __shared__ __align__(16) float2 table[kRotaryTable];
+  __shared__ __align__(16) float table[2 * kRotaryTable];
+  __shared__ long long offs[norm_bwd ? 4 : 2][kRotarySpan];  // of the span's positions in q, k and their cotangents
   __shared__ __align__(16) float weight[norm ? 2 * 16 * W : 4];  // W <= 16: the first 2 W threads fill it
   const int lane = threadIdx.x % W, team = threadIdx.x / W, half = p.R / 2;
   const int turning = p.R / 16;
@@ -109,128 +110,153 @@ __global__ void __launch_bounds__(256, MODE == NORM_BWD ? 2 : 4) rotary_kernel(c
 #pragma unroll
       for (int e = 0; e < 4; ++e) weight[((team * 4 + j) * W + lane) * 4 + e] = p.t[team].w[(j < 2 ? c0 : c1) + j % 2 * 4 + e];
   }
-  float dw[2][16];  // (NORM_BWD)  of the tensor that is being worked on, of the other
+  // NORM_BWD: the sums for the weights of the tensor `of` that is being worked on; what a team has of either is kept in shared memory
+  __shared__ __align__(16) float kept[norm_bwd ? 2 : 1][norm_bwd ? TEAMS : 1][norm_bwd ? 16 * W : 4];
+  float2 dw[8];
+  int of = 0;
+  auto keep = [&]() {  // (the lane's own entries)
+    float2 *const u = reinterpret_cast<float2*>(&kept[of][team][c0]), *const v = reinterpret_cast<float2*>(&kept[of][team][c1]);
 #pragma unroll
-  for (int e = 0; e < 16; ++e) dw[0][e] = dw[1][e] = 0.f;
-  int of = 0;  // the former
+    for (int e = 0; e < 4; ++e) {
+      u[e] = __fadd2_rn(u[e], dw[e]), v[e] = __fadd2_rn(v[e], dw[4 + e]);
+      dw[e] = dw[4 + e] = both(0.f);
+    }
+  };
+  if constexpr (norm_bwd) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[e] = both(0.f);
+    if (active) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) kept[0][team][c0 + e] = kept[0][team][c1 + e] = kept[1][team][c0 + e] = kept[1][team][c1 + e] = 0.f;
+    }
+  }
   for (long long row0 = (long long)(blockIdx.x / p.parts) * p.span; row0 < rows; row0 += stride) {
     const int span = (int)min((long long)p.span, rows - row0), of_q = span * p.t[0].heads, count = of_q + span * p.t[1].heads;
     const int turns = (count + step - 1) / step;  // the same for every lane: shuffles
     Chunks<T> x_next, g_next;
-    auto place = [&](int i, int& which, int& at, int& h) {  // (i < 2^20: the product is off by less than what 0.5 leaves)
-      which = i >= of_q;
-      const int j = which ? i - of_q : i, heads = which ? p.t[1].heads : p.t[0].heads;
-      at = (int)((j + 0.5f) * (which ? inv[1] : inv[0]));
-      h = j - at * heads;
-    };
-    auto fetch = [&](int i) {
+    int which = 0, at = 0, h = 0, next_which, next_at, next_h;  // of the head that is worked on, of the next one
+    auto fetch = [&](int i, bool first_one) {
       x_next.clear();
       if (norm_bwd) g_next.clear();
+      // (i < 2^20: the product is off by less than what 0.5 leaves)
+      next_which = i >= of_q;
+      const int j = next_which ? i - of_q : i;
+      next_at = (int)((j + 0.5f) * (next_which ? inv[1] : inv[0]));
+      next_h = j - next_at * (next_which ? p.t[1].heads : p.t[0].heads);
       if (active && i < count) {
-        int which, at, h;
-        long long b, n;
-        place(i, which, at, h);
-        split(row0 + at, b, n);
-        const RotaryTensor& t = p.t[which];
-        x_next.load(static_cast<const T*>(t.x) + b * t.sb + n * t.sn + (long long)h * p.d, c0, c1);
-        if (norm_bwd) g_next.load(static_cast<const T*>(t.dy) + b * t.gb + n * t.gn + (long long)h * p.d, c0, c1);
+        const RotaryTensor& t = p.t[next_which];
+        long long xo, go = 0;
+        if (first_one) {
+          long long b, n;
+          split(row0 + next_at, b, n);
+          xo = b * t.sb + n * t.sn, go = b * t.gb + n * t.gn;
+        } else {
+          xo = offs[next_which][next_at];
+          if (norm_bwd) go = offs[2 + next_which][next_at];
+        }
+        x_next.load(static_cast<const T*>(t.x) + xo + next_h * p.d, c0, c1);
+        if (norm_bwd) g_next.load(static_cast<const T*>(t.dy) + go + next_h * p.d, c0, c1);
       }
     };
-    fetch(first);
+    fetch(first, true);
     __syncthreads();  // (the span before is done with the sines)
     for (int e = threadIdx.x; e < span * half; e += 256) {
-      const int at = e / half;
+      const int pos_at = e / half, pair = e - pos_at * half;
       long long b, n;
-      split(row0 + at, b, n);
-      const int pair = e - at * half;
-      table[at * half + (pair % 8 / 2 * turning + pair / 8) * 2 + pair % 2] = cos_sin(p, p.pos ? p.pos[b * p.pos_b + n] : p.start + n, pair);
+      split(row0 + pos_at, b, n);
+      const float2 cs = cos_sin(p, p.pos ? p.pos[b * p.pos_b + n] : p.start + n, pair);
+      // of a lane's 8 pairs: two words of four cosines, two of four sines
+      float* const to = table + pos_at * p.R + (pair % 8 / 4 * turning + pair / 8) * 4 + pair % 4;
+      to[0] = cs.x;
+      to[8 * turning] = cs.y;
+    }
+    if (threadIdx.x < span) {
+      long long b, n;
+      split(row0 + threadIdx.x, b, n);
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        offs[w][threadIdx.x] = b * p.t[w].sb + n * p.t[w].sn;
+        if (norm_bwd) offs[2 + w][threadIdx.x] = b * p.t[w].gb + n * p.t[w].gn;
+      }
     }
     __syncthreads();
     for (int k = 0; k < turns; ++k) {
       const int i = first + k * step;
       const bool here = active && i < count;
-      int which, at, h;
-      place(i, which, at, h);
+      which = next_which, at = next_at, h = next_h;
       const float4* w = reinterpret_cast<const float4*>(weight) + which * 4 * W + lane;
-      float a[8], c[8], ga[8], gc[8];
+      float2 a[4], c[4], ga[4], gc[4];
       Chunks<T>::widen(x_next.a, a);
       Chunks<T>::widen(x_next.c, c);
       if (norm_bwd) {
         Chunks<T>::widen(g_next.a, ga);
         Chunks<T>::widen(g_next.c, gc);
       }
-      if (k + 1 < turns) fetch(i + step);
+      if (k + 1 < turns) fetch(i + step, false);
       float r = 1.f;
       if (norm) {
-        float sq = 0.f;
+        float2 sq = both(0.f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sq = fmaf(a[e], a[e], fmaf(c[e], c[e], sq));
-        r = rsqrtf(team_sum<W>(sq) * inv_d + p.eps);
+        for (int e = 0; e < 4; ++e) sq = __ffma2_rn(a[e], a[e], __ffma2_rn(c[e], c[e], sq));
+        r = rsqrtf(team_sum<W>(sq.x + sq.y) * inv_d + p.eps);
         if (!here) r = 0.f;  // (infinite where eps is 0)
       }
-      float wa[8], wc[8];
+      float2 wa[4], wc[4];
       if (norm) {
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-          const float4 u = here ? w[e / 4 * W] : make_float4(0, 0, 0, 0), v = here ? w[(2 + e / 4) * W] : make_float4(0, 0, 0, 0);
-          wa[e] = u.x, wa[e + 1] = u.y, wa[e + 2] = u.z, wa[e + 3] = u.w;
-          wc[e] = v.x, wc[e + 1] = v.y, wc[e + 2] = v.z, wc[e + 3] = v.w;
+        for (int e = 0; e < 2; ++e) {
+          const float4 u = w[e * W], v = w[(2 + e) * W];
+          wa[2 * e] = make_float2(u.x, u.y), wa[2 * e + 1] = make_float2(u.z, u.w);
+          wc[2 * e] = make_float2(v.x, v.y), wc[2 * e + 1] = make_float2(v.z, v.w);
         }
       }
       if (!norm_bwd) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          ga[e] = norm ? a[e] * r * wa[e] : a[e];
-          gc[e] = norm ? c[e] * r * wc[e] : c[e];
+        for (int e = 0; e < 4; ++e) {
+          ga[e] = norm ? __fmul2_rn(a[e], __fmul2_rn(both(r), wa[e])) : a[e];
+          gc[e] = norm ? __fmul2_rn(c[e], __fmul2_rn(both(r), wc[e])) : c[e];
         }
       }
       if (turn && here) {
-        const float4* tab = reinterpret_cast<const float4*>(table + at * half) + lane;  // (entry e: the lane's pairs 2 e, 2 e + 1)
-        if (p.interleaved) {
+        const float4* tab = reinterpret_cast<const float4*>(table + at * p.R) + lane;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float4 s = tab[e * turning], u = tab[(2 + e) * turning];
-            float y0 = ga[4 * e], y1 = ga[4 * e + 1];
-            ga[4 * e] = y0 * s.x - y1 * s.y, ga[4 * e + 1] = y1 * s.x + y0 * s.y;
-            y0 = ga[4 * e + 2], y1 = ga[4 * e + 3];
-            ga[4 * e + 2] = y0 * s.z - y1 * s.w, ga[4 * e + 3] = y1 * s.z + y0 * s.w;
-            y0 = gc[4 * e], y1 = gc[4 * e + 1];
-            gc[4 * e] = y0 * u.x - y1 * u.y, gc[4 * e + 1] = y1 * u.x + y0 * u.y;
-            y0 = gc[4 * e + 2], y1 = gc[4 * e + 3];
-            gc[4 * e + 2] = y0 * u.z - y1 * u.w, gc[4 * e + 3] = y1 * u.z + y0 * u.w;
-          }
-        } else {
+        for (int q = 0; q < 2; ++q) {
+          const float4 cw = tab[q * turning], sw = tab[(2 + q) * turning];
+          if (p.interleaved) {  // pairs 4 q .. 4 q + 3: a's for q = 0, c's for q = 1
+            float2(&g)[4] = q ? gc : ga;
+            const float cs[4] = {cw.x, cw.y, cw.z, cw.w}, sn[4] = {sw.x, sw.y, sw.z, sw.w};
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const float4 s = tab[e / 2 * turning];
-            float a0 = ga[e], b0 = gc[e];
-            ga[e] = a0 * s.x - b0 * s.y, gc[e] = b0 * s.x + a0 * s.y;
-            a0 = ga[e + 1], b0 = gc[e + 1];
-            ga[e + 1] = a0 * s.z - b0 * s.w, gc[e + 1] = b0 * s.z + a0 * s.w;
+            for (int e = 0; e < 4; ++e) g[e] = make_float2(g[e].x * cs[e] - g[e].y * sn[e], g[e].y * cs[e] + g[e].x * sn[e]);
+          } else {
+            const float2 cs[2] = {make_float2(cw.x, cw.y), make_float2(cw.z, cw.w)}, sn[2] = {make_float2(sw.x, sw.y), make_float2(sw.z, sw.w)};
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float2 u = ga[2 * q + e], v = gc[2 * q + e];
+              ga[2 * q + e] = __ffma2_rn(u, cs[e], minus(__fmul2_rn(v, sn[e])));
+              gc[2 * q + e] = __ffma2_rn(v, cs[e], __fmul2_rn(u, sn[e]));
+            }
           }
         }
       }
       if (norm_bwd) {
         if (here && which != of) {  // from the queries to the keys, or to the next span's queries
+          keep();
           of = which;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float t = dw[0][e];
-            dw[0][e] = dw[1][e];
-            dw[1][e] = t;
-          }
         }
-        float dot = 0.f;
+        float2 dot = both(0.f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          a[e] *= r, c[e] *= r;  // x r
-          dw[0][e] = fmaf(ga[e], a[e], dw[0][e]), dw[0][8 + e] = fmaf(gc[e], c[e], dw[0][8 + e]);  // (zeros where nothing is)
-          ga[e] *= wa[e], gc[e] *= wc[e];
-          dot = fmaf(ga[e], a[e], fmaf(gc[e], c[e], dot));
+        for (int e = 0; e < 4; ++e) {
+          a[e] = __fmul2_rn(a[e], both(r)), c[e] = __fmul2_rn(c[e], both(r));  // x r
+          dw[e] = __ffma2_rn(ga[e], a[e], dw[e]), dw[4 + e] = __ffma2_rn(gc[e], c[e], dw[4 + e]);  // (zeros where nothing is)
+          ga[e] = __fmul2_rn(ga[e], wa[e]), gc[e] = __fmul2_rn(gc[e], wc[e]);
+          dot = __ffma2_rn(ga[e], a[e], __ffma2_rn(gc[e], c[e], dot));
         }
-        const float mean = team_sum<W>(dot) * inv_d;
+        const float2 mean = both(-team_sum<W>(here ? dot.x + dot.y : 0.f) * inv_d);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ga[e] = r * (ga[e] - a[e] * mean), gc[e] = r * (gc[e] - c[e] * mean);
+        for (int e = 0; e < 4; ++e) {
+          ga[e] = __fmul2_rn(both(r), __ffma2_rn(a[e], mean, ga[e]));
+          gc[e] = __fmul2_rn(both(r), __ffma2_rn(c[e], mean, gc[e]));
+        }
       }
       if (here) {
         const RotaryTensor& t = p.t[which];
@@ -241,21 +267,20 @@ __global__ void __launch_bounds__(256, MODE == NORM_BWD ? 2 : 4) rotary_kernel(c
     }
   }
   if constexpr (norm_bwd) {  // the CTA's sums, team after team
-    __shared__ float red[TEAMS][16 * W + 1];
+    if (active) keep();
+    __syncthreads();
+    // WAYS threads per column, then their sums
+    constexpr int COLUMNS = 16 * W, WAYS = 256 / COLUMNS;
+    const int c = threadIdx.x % COLUMNS, way = threadIdx.x / COLUMNS;
     for (int which = 0; which < 2; ++which) {
       if (!p.t[which].heads) continue;
+      float sum = 0.f;
+      for (int i = way; i < TEAMS; i += WAYS) sum += kept[which][i][c];
       __syncthreads();
-      if (active) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          red[team][c0 + e] = which == of ? dw[0][e] : dw[1][e];
-          red[team][c1 + e] = which == of ? dw[0][8 + e] : dw[1][8 + e];
-        }
-      }
+      kept[which][way][c] = sum;  // (over what this way alone has read)
       __syncthreads();
-      for (int c = threadIdx.x; c < p.d; c += 256) {
-        float sum = 0.f;
-        for (int i = 0; i < TEAMS; ++i) sum += red[i][c];
+      if (way == 0 && c < p.d) {
+        for (int i = 1; i < WAYS; ++i) sum += kept[which][i][c];
         p.partial[((long long)which * gridDim.x + blockIdx.x) * p.d + c] = sum;
       }
     }
@@ -384,8 +409,10 @@ cudaError_t by_width(const RotaryParams& p, int grid, cudaStream_t st) {
 
 }  // namespace
 
-// Positions that a CTA takes at a time, CTAs that share one position's heads, and CTAs.  A span is as long as leaves 8 CTAs per SM
-// (the last ones are not waited for long), its sines are formed once; with few positions their heads are spread out, a team each.  The
+// Positions that a CTA takes at a time, CTAs that share one position's heads, and CTAs.  Sines, launch and first loads are the same for
+// any span, so a span is as long as leaves two CTAs per SM (5997 positions, 18 heads of 96: 31.5 us with one position per CTA, 16.6 where 8
+// CTAs are left per SM, 14.0 with 2; 32768 positions of 40 heads of 128: the same from 2 to 8, 26 % slower with one position), or half a
+// one where its heads would not give each team one; with few positions their heads are spread out, a team each.  The
 // backward of a norm takes 4 CTAs per SM at most, each with several spans: every CTA leaves a row of sums behind.
 int rotary_plan(RotaryParams& p, int sms) {
   const long long rows = (long long)p.B * p.N, heads = p.t[0].heads;
@@ -393,7 +420,8 @@ int rotary_plan(RotaryParams& p, int sms) {
   p.span = p.parts = 1;
   if (in_chunks(p)) {
     const int teams = 256 / team_width(p), most = p.R ? kRotaryTable / (p.R / 2) : kRotarySpan;
-    while (2 * p.span <= most && 2 * p.span <= kRotarySpan && rows / (2 * p.span) >= 8ll * sms) p.span *= 2;
+    auto doubled = [&](long long ctas_left) { return 2 * p.span <= most && 2 * p.span <= kRotarySpan && 2 * rows / (2 * p.span) >= ctas_left; };
+    while (doubled(4ll * sms) || (p.span * (heads + p.t[1].heads) < teams && doubled(sms))) p.span *= 2;
     const long long spans = (rows + p.span - 1) / p.span;
     while (p.parts * teams < heads && spans * p.parts < 4ll * sms) ++p.parts;
     ctas = spans * p.parts;
