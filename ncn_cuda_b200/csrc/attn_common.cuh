@@ -84,6 +84,12 @@ __device__ __forceinline__ bool sees(const AttnParams& p, int ctx, int pos, int 
   return key <= pos && pos < ctx && (pos - key < p.window || key < p.n_sink);
 }
 
+// whether queries i0 .. i0 + n - 1 see all of keys k0 .. k0 + m - 1
+__device__ __forceinline__ bool sees_all(const AttnParams& p, const RowGeom& g, int i0, int n, int k0, int m) {
+  const int lo = g.start + i0, hi = lo + n - 1;
+  return i0 + n <= p.Nq && k0 + m - 1 <= lo && hi < g.ctx && (k0 > hi - p.window || k0 + m <= p.n_sink);
+}
+
 // Work items of the backward of the keys.  Item x < key tiles: the queries within reach of tile x's window (all of their pairs with
 // the tile, sinks included).  Beyond these: piece c of the queries that see only the sinks of sink tile st.
 // Query tiles of size TQ; `first .. last` of each of the G heads of the group, entries [begin, end) of the list head * tiles + tile.

@@ -148,15 +148,18 @@ __global__ void __launch_bounds__(256) attn_simt_fwd_kernel(const AttnParams p) 
     __syncthreads();
     float s[4][CJ] = {};
     rows_by_rows<DP, CJ>(Q, K, s);
+    if (!sees_all(p, g, i0, kOwn, k0, BN)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < CJ; ++j)
+          if (!sees(p, g.ctx, g.start + i0 + 4 * ty + i, k0 + tx + 16 * j)) s[i][j] = -INFINITY;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int pos = g.start + i0 + 4 * ty + i;
       float mx = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < CJ; ++j) {
-        if (!sees(p, g.ctx, pos, k0 + tx + 16 * j)) s[i][j] = -INFINITY;
-        mx = fmaxf(mx, s[i][j]);
-      }
+      for (int j = 0; j < CJ; ++j) mx = fmaxf(mx, s[i][j]);
       const float now = fmaxf(m[i], max16(mx));
       const float ref = now == -INFINITY ? 0.f : now * p.scale_log2;
       const float keep = m[i] == -INFINITY ? 0.f : ex2(m[i] * p.scale_log2 - ref);
@@ -241,13 +244,14 @@ __global__ void __launch_bounds__(256) attn_simt_dq_kernel(const AttnParams p) {
     float s[4][CJ] = {}, dp[4][CJ] = {};
     rows_by_rows<DP, CJ>(Q, K, s);
     rows_by_rows<DP, CJ>(dO, V, dp);
+    const bool all = sees_all(p, g, i0, kOwn, k0, BN);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int pos = g.start + i0 + 4 * ty + i;
 #pragma unroll
       for (int j = 0; j < CJ; ++j) {
         const float w = ex2(fmaf(s[i][j], p.scale_log2, -lse[i]));
-        S[(4 * ty + i) * (BN + 4) + tx + 16 * j] = sees(p, g.ctx, pos, k0 + tx + 16 * j) ? w * (dp[i][j] - delta[i]) : 0.f;
+        S[(4 * ty + i) * (BN + 4) + tx + 16 * j] = all || sees(p, g.ctx, pos, k0 + tx + 16 * j) ? w * (dp[i][j] - delta[i]) : 0.f;
       }
     }
     __syncwarp();
@@ -304,6 +308,7 @@ __global__ void __launch_bounds__(256) attn_simt_dkv_kernel(const AttnParams p) 
     float s[4][CJ] = {}, dp[4][CJ] = {};
     rows_by_rows<DP, CJ>(K, Q, s);
     rows_by_rows<DP, CJ>(V, dO, dp);
+    const bool all = sees_all(p, g, i0, BN, k0, kOwn);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int key = k0 + 4 * ty + i;
@@ -311,7 +316,7 @@ __global__ void __launch_bounds__(256) attn_simt_dkv_kernel(const AttnParams p) 
       for (int j = 0; j < CJ; ++j) {
         const int c = tx + 16 * j;
         float w = ex2(fmaf(s[i][j], p.scale_log2, -lse_s[c])), t = w * (dp[i][j] - del_s[c]);
-        if (!sees(p, g.ctx, g.start + i0 + c, key)) w = t = 0.f;
+        if (!all && !sees(p, g.ctx, g.start + i0 + c, key)) w = t = 0.f;
         P[(4 * ty + i) * (BN + 4) + c] = w;
         S[(4 * ty + i) * (BN + 4) + c] = t;
       }
