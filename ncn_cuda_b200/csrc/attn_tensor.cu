@@ -14,8 +14,6 @@
 // return no sum depends on the order in which CTAs finish.
 #include <cuda.h>
 
-#include <type_traits>
-
 #include "attn_tensor.h"
 #include "ncn_common.cuh"
 
@@ -258,8 +256,7 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 // Exponentials.  The special-function pipe gives 16 per SM and cycle, 1024 cycles per tile of 128 x 128, as long as both products of heads
 // of 128 take; so some pairs (kOnFma of 8) are computed on the FMA pipe instead, two at a time: 2^x = 2^n 2^f, n the nearest whole number,
 // |f| <= 1/2, 2^f by the polynomial of degree 4 of least relative error (Remez exchange; 2.6e-6 = 2^-18.6, a thousandth of the weights'
-// rounding to bf16).  Below 2^-120 the result is 2^-120 rather than less, so masked scores (-inf) go to the other pipe: tiles with a mask
-// do entirely.  NaN stays NaN.
+// rounding to bf16).  Below 2^-120 the result is 2^-120 rather than less: masks are laid over the weights, not the scores.  NaN stays NaN.
 constexpr int kOnFma = 3;
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-120.f));
@@ -275,11 +272,10 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
   const float2 two_n = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000));
   return __fmul2_rn(p, two_n);
 }
-// s[e] = 2^(s[e] * scale + bias)
-template <bool MIX>
+// a, b = 2^(a scale + bias), 2^(b scale + bias); pair: its number
 __device__ __forceinline__ void exp2_pair(float& a, float& b, float2 scale, float2 bias, int pair) {
   float2 x = __ffma2_rn(make_float2(a, b), scale, bias);
-  if (MIX && pair % 8 < kOnFma)
+  if (pair % 8 < kOnFma)
     x = exp2_fma(x);
   else
     x = make_float2(ex2(x.x), ex2(x.y));
@@ -363,7 +359,10 @@ __device__ __forceinline__ Columns columns_of(const AttnParams& p, int pos, int 
   c.sink = p.n_sink - k0;
   return c;
 }
-__device__ __forceinline__ bool visible(const Columns& c, int x) { return x < c.hi && (x >= c.lo || x < c.sink); }
+// columns x .. x + 31 as bits.  Every tile goes through the same code, and one with a mask through a few selections more: code of its own
+// for masked tiles, in short windows met once or twice per CTA, is fetched as often as it is run.
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; }
+__device__ __forceinline__ uint32_t visible32(const Columns& c, int x) { return below(c.hi - x) & (~below(c.lo - x) | below(c.sink - x)); }
 
 // ------------------------------------------------------------------ forward
 // Two tiles of 128 queries per CTA, eight warps each: while one's scores are exponentiated, the other's products run.  Two threads own a
@@ -525,10 +524,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
         tmem_loaded(s);
         if (!whole) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t bits = visible32(col, 32 * c);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!visible(col, 32 * c + e)) s[c][e] = -INFINITY;
+            for (int e = 0; e < 32; ++e) s[c][e] = bits & (1u << e) ? s[c][e] : -INFINITY;
+          }
         }
         float mx[4];
 #pragma unroll
@@ -562,36 +562,33 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
       const float bias = ref == -INFINITY ? 0.f : ref;
       const float2 bias2 = make_float2(-bias, -bias);
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      auto weights = [&](auto mix) {
-        float s[2][16];
-        tmem_load16f(ts, s[0]);
+      float s[2][16];
+      tmem_load16f(ts, s[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {  // the weights of scores 16 c .. lie over scores 8 c .., which have been used
-          tmem_loaded(s[c % 2]);
-          if (c < 3) tmem_load16f(ts + 16 * (c + 1), s[(c + 1) % 2]);
-          uint32_t w[8];
-          float(&t)[16] = s[c % 2];
-          if (!decltype(mix)::value) {
+      for (int c = 0; c < 4; ++c) {  // the weights of scores 16 c .. lie over scores 8 c .., which have been used
+        float(&t)[16] = s[c % 2];
+        tmem_loaded(t);
+        if (c < 3) tmem_load16f(ts + 16 * (c + 1), s[(c + 1) % 2]);
+        uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (!visible(col, 16 * c + e)) t[e] = -INFINITY;
-          }
+        for (int e = 0; e < 16; e += 2) exp2_pair(t[e], t[e + 1], scale2, bias2, e / 2);
+        if (!whole) {
+          const uint32_t bits = visible32(col, 16 * c);
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            exp2_pair<decltype(mix)::value>(t[e], t[e + 1], scale2, bias2, e / 2);
-            sum[e / 2 % 2] = __fadd2_rn(sum[e / 2 % 2], make_float2(t[e], t[e + 1]));
-            w[e / 2] = pack(t[e], t[e + 1]);
-          }
-          tmem_store8(ts + 8 * c, w);
-          if (c == 1) {
-            tmem_stored();
-            tmem_before();
-            mbar_arrive(p_half + x);
-          }
+          for (int e = 0; e < 16; ++e) t[e] = bits & (1u << e) ? t[e] : 0.f;
         }
-      };
-      if (whole) weights(std::true_type());
-      else weights(std::false_type());
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          sum[e / 2 % 2] = __fadd2_rn(sum[e / 2 % 2], make_float2(t[e], t[e + 1]));
+          w[e / 2] = pack(t[e], t[e + 1]);
+        }
+        tmem_store8(ts + 8 * c, w);
+        if (c == 1) {
+          tmem_stored();
+          tmem_before();
+          mbar_arrive(p_half + x);
+        }
+      }
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       tmem_stored();
       tmem_before();
@@ -765,6 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
     const bool live = pos >= 0 && pos < end;
     const long long head_row = ((long long)b * p.H + h) * p.Nqp + qi;
     const float lse = live ? p.lse[head_row] : INFINITY;
+    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
     float delta = 0.f;
     if (n > 0) {
@@ -798,21 +796,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
       const uint32_t ts = tmem + (j & 1) * kT + half * 64 + lanes;
       if (!(ok = wait(s_full + (j & 1), (j >> 1) & 1))) break;
       tmem_after();
+      const bool whole = k0 + 63 <= p_lo && p_hi < end && k0 + 64 <= g.ctx && (k0 > p_hi - p.window || k0 + 64 <= p.n_sink);
+      const Columns col = columns_of(p, pos, end, k0);
+      const float2 bias2 = make_float2(-lse, -lse), delta2 = make_float2(-delta, -delta);
       float s[2][32];
       tmem_load32f(ts, s[0]);
       tmem_load32f(ts + 32, s[1]);
       tmem_loaded(s);
-      const bool whole = k0 + 63 <= p_lo && p_hi < end && k0 + 64 <= g.ctx && (k0 > p_hi - p.window || k0 + 64 <= p.n_sink);
-      const Columns col = columns_of(p, pos, end, k0);
-      const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), bias2 = make_float2(-lse, -lse);
-      auto weights = [&](auto mix) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) exp2_pair<decltype(mix)::value>(s[c][e], s[c][e + 1], scale2, bias2, e / 2);
-      };
-      if (whole) weights(std::true_type());
-      else weights(std::false_type());
+        for (int e = 0; e < 32; e += 2) exp2_pair(s[c][e], s[c][e + 1], scale2, bias2, e / 2);
       if (!(ok = wait(dp_full, j & 1))) break;
       tmem_after();
 #pragma unroll
@@ -821,15 +815,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
         uint32_t w[16];
         tmem_load32f(t_dp + half * 64 + 32 * c + lanes, dp);
         tmem_loaded(dp);
-        if (whole) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 t = __fmul2_rn(make_float2(s[c][e], s[c][e + 1]), __fadd2_rn(make_float2(dp[e], dp[e + 1]), make_float2(-delta, -delta)));
-            dp[e] = t.x, dp[e + 1] = t.y;
-          }
-        } else {
+        for (int e = 0; e < 32; e += 2) {
+          const float2 t = __fmul2_rn(make_float2(s[c][e], s[c][e + 1]), __fadd2_rn(make_float2(dp[e], dp[e + 1]), delta2));
+          dp[e] = t.x, dp[e + 1] = t.y;
+        }
+        if (!whole) {
+          const uint32_t bits = visible32(col, 32 * c);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) dp[e] = visible(col, 32 * c + e) ? s[c][e] * (dp[e] - delta) : 0.f;
+          for (int e = 0; e < 32; ++e) dp[e] = bits & (1u << e) ? dp[e] : 0.f;
         }
 #pragma unroll
         for (int e = 0; e < 32; e += 2) w[e / 2] = pack(dp[e], dp[e + 1]);
@@ -1033,6 +1027,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
     const int half = warp / 4, r = warp % 4 * 32 + lane, key = k0 + r;
     const int end = min(g.ctx, g.start + p.Nq);
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16, ts = tmem + half * 64 + lanes, td = t_dp + half * 64 + lanes;
+    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
     for (int i = 0; i < n; ++i) {
       const int first = g.start + entry.row() + half * 64;  // position of column 0
@@ -1050,21 +1045,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t w[16];
-        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
-        auto weights = [&](auto mix) {
+        const uint32_t bits = below(hi - 32 * c) & ~below(lo - 32 * c);
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 ls = *reinterpret_cast<const float4*>(lse + 32 * c + e);
-            exp2_pair<decltype(mix)::value>(s[c][e], s[c][e + 1], scale2, make_float2(-ls.x, -ls.y), e / 2);
-            exp2_pair<decltype(mix)::value>(s[c][e + 2], s[c][e + 3], scale2, make_float2(-ls.z, -ls.w), e / 2 + 1);
-          }
-        };
-        if (whole) weights(std::true_type());
-        else weights(std::false_type());
+        for (int e = 0; e < 32; e += 4) {
+          const float4 ls = *reinterpret_cast<const float4*>(lse + 32 * c + e);
+          exp2_pair(s[c][e], s[c][e + 1], scale2, make_float2(-ls.x, -ls.y), e / 2);
+          exp2_pair(s[c][e + 2], s[c][e + 3], scale2, make_float2(-ls.z, -ls.w), e / 2 + 1);
+        }
         if (!whole) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (32 * c + e < lo || 32 * c + e >= hi) s[c][e] = 0.f;
+          for (int e = 0; e < 32; ++e) s[c][e] = bits & (1u << e) ? s[c][e] : 0.f;
         }
 #pragma unroll
         for (int e = 0; e < 32; e += 2) w[e / 2] = pack(s[c][e], s[c][e + 1]);
@@ -1089,9 +1079,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
           dp[e] = t.x, dp[e + 1] = t.y, dp[e + 2] = u.x, dp[e + 3] = u.y;
         }
         if (!whole) {
+          const uint32_t bits = below(hi - 32 * c) & ~below(lo - 32 * c);
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (32 * c + e < lo || 32 * c + e >= hi) dp[e] = 0.f;
+          for (int e = 0; e < 32; ++e) dp[e] = bits & (1u << e) ? dp[e] : 0.f;
         }
 #pragma unroll
         for (int e = 0; e < 32; e += 2) w[e / 2] = pack(dp[e], dp[e + 1]);
