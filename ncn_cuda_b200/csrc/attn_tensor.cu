@@ -254,10 +254,10 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 // Exponentials.  The special-function pipe gives 16 per SM and cycle, 1024 cycles per tile of 128 x 128, as long as both products of heads
-// of 128 take; so some pairs (kOnFma of 8) are computed on the FMA pipe instead, two at a time: 2^x = 2^n 2^f, n the nearest whole number,
+// of 128 take; so some pairs (kOnFma of 8; 2 and 3 measured best, 0 and 4 two to four per cent slower) are computed on the FMA pipe instead, two at a time: 2^x = 2^n 2^f, n the nearest whole number,
 // |f| <= 1/2, 2^f by the polynomial of degree 4 of least relative error (Remez exchange; 2.6e-6 = 2^-18.6, a thousandth of the weights'
 // rounding to bf16).  Below 2^-120 the result is 2^-120 rather than less: masks are laid over the weights, not the scores.  NaN stays NaN.
-constexpr int kOnFma = 3;
+constexpr int kOnFma = 2;
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-120.f));
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-120.f));
