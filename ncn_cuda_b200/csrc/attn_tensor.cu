@@ -133,7 +133,6 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
                "l"(map), "r"(c), "r"(head), "r"(row), "r"(b), "r"(smem_u32(bar))
                : "memory");
 }
-__device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int c, int head, int row, int b) {
   asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(src), "r"(c), "r"(head),
                "r"(row), "r"(b)
@@ -295,10 +294,11 @@ __device__ __forceinline__ void stage_row(uint32_t tile, int r, const float (&x)
   }
 }
 // The same for a warp's 32 rows by themselves (rows of 64 bytes), on their way when its lanes are done: no other warp is waited for.  Rows
-// and features beyond the tensor are left out.
+// and features beyond the tensor are left out.  OTHERS: how many of the sends before may still be reading, from other places.
+template <int OTHERS>
 __device__ __forceinline__ void send_rows(const CUtensorMap* map, uint32_t at, const float (&x)[32], float f, int c, int head, int row, int b) {
   const int lane = threadIdx.x % 32;
-  if (lane == 0) bulk_wait_read0();  // the place is free again
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(OTHERS) : "memory");
   __syncwarp();
 #pragma unroll
   for (int e = 0; e < 32; e += 8)
@@ -365,7 +365,8 @@ __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0
 __device__ __forceinline__ uint32_t visible32(const Columns& c, int x) { return below(c.hi - x) & (~below(c.lo - x) | below(c.sink - x)); }
 
 // ------------------------------------------------------------------ forward
-// Two tiles of 128 queries per CTA, eight warps each: while one's scores are exponentiated, the other's products run.  Two threads own a
+// Two tiles of 128 queries per CTA: of two heads that share their keys (the tiles need the same ones, at the same time), or, where heads
+// do not come in such pairs, one behind the other (the second starts one tile of keys later, and ends later).  Eight warps each: while one's scores are exponentiated, the other's products run.  Two threads own a
 // row, 64 keys each (with one, the single warp that a tile then has on each of the SM's four parts waits for its own instructions: 2000
 // cycles per tile, and 3400 per pair of tiles where heads of 128 need 2048 for their products).  They agree on the largest score through
 // shared memory, read the scores twice from tensor memory rather than keep them, and rescale and write half of the features each.
@@ -397,47 +398,61 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
   volatile int* const stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
-  if (warp == 17 && elect_one()) tma_prefetch(&maps.q), tma_prefetch(&maps.k), tma_prefetch(&maps.v), tma_prefetch(&maps.y);
+  // The thread that loads sets the barriers up and sends for the first tiles before it meets the others: the loads are under way while
+  // tensor memory is taken and everybody finds out what the item is.
   if (warp == 16) tmem_alloc(tmem_slot, 512);
-  if (threadIdx.x == 0) {
+  if (warp == 17 && elect_one()) {
     mbar_init(q_full, 1), mbar_init(go, 1), mbar_init(cleared, 1);
     for (int x = 0; x < 2; ++x) mbar_init(s_full + x, 1), mbar_init(p_half + x, 2 * kT), mbar_init(p_ready + x, 2 * kT), mbar_init(o_full + x, 1);
     for (int i = 0; i < SLOTS; ++i) mbar_init(ring.full + i, 1), mbar_init(ring.empty + i, 1);
     fence_mbar_init();
     *stop = 0;
   }
+  wait_for_inputs();
+  const bool by_head = p.G % 2 == 0;
+  const Block at = by_head ? block_of(p.H / 2, (p.Nq + kT - 1) / kT) : block_of(p.H, (p.Nq + 2 * kT - 1) / (2 * kT));
+  const int i0 = at.last_first * (by_head ? kT : 2 * kT), h0 = by_head ? 2 * at.head : at.head, b = at.b, hk = h0 / p.G;
+  auto first_of = [&](int x) { return by_head ? i0 : i0 + x * kT; };  // tile x's first query, and its head
+  auto head_of = [&](int x) { return by_head ? h0 + x : h0; };
+  const RowGeom g = row_geom(p, b);
+  const KeyTiles all = key_tiles<kT>(p, g, i0, first_of(1) + kT);
+  const int n = all.count();
+  // the last tile may end in padding, whose values would meet weights of zero
+  const bool clear = n > 0 && g.ctx < p.Nk && all.tile(n - 1) * kT + kT > g.ctx;
+  const int at_once = min(2 * n, SLOTS);
+  auto load = [&](int i) {
+    const auto to = ring.place(i);
+    mbar_expect_tx(ring.arrived(to), TILE);
+    load_tile<DP>(ring.at(to), i & 1 ? &maps.v : &maps.k, hk, all.tile(i >> 1) * kT, b, ring.arrived(to));
+  };
+  if (warp == 17) {
+    __syncwarp();
+    if (n > 0 && elect_one()) {
+      const int queries = first_of(1) < p.Nq ? 2 : 1;
+      mbar_expect_tx(q_full, queries * TILE);
+      for (int x = 0; x < queries; ++x) load_tile<DP>(qs + x * TILE, &maps.q, head_of(x), first_of(x), b, q_full);
+      for (int i = 0; i < at_once; ++i) load(i);
+    }
+    __syncwarp();
+  }
   tmem_before();
   __syncthreads();
   tmem_after();
   const uint32_t tmem = *tmem_slot;
-  wait_for_inputs();
-
-  const Block at = block_of(p.H, (p.Nq + 2 * kT - 1) / (2 * kT));
-  const int i0 = at.last_first * 2 * kT, h = at.head, b = at.b, hk = h / p.G;
-  const RowGeom g = row_geom(p, b);
-  const KeyTiles all = key_tiles<kT>(p, g, i0, i0 + 2 * kT);
-  const int n = all.count();
   const Waiter wait{stop, p.status};
-  // the last tile may end in padding, whose values would meet weights of zero
-  const bool clear = n > 0 && g.ctx < p.Nk && all.tile(n - 1) * kT + kT > g.ctx;
 
   if (warp == 17) {
-    if (n > 0 && elect_one()) {
-      const int queries = i0 + kT < p.Nq ? 2 : 1;
-      mbar_expect_tx(q_full, queries * TILE);
-      for (int x = 0; x < queries; ++x) load_tile<DP>(qs + x * TILE, &maps.q, h, i0 + x * kT, b, q_full);
-      typename Ring<SLOTS>::Place to;
-      for (int i = 0; i < 2 * n; ++i) {
-        if (!ring.wait_empty(wait, to)) {
+    if (elect_one()) {
+      for (int i = at_once; i < 2 * n; ++i) {
+        if (!ring.wait_empty(wait, ring.place(i))) {
           mbar_wait_bounded(q_full, 0, 1u << 16);
           settle(ring, i);
           break;
         }
-        mbar_expect_tx(ring.arrived(to), TILE);
-        load_tile<DP>(ring.at(to), i & 1 ? &maps.v : &maps.k, hk, all.tile(i >> 1) * kT, b, ring.arrived(to));
-        to.next();
+        load(i);
       }
     }
+    __syncwarp();
   } else if (warp == 18) {
     if (clear && wait(go, 0)) clear_rows<DP>(ring.at(ring.place(2 * n - 1)), 0, g.ctx - all.tile(n - 1) * kT, cleared);
   } else if (warp == 16) {
@@ -445,7 +460,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
       // what tile x needs of the list: entries below ns, and lo .. hi
       int ns[2], lo[2], hi[2], last[2];
       for (int x = 0; x < 2; ++x) {
-        const KeyTiles kt = key_tiles<kT>(p, g, i0 + x * kT, i0 + x * kT + kT);
+        const KeyTiles kt = key_tiles<kT>(p, g, first_of(x), first_of(x) + kT);
         ns[x] = kt.ns;
         lo[x] = all.entry(kt.t0);
         hi[x] = kt.t1 >= kt.t0 ? all.entry(kt.t1) : -1;
@@ -499,12 +514,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
     }
     __syncwarp();
   } else {
-    const int x = warp / 8, half = warp / 4 % 2, r = threadIdx.x % kT, qi = i0 + x * kT + r, pos = g.start + qi;
+    const int x = warp / 8, half = warp / 4 % 2, r = threadIdx.x % kT, first = first_of(x), h = head_of(x), qi = first + r, pos = g.start + qi;
     const int end = min(g.ctx, g.start + p.Nq);
-    const KeyTiles kt = key_tiles<kT>(p, g, i0 + x * kT, i0 + x * kT + kT);
+    const KeyTiles kt = key_tiles<kT>(p, g, first_of(x), first_of(x) + kT);
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     const uint32_t ts = tmem + x * kT + half * 64 + lanes, to = tmem + 2 * kT + x * 128 + lanes;
-    const int p_lo = g.start + i0 + x * kT, p_hi = p_lo + kT - 1;  // positions of the tile, padding included
+    const int p_lo = g.start + first, p_hi = p_lo + kT - 1;  // positions of the tile, padding included
     const int mine = kt.count(), pair_bar = 1 + x * 4 + warp % 4;  // the barrier of the two warps that share rows
     float *const my_row = shared_row + (2 * x + half) * kT + r, *const other_row = shared_row + (2 * x + 1 - half) * kT + r;
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
@@ -605,12 +620,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
       const bool some = mine > 0 && pos >= 0 && pos < end && !(l == 0.f);
       const float inv = some ? 1.f / l : 0.f;
       if (p.lse && half == 0 && qi < p.Nq) p.lse[((long long)b * p.H + h) * p.Nqp + qi] = some ? ref + log2f(l) : INFINITY;
-      // through the place of the tile's queries, 2 KB of it to a warp: the last of its products has read them (with no
+      // through the place of the tile's queries, 4 KB of it to a warp (2 KB in heads of 64): the last of its products has read them (with no
       // products, they may still be arriving)
-      const int row0 = i0 + x * kT + warp % 4 * 32;
-      if (n > 0 && i0 + x * kT < p.Nq) ok = wait(q_full, 0);
+      const int row0 = first + warp % 4 * 32;
+      if (n > 0 && first < p.Nq) ok = wait(q_full, 0);
       if (ok && row0 < p.Nq) {
-        const uint32_t place = qs + x * TILE + warp % 8 * 2048;
+        constexpr uint32_t MINE = TILE / 8;
+        constexpr int OTHERS = MINE / 2048 - 1;
+        const uint32_t place = qs + x * TILE + warp % 8 * MINE, second = place + OTHERS * 2048;
 #pragma unroll 1
         for (int c = half * (DP / 2); c < (half + 1) * (DP / 2) && c < p.d; c += 32) {
           float o[32];
@@ -622,10 +639,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0.f;
           }
-          send_rows(&maps.y, place, o, inv, c, h, row0, b);
+          send_rows<OTHERS>(&maps.y, p.rest || c % 64 == 0 ? place : second, o, inv, c, h, row0, b);
           if (p.rest) {
             keep_rest(o, inv);
-            send_rows(&maps.rest, place, o, 1.f, c, h, row0, b);
+            send_rows<OTHERS>(&maps.rest, second, o, 1.f, c, h, row0, b);
           }
         }
         if (lane == 0) bulk_wait_read0();
@@ -668,53 +685,61 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
   volatile int* const stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
-  if (warp == 9 && elect_one()) tma_prefetch(&maps.q), tma_prefetch(&maps.dy), tma_prefetch(&maps.k), tma_prefetch(&maps.v), tma_prefetch(&maps.dq);
   if (warp == 8) tmem_alloc(tmem_slot, 512);
-  if (threadIdx.x == 0) {
+  if (warp == 9 && elect_one()) {
     mbar_init(q_full, 1), mbar_init(s_full, 1), mbar_init(s_full + 1, 1), mbar_init(dp_full, 1), mbar_init(ds_half, 256), mbar_init(ds_ready, 256);
     mbar_init(done, 1), mbar_init(go, 1), mbar_init(cleared, 1), mbar_init(staged, 256);
     for (int i = 0; i < SLOTS; ++i) mbar_init(ring.full + i, 1), mbar_init(ring.empty + i, 1);
     fence_mbar_init();
     *stop = 0;
   }
-  tmem_before();
-  __syncthreads();
-  tmem_after();
-  const uint32_t tmem = *tmem_slot, t_dp = tmem + 256, t_dq = tmem + 384;
   wait_for_inputs();
-
   const Block at = block_of(p.H, (p.Nq + kT - 1) / kT);
   const int i0 = at.last_first * kT, h = at.head, b = at.b, hk = h / p.G;
   const RowGeom g = row_geom(p, b);
   const KeyTiles kt = key_tiles<kT>(p, g, i0, i0 + kT);
   const int n = kt.count();
-  const Waiter wait{stop, p.status};
 
   // the last tile may end in padding: keys that would meet a dS of zero
   const bool clear = n > 0 && g.ctx < p.Nk && kt.tile(n - 1) * kT + kT > g.ctx;
-
+  // (as in the forward: the first tiles are sent for before the warps meet)
+  const int at_once = min(2 * n + 2, SLOTS);
+  auto load = [&](int i) {  // y and its rest, for delta, in the ring's first places; then keys and values
+    const auto to = ring.place(i);
+    mbar_expect_tx(ring.arrived(to), TILE);
+    if (i < 2)
+      load_tile<DP>(ring.at(to), i ? &maps.rest : &maps.y, h, i0, b, ring.arrived(to));
+    else
+      load_tile<DP>(ring.at(to), i & 1 ? &maps.v : &maps.k, hk, kt.tile((i >> 1) - 1) * kT, b, ring.arrived(to));
+  };
   if (warp == 9) {
+    __syncwarp();
     if (n > 0 && elect_one()) {
       mbar_expect_tx(q_full, 2 * TILE);
       load_tile<DP>(qs, &maps.q, h, i0, b, q_full);
       load_tile<DP>(dys, &maps.dy, h, i0, b, q_full);
-      typename Ring<SLOTS>::Place to;
-      for (int which = 0; which < 2; ++which) {  // y and its rest, for delta, in the ring's first places
-        mbar_expect_tx(ring.arrived(to), TILE);
-        load_tile<DP>(ring.at(to), which ? &maps.rest : &maps.y, h, i0, b, ring.arrived(to));
-        to.next();
-      }
-      for (int i = 0; i < 2 * n; ++i) {
-        if (!ring.wait_empty(wait, to)) {
+      for (int i = 0; i < at_once; ++i) load(i);
+    }
+    __syncwarp();
+  }
+  tmem_before();
+  __syncthreads();
+  tmem_after();
+  const uint32_t tmem = *tmem_slot, t_dp = tmem + 256, t_dq = tmem + 384;
+  const Waiter wait{stop, p.status};
+
+  if (warp == 9) {
+    if (n > 0 && elect_one()) {
+      for (int i = at_once; i < 2 * n + 2; ++i) {
+        if (!ring.wait_empty(wait, ring.place(i))) {
           mbar_wait_bounded(q_full, 0, 1u << 16);
-          settle(ring, i + 2);
+          settle(ring, i);
           break;
         }
-        mbar_expect_tx(ring.arrived(to), TILE);
-        load_tile<DP>(ring.at(to), i & 1 ? &maps.v : &maps.k, hk, kt.tile(i >> 1) * kT, b, ring.arrived(to));
-        to.next();
+        load(i);
       }
     }
+    __syncwarp();
   } else if (warp == 10) {
     if (clear && wait(go, 0)) clear_rows<DP>(ring.at(ring.place(2 * n)), 0, g.ctx - kt.tile(n - 1) * kT, cleared);
   } else if (warp == 8) {
@@ -891,9 +916,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
   volatile int* const stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
-  if (warp == 9 && elect_one()) tma_prefetch(&maps.k), tma_prefetch(&maps.v), tma_prefetch(&maps.q), tma_prefetch(&maps.dy), tma_prefetch(&maps.dk);
   if (warp == 8) tmem_alloc(tmem_slot, 512);
-  if (threadIdx.x == 0) {
+  if (warp == 9 && elect_one()) {
     mbar_init(kv_full, 1), mbar_init(s_full, 1), mbar_init(dp_full, 1), mbar_init(done, 1), mbar_init(go, 1), mbar_init(cleared, 1), mbar_init(staged, 256);
     mbar_init(p_half, 256), mbar_init(p_ready, 256), mbar_init(ds_half, 256), mbar_init(ds_ready, 256);
     for (int i = 0; i < STATS; ++i) mbar_init(st_full + i, 1), mbar_init(st_empty + i, 8);
@@ -901,18 +925,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
     fence_mbar_init();
     *stop = 0;
   }
-  tmem_before();
-  __syncthreads();
-  tmem_after();
-  const uint32_t tmem = *tmem_slot, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
   wait_for_inputs();
-
   const Block at = block_of(p.Hk, (p.Nk + kT - 1) / kT + p.sink_tiles * p.chunks);
   const int hk = at.head, b = at.b;
   const RowGeom g = row_geom(p, b);
   const KeyItem it = key_item<kT, kT>(p, g, at.first_last);
   const int k0 = it.tile * kT, n = it.end - it.begin;
-  const Waiter wait{stop, p.status};
   // an entry of the list of the item's heads and tiles of queries, and the next one (each role walks the list by itself)
   struct Entry {
     int head, tile, first, end;  // tile: first <= tile < end
@@ -929,41 +947,57 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
     const int first = g.start + e.row();
     return first < 0 || (first + kT > g.ctx && g.start + p.Nq > g.ctx);
   };
-
+  // (as in the forward: the first tiles are sent for before the warps meet)
+  const int at_once = min(2 * n, 4);
+  auto load = [&](int i, const Entry& e) {  // queries, their cotangents, and with these the stats, whose place is free before that
+    const auto to = ring.place(i);
+    mbar_expect_tx(ring.arrived(to), TILE);
+    load_tile<DP>(ring.at(to), i & 1 ? &maps.dy : &maps.q, e.head, e.row(), b, ring.arrived(to));
+    if (i & 1) {
+      const int u = i >> 1;
+      float* const st = stats + u % STATS * 2 * kT;
+      const long long row = ((long long)b * p.H + e.head) * p.Nqp + e.row();
+      mbar_expect_tx(st_full + u % STATS, 2 * kT * 4);
+      bulk_g2s(st, p.lse + row, kT * 4, st_full + u % STATS);
+      bulk_g2s(st + kT, p.delta + row, kT * 4, st_full + u % STATS);
+    }
+  };
   if (warp == 9) {
+    __syncwarp();
     if (n > 0 && elect_one()) {
       mbar_expect_tx(kv_full, 2 * TILE);
       load_tile<DP>(ks, &maps.k, hk, k0, b, kv_full);
       load_tile<DP>(vs, &maps.v, hk, k0, b, kv_full);
-      typename Ring<SLOTS>::Place to;
-      bool ok = true;
-      int i = 0, held = 0;  // tiles and stats under way
-      for (; i < 2 * n; ++i) {
-        if (!(ok = ring.wait_empty(wait, to))) break;
-        const int u = i >> 1, h = entry.head, i0 = entry.row();
-        mbar_expect_tx(ring.arrived(to), TILE);
-        load_tile<DP>(ring.at(to), i & 1 ? &maps.dy : &maps.q, h, i0, b, ring.arrived(to));
-        to.next();
-        if (i & 1) {  // the stats last: their place is free only when tile u - STATS is done with
-          if (!(ok = wait.one(st_empty + u % STATS, (u / STATS & 1) ^ 1))) {
-            ++i;
-            break;
-          }
-          float* const st = stats + u % STATS * 2 * kT;
-          const long long row = ((long long)b * p.H + h) * p.Nqp + i0;
-          mbar_expect_tx(st_full + u % STATS, 2 * kT * 4);
-          bulk_g2s(st, p.lse + row, kT * 4, st_full + u % STATS);
-          bulk_g2s(st + kT, p.delta + row, kT * 4, st_full + u % STATS);
-          held = u + 1;
-          entry.next();
-        }
-      }
-      if (!ok) {
-        mbar_wait_bounded(kv_full, 0, 1u << 16);
-        for (int e = held > STATS ? held - STATS : 0; e < held; ++e) mbar_wait_bounded(st_full + e % STATS, (e / STATS) & 1, 1u << 16);
-        settle(ring, i);
+      Entry e = entry;
+      for (int i = 0; i < at_once; ++i) {
+        load(i, e);
+        if (i & 1) e.next();
       }
     }
+    __syncwarp();
+  }
+  tmem_before();
+  __syncthreads();
+  tmem_after();
+  const uint32_t tmem = *tmem_slot, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
+  const Waiter wait{stop, p.status};
+
+  if (warp == 9) {
+    if (n > 0 && elect_one()) {
+      for (int i = 0; i < at_once; i += 2) entry.next();
+      for (int i = at_once; i < 2 * n; ++i) {
+        const int u = i >> 1;
+        if (!ring.wait_empty(wait, ring.place(i)) || (i & 1 && !wait.one(st_empty + u % STATS, (u / STATS & 1) ^ 1))) {
+          mbar_wait_bounded(kv_full, 0, 1u << 16);
+          for (int e = u > STATS ? u - STATS : 0; e < u; ++e) mbar_wait_bounded(st_full + e % STATS, (e / STATS) & 1, 1u << 16);
+          settle(ring, i);
+          break;
+        }
+        load(i, entry);
+        if (i & 1) entry.next();
+      }
+    }
+    __syncwarp();
   } else if (warp == 10) {
     uint32_t clears = 0;
     for (int i = 0; i < 2 * n; ++i) {
@@ -1193,8 +1227,8 @@ cudaError_t run_fwd(const AttnParams& p, const Maps& maps, cudaStream_t st) {
   constexpr uint32_t smem = FwdSmem<DP, SLOTS>::bytes;
   const cudaError_t e = grant_smem(grant, attn_tensor_fwd_kernel<DP, SLOTS>, smem);
   if (e != cudaSuccess) return e;
-  const int tiles = (p.Nq + 2 * kT - 1) / (2 * kT);
-  return launch_behind(attn_tensor_fwd_kernel<DP, SLOTS>, dim3((unsigned)(tiles * p.H * p.B)), kFwdThreads, smem, st, p, maps);
+  const unsigned items = p.G % 2 == 0 ? (unsigned)((p.Nq + kT - 1) / kT) * (p.H / 2) * p.B : (unsigned)((p.Nq + 2 * kT - 1) / (2 * kT)) * p.H * p.B;
+  return launch_behind(attn_tensor_fwd_kernel<DP, SLOTS>, dim3(items), kFwdThreads, smem, st, p, maps);
 }
 template <int DP, int SLOTS>
 cudaError_t run_bwd(const AttnParams& p, const Maps& maps, cudaStream_t st) {
