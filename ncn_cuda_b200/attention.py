@@ -15,6 +15,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch import nn
 
 from . import _lib, ops
 
@@ -179,3 +180,77 @@ def window_attention_decode(q, k_cache, v_cache, ctxlen, n_head, window, n_sink=
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_cache, v_cache)):
         raise RuntimeError("window_attention_decode has no gradient: use fused_window_attention, or torch.no_grad()")
     return _lib.native().window_decode(q, k_cache, v_cache, torch.as_tensor(ctxlen), n_head, window, n_sink, scale)
+
+
+class NCNWindowAttention(nn.Module):
+    """A local attention layer to stand between NCN layers: [B, N, embed_dim] -> [B, N, embed_dim].
+
+    One projection to queries, keys and values, the norm of every head of queries and keys (qk_norm) with the rotation of its first
+    rot_dim features (None: all of them, 0: none), windowed attention with sinks, a projection back.  n_kv_head: heads of
+    keys and values (None: n_head).  base, scaling, factor, trained_length: as in rotary_frequencies.
+
+    forward(x, ctxlen=None) is the training form.  For serving, new_cache(B, length) and step(x, cache, ctxlen)."""
+
+    def __init__(self, embed_dim, n_head, window, n_sink=0, n_kv_head=None, rot_dim=None, base=10000.0, scaling=None, factor=1.0,
+                 trained_length=4096, interleaved=False, qk_norm=True, eps=1e-6):
+        super().__init__()
+        n_kv_head = n_head if n_kv_head is None else n_kv_head
+        if n_head < 1 or n_kv_head < 1 or embed_dim % n_head or n_head % n_kv_head:
+            raise ValueError(f"n_head = {n_head} must divide embed_dim = {embed_dim}, and n_kv_head = {n_kv_head} n_head")
+        self.embed_dim, self.n_head, self.n_kv_head = embed_dim, n_head, n_kv_head
+        self.window, self.n_sink, self.interleaved, self.eps = window, n_sink, interleaved, eps
+        d = embed_dim // n_head
+        self.qkv = nn.Linear(embed_dim, (n_head + 2 * n_kv_head) * d, bias=False)
+        self.out = nn.Linear(embed_dim, embed_dim, bias=False)
+        self.q_weight = nn.Parameter(torch.ones(d)) if qk_norm else None
+        self.k_weight = nn.Parameter(torch.ones(d)) if qk_norm else None
+        self.freqs, self.magnitude = rotary_frequencies(d if rot_dim is None else rot_dim, base, scaling, factor, trained_length)
+
+    def _apply(self, fn, *args, **kwargs):
+        # the frequencies go where the weights go, and stay in 64 bits whatever the weights' type becomes
+        super()._apply(fn, *args, **kwargs)
+        if self.qkv.weight.device.type != "meta":
+            self.freqs = self.freqs.to(self.qkv.weight.device)
+        return self
+
+    def _rotated(self, x, positions):
+        d = self.embed_dim // self.n_head
+        q, k, v = self.qkv(x).split([self.embed_dim, self.n_kv_head * d, self.n_kv_head * d], -1)
+        if self.q_weight is None:
+            q, k = fused_rotary(q, k, self.freqs, self.n_head, positions, self.interleaved, self.magnitude)
+        else:
+            q, k = fused_qk_norm_rotary(q, k, self.q_weight, self.k_weight, self.freqs, self.n_head, positions, self.interleaved,
+                                        self.magnitude, self.eps)
+        return q, k, v
+
+    def forward(self, x, ctxlen=None):
+        q, k, v = self._rotated(x, None)
+        return self.out(fused_window_attention(q, k, v, self.n_head, self.window, n_sink=self.n_sink, ctxlen=ctxlen))
+
+    def new_cache(self, B: int, length: int):
+        """Keys and values of B rows of up to `length` positions, in the weights' type.  (The place behind them takes what has none.)"""
+        w = self.qkv.weight
+        width = self.n_kv_head * (self.embed_dim // self.n_head)
+        return tuple(torch.zeros(B, length + 1, width, dtype=w.dtype, device=w.device) for _ in range(2))
+
+    @torch.no_grad()
+    def step(self, x, cache, ctxlen):
+        """The next positions of each row: x [B, n, embed_dim], ctxlen int tensor [B], the rows' lengths with these n counted.  Enters their
+        keys and values into the cache and returns [B, n, embed_dim].  Rows shorter than n are padded in front: what stands there is not
+        entered and gives out(0).  Positions beyond the cache's length are lost: make it long enough."""
+        k_cache, v_cache = cache
+        B, n, _ = x.shape
+        length = k_cache.shape[1] - 1
+        ctxlen = torch.as_tensor(ctxlen).to(device=x.device, dtype=torch.int64)
+        positions = ctxlen[:, None] - n + torch.arange(n, device=x.device)
+        q, k, v = self._rotated(x, positions)
+        place = torch.where((positions < 0) | (positions >= length), length, positions)
+        rows = torch.arange(B, device=x.device)[:, None]
+        k_cache[rows, place] = k
+        v_cache[rows, place] = v
+        k_cache, v_cache = k_cache[:, :length], v_cache[:, :length]
+        if n == 1:
+            y = window_attention_decode(q, k_cache, v_cache, ctxlen, self.n_head, self.window, n_sink=self.n_sink)
+        else:
+            y = fused_window_attention(q, k_cache, v_cache, self.n_head, self.window, n_sink=self.n_sink, ctxlen=ctxlen, q_start=ctxlen - n)
+        return self.out(y)

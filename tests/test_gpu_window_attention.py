@@ -170,7 +170,12 @@ def test_nothing_to_do(dtype):
 def test_the_tensor_cores_are_reached():
     q, k, v, dy = make(1, 1, 256, 256, 2, 1, 128, BF16)
     leaves = [t.requires_grad_(True) for t in (q, k, v)]
-    _, names = kernels_of(lambda: torch.autograd.grad(ncn.fused_window_attention(*leaves, 2, 64, n_sink=2), leaves, dy))
+
+    def steps():  # (a profiler that has been in use for a minute may miss the first milliseconds)
+        for _ in range(200):
+            torch.autograd.grad(ncn.fused_window_attention(*leaves, 2, 64, n_sink=2), leaves, dy)
+
+    _, names = kernels_of(steps)
     for part in ("attn_tensor_fwd", "attn_tensor_dq", "attn_tensor_dkv", "attn_sink_sum"):
         assert launched(names, part), (part, names)
 
@@ -364,3 +369,81 @@ def test_decode_captured_and_strided():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, check_decode(q, kc, vc, H, 300, 4, ctxlen))
+
+
+# ---------------------------------------------------------------- refusals, and calls side by side
+def test_refusals_on_the_device():
+    q, k, v, _ = make(1, 2, 8, 8, 4, 2, 32, BF16)
+    freqs, _ = ncn.rotary_frequencies(32, device="cuda")
+    half = q.half()
+    for call in (lambda: ncn.fused_window_attention(half, half, half, 4, 3), lambda: ncn.fused_rotary(half, half, freqs, 4),
+                 lambda: ncn.window_attention_decode(half, half, half, [1, 1], 4, 3)):
+        with pytest.raises(TypeError, match="float32 or bfloat16"):
+            call()
+    for bad in ((q, k.float(), v), (q, k, v[:, :5]), (q, k[:1], v[:1]), (q[0], k, v), (q, k[..., :40], v[..., :40])):
+        with pytest.raises(ValueError):
+            ncn.fused_window_attention(*bad, 4, 3)
+        with pytest.raises(ValueError):
+            ncn.window_attention_decode(*bad, torch.tensor([1, 1]), 4, 3)
+    with pytest.raises(ValueError, match="n_head"):
+        ncn.fused_window_attention(q, k, v, 3, 3)
+    with pytest.raises(ValueError, match="ctxlen has 3"):
+        ncn.fused_window_attention(q, k, v, 4, 3, ctxlen=[1, 2, 3])
+    with pytest.raises(ValueError, match="q_start has 1"):
+        ncn.fused_window_attention(q, k, v, 4, 3, q_start=torch.tensor([1]))
+    with pytest.raises(ValueError, match="positions"):
+        ncn.fused_rotary(q, k, freqs, 4, positions=torch.arange(7))
+    with pytest.raises(TypeError, match="whole numbers"):
+        ncn.fused_rotary(q, k, freqs, 4, positions=torch.arange(8).float())
+    with pytest.raises(ValueError, match="freqs"):
+        ncn.fused_rotary(q, k, torch.ones(17, device="cuda"), 4)
+    with pytest.raises(ValueError, match="weight has"):
+        ncn.fused_qk_norm_rotary(q, k, torch.ones(31, device="cuda"), torch.ones(32, device="cuda"), freqs, 4)
+    wide = torch.zeros(1, 4, 2 * 264, device="cuda")
+    with pytest.raises(ncn._lib.NCNError, match="bad shape"):
+        ncn.fused_window_attention(wide, wide, wide, 2, 3)
+    # heads of the queries that the heads of the keys do not divide
+    with pytest.raises(ncn._lib.NCNError, match="bad shape"):
+        ncn.fused_window_attention(torch.zeros(1, 4, 96, device="cuda"), torch.zeros(1, 4, 64, device="cuda"), torch.zeros(1, 4, 64, device="cuda"), 3, 3)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_calls_at_once_on_two_streams(dtype):
+    """Workspaces, results and saved states belong to a call."""
+    sets = [make(20 + i, 1, 1500, 1500, 4, 2, 128, dtype) for i in range(2)]
+    sets = [([t.requires_grad_(True) for t in s[:3]], s[3]) for s in sets]
+
+    def step(i):
+        leaves, dy = sets[i]
+        y = ncn.fused_window_attention(*leaves, 4, 300, n_sink=40)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    alone = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = step(i)
+    torch.cuda.synchronize()
+    for a, b in zip(alone, got):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
+def test_gradients_of_shared_and_broadcast_inputs():
+    """The same tensor as keys and values, and one row of keys broadcast over the batch."""
+    q, k, _, dy = make(30, 3, 100, 100, 2, 1, 64, BF16)
+    both = k.clone().requires_grad_(True)
+    y = ncn.fused_window_attention(q, both, both, 2, 30)
+    g, = torch.autograd.grad(y, both, dy)
+    want = O.attention(q, k, k, 2, 30, 0, 1 / 8, 100, 0, dy)
+    value, bound = (a + b for a, b in zip(want["dk"], want["dv"]))
+    O.close("d both", g, (value, bound + 2.0**-8 * (value.abs() + bound)))  # (the sum is rounded once more)
+    row = k[:1].clone().requires_grad_(True)
+    y = ncn.fused_window_attention(q, row.expand(3, 100, 64), k, 2, 30)
+    g, = torch.autograd.grad(y, row, dy)
+    want = O.attention(q, row.expand(3, 100, 64), k, 2, 30, 0, 1 / 8, 100, 0, dy)["dk"]
+    value, bound = want[0].sum(0, keepdim=True), want[1].sum(0, keepdim=True)
+    O.close("d row", g, (value, bound + 2.0**-8 * (value.abs() + bound)))

@@ -266,3 +266,44 @@ def test_layer_in_training_and_serving(dtype, d):
             assert torch.equal(a, qr[:, lo:hi]) and torch.equal(b, kr[:, lo:hi])
             O.close(f"serving {lo}", out, tuple(t[:, lo:hi] for t in want["y"]))
     ops.device_status()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kw", [{}, {"qk_norm": False, "rot_dim": 32, "interleaved": True}, {"n_kv_head": 4, "scaling": "yarn", "factor": 4.0}])
+def test_layer_module(dtype, kw):
+    """forward against the operators one by one; step by step against forward, rows of different lengths."""
+    torch.manual_seed(3)
+    B, N, E, H = 3, 90, 256, 4
+    layer = ncn.NCNWindowAttention(E, H, 20, n_sink=2, **{"n_kv_head": 2, **kw}).cuda().to(dtype)
+    x = torch.randn(B, N, E, device="cuda").to(dtype)
+    y = layer(x)
+    y.float().square().mean().backward()
+    for name, p in layer.named_parameters():
+        assert p.grad is not None and torch.isfinite(p.grad).all() and p.grad.abs().sum() > 0, name
+    q, k, v = layer._rotated(x, None)
+    inner = ncn.fused_window_attention(q, k, v, H, 20, n_sink=2)
+    assert torch.equal(y, layer.out(inner))
+    want = O.attention(q, k, v, H, 20, 2, 1 / 8, N, 0)["y"]
+    O.close("inner", inner.detach(), want)
+
+    # rows of 40, 7 and 1 positions, padded in front to a prompt of 40, then 30 more each, one by one
+    lens = torch.tensor([40, 7, 1], device="cuda")
+    cache = layer.new_cache(B, N)
+    prompt = torch.full((B, 40, E), math.nan, device="cuda", dtype=dtype)
+    for b, n in enumerate(lens.tolist()):
+        prompt[b, 40 - n :] = x[b, :n]
+    got = layer.step(prompt, cache, lens)
+    # The same projections in other batches may be summed in another order.  bf16: roundings of the projection, the rotated heads, the inner
+    # result and the last one, 2^-8 of the largest each, on both sides: 8 * 2^-8.  fp32: three sums of 256 terms on both sides, 2^-24 of
+    # the terms each: 6 * 256 * 2^-24 of the terms, which are no larger than 1.1 times the results' largest here.
+    tol = {F32: 1.1 * 6 * 256 * 2.0**-24, BF16: 8 * 2.0**-8}[dtype]
+    for b, n in enumerate(lens.tolist()):
+        assert (got[b, 40 - n :] - y[b, :n]).abs().max() <= tol * y.abs().max()
+        assert (got[b, : 40 - n] == 0).all()
+        assert torch.isfinite(cache[0][b, :N]).all()
+    for t in range(30):
+        lens += 1
+        one = torch.stack([x[b, n - 1 : n] for b, n in enumerate(lens.tolist())])
+        got = layer.step(one, cache, lens)
+        for b, n in enumerate(lens.tolist()):
+            assert (got[b, 0] - y[b, n - 1]).abs().max() <= tol * y.abs().max(), (t, b)
