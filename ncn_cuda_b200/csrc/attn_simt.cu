@@ -3,8 +3,14 @@
 //
 // A CTA of 256 threads owns 64 rows (queries; in the backward of the keys: keys) and walks the tiles of the other side.  Thread
 // (ty, tx) of 16 x 16 holds rows 4 ty .. 4 ty + 3.  Tiles are fp32 in shared memory whatever the storage type; a row is DP + 4
-// floats, so that eight lanes that read eight rows 16 bytes at a time hit 32 different banks.  A product of 4 features takes 4
-// broadcast reads and 4 rows' reads for 64 FMAs of a thread: the FMA pipe is the bound, not shared memory.
+// floats, so that eight lanes that read eight rows 16 bytes at a time hit 32 different banks.  DP is the head size, rounded up to
+// 32, 64, 96, 128 or 256: without 96, heads of 72 to 96 did a third more products on zeros.
+//
+// What bounds it: the reads of shared memory.  A product over 4 features takes a thread 8 reads of 16 bytes, which return to a
+// warp in 32 cycles, for 64 FMAs, which take 16: half the FMA rate (36 of 72 TFLOP/s) is the most this split can give.  Measured,
+// 2 x 4096 positions of 8 heads, windows of 1024: heads of 128 forward 928 us (32.4 TFLOP/s), dq 1332 (33.9), dk and dv 1761
+// (34.2); heads of 64 453, 649, 862 us (33 to 35).  Tiles of 8 rows a thread would lower the reads by a quarter, but with heads
+// of 128 the backward's four tiles then no longer fit in shared memory.
 #include "attn_common.cuh"
 #include "ncn_common.cuh"
 
@@ -14,27 +20,29 @@ namespace {
 constexpr int kOwn = 64;
 template <int DP> constexpr int other_rows() { return DP > 128 ? 32 : 64; }
 
-// rows x d of `src` (row stride in elements) -> fp32 tile [rows][DP + 4]; rows outside [r_lo, r_hi) and features beyond d are zero
-template <typename T, int DP>
-__device__ __forceinline__ void load_tile(float* dst, const T* src, long long stride, int rows, int r_lo, int r_hi, int d, int vec) {
-  constexpr int V = 16 / sizeof(T);
+// ROWS x d of `src` (row stride in elements) -> fp32 tile [ROWS][DP + 4]; rows outside [r_lo, r_hi) and features beyond d are zero.
+// All of a thread's loads are under way at once: one after the other they took longer than the tile's arithmetic.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void load_tile(float* dst, const T* src, long long stride, int r_lo, int r_hi, int d, int vec) {
+  constexpr int V = 16 / sizeof(T), PER = DP / V, COUNT = ROWS * PER, EACH = (COUNT + 255) / 256;
   if (vec) {
-    for (int e = threadIdx.x; e < rows * (DP / V); e += 256) {
-      const int r = e / (DP / V), c = e % (DP / V) * V;
-      float x[V];
+    uint4 raw[EACH];
 #pragma unroll
-      for (int i = 0; i < V; ++i) x[i] = 0.f;
-      if (r >= r_lo && r < r_hi && c < d) {  // (d is a multiple of V here)
-        const uint4 raw = *reinterpret_cast<const uint4*>(src + r * stride + c);
-        const T* t = reinterpret_cast<const T*>(&raw);
+    for (int i = 0; i < EACH; ++i) {
+      const int e = threadIdx.x + 256 * i, r = e / PER, c = e % PER * V;
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (e < COUNT && r >= r_lo && r < r_hi && c < d) raw[i] = *reinterpret_cast<const uint4*>(src + r * stride + c);  // (d is a multiple of V)
+    }
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = to_f(t[i]);
-      }
+    for (int i = 0; i < EACH; ++i) {
+      const int e = threadIdx.x + 256 * i, r = e / PER, c = e % PER * V;
+      if (e >= COUNT) break;
+      const T* t = reinterpret_cast<const T*>(&raw[i]);
 #pragma unroll
-      for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(dst + r * (DP + 4) + c + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+      for (int x = 0; x < V; x += 4) *reinterpret_cast<float4*>(dst + r * (DP + 4) + c + x) = make_float4(to_f(t[x]), to_f(t[x + 1]), to_f(t[x + 2]), to_f(t[x + 3]));
     }
   } else {
-    for (int e = threadIdx.x; e < rows * DP; e += 256) {
+    for (int e = threadIdx.x; e < ROWS * DP; e += 256) {
       const int r = e / DP, c = e % DP;
       dst[r * (DP + 4) + c] = r >= r_lo && r < r_hi && c < d ? to_f(src[r * stride + c]) : 0.f;
     }
@@ -65,7 +73,7 @@ __device__ __forceinline__ void rows_by_rows(const float* A, const float* B, flo
 }
 
 // A thread's features of a row: VW at a time, VW * tx + 16 VW m
-template <int DP> constexpr int vec_width() { return DP >= 64 ? 4 : 2; }
+template <int DP> constexpr int vec_width() { return DP % 64 == 0 ? 4 : 2; }
 template <int DP> __device__ __forceinline__ int feature_of(int e) {
   constexpr int VW = vec_width<DP>();
   return VW * (threadIdx.x % 16) + 16 * VW * (e / VW) + e % VW;
@@ -139,12 +147,12 @@ __global__ void __launch_bounds__(256) attn_simt_fwd_kernel(const AttnParams p) 
     for (int e = 0; e < DP / 16; ++e) o[i][e] = 0.f;
   }
   const int n = kt.count();
-  if (n) load_tile<T, DP>(Q, q, p.sq_n, kOwn, 0, p.Nq - i0, p.d, p.vec);
+  if (n) load_tile<T, DP, kOwn>(Q, q, p.sq_n, 0, p.Nq - i0, p.d, p.vec);
   for (int it = 0; it < n; ++it) {
     const int k0 = kt.tile(it) * BN;
     __syncthreads();
-    load_tile<T, DP>(K, k + k0 * p.sk_n, p.sk_n, BN, 0, g.ctx - k0, p.d, p.vec);
-    load_tile<T, DP>(V, v + k0 * p.sv_n, p.sv_n, BN, 0, g.ctx - k0, p.d, p.vec);
+    load_tile<T, DP, BN>(K, k + k0 * p.sk_n, p.sk_n, 0, g.ctx - k0, p.d, p.vec);
+    load_tile<T, DP, BN>(V, v + k0 * p.sv_n, p.sv_n, 0, g.ctx - k0, p.d, p.vec);
     __syncthreads();
     float s[4][CJ] = {};
     rows_by_rows<DP, CJ>(Q, K, s);
@@ -212,8 +220,8 @@ __global__ void __launch_bounds__(256) attn_simt_dq_kernel(const AttnParams p) {
   const T* k = static_cast<const T*>(p.k) + b * p.sk_b + (long long)hk * p.d;
   const T* v = static_cast<const T*>(p.v) + b * p.sv_b + (long long)hk * p.d;
   const int r_lo = max(0, -(g.start + i0)), r_hi = min(p.Nq, g.ctx - g.start) - i0;  // rows that are not padding
-  load_tile<T, DP>(Q, q, p.sq_n, kOwn, r_lo, r_hi, p.d, p.vec);
-  load_tile<T, DP>(dO, dy, p.sdy_n, kOwn, r_lo, r_hi, p.d, p.vec);
+  load_tile<T, DP, kOwn>(Q, q, p.sq_n, r_lo, r_hi, p.d, p.vec);
+  load_tile<T, DP, kOwn>(dO, dy, p.sdy_n, r_lo, r_hi, p.d, p.vec);
   __syncthreads();
   float acc[4][DP / 16] = {}, lse[4], delta[4];
 #pragma unroll
@@ -238,8 +246,8 @@ __global__ void __launch_bounds__(256) attn_simt_dq_kernel(const AttnParams p) {
   for (int it = 0; it < n; ++it) {
     const int k0 = kt.tile(it) * BN;
     __syncthreads();
-    load_tile<T, DP>(K, k + k0 * p.sk_n, p.sk_n, BN, 0, g.ctx - k0, p.d, p.vec);
-    load_tile<T, DP>(V, v + k0 * p.sv_n, p.sv_n, BN, 0, g.ctx - k0, p.d, p.vec);
+    load_tile<T, DP, BN>(K, k + k0 * p.sk_n, p.sk_n, 0, g.ctx - k0, p.d, p.vec);
+    load_tile<T, DP, BN>(V, v + k0 * p.sv_n, p.sv_n, 0, g.ctx - k0, p.d, p.vec);
     __syncthreads();
     float s[4][CJ] = {}, dp[4][CJ] = {};
     rows_by_rows<DP, CJ>(Q, K, s);
@@ -288,15 +296,15 @@ __global__ void __launch_bounds__(256) attn_simt_dkv_kernel(const AttnParams p) 
   const T* v = static_cast<const T*>(p.v) + b * p.sv_b + k0 * p.sv_n + (long long)hk * p.d;
   float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
   if (it.begin < it.end) {
-    load_tile<T, DP>(K, k, p.sk_n, kOwn, 0, g.ctx - k0, p.d, p.vec);
-    load_tile<T, DP>(V, v, p.sv_n, kOwn, 0, g.ctx - k0, p.d, p.vec);
+    load_tile<T, DP, kOwn>(K, k, p.sk_n, 0, g.ctx - k0, p.d, p.vec);
+    load_tile<T, DP, kOwn>(V, v, p.sv_n, 0, g.ctx - k0, p.d, p.vec);
   }
   for (int e = it.begin; e < it.end; ++e) {
     const int h = hk * p.G + e / it.tiles, i0 = (it.first + e % it.tiles) * BN;
     const int r_lo = max(0, -(g.start + i0)), r_hi = min(p.Nq, g.ctx - g.start) - i0;
     __syncthreads();
-    load_tile<T, DP>(Q, static_cast<const T*>(p.q) + b * p.sq_b + i0 * p.sq_n + (long long)h * p.d, p.sq_n, BN, r_lo, r_hi, p.d, p.vec);
-    load_tile<T, DP>(dO, static_cast<const T*>(p.dy) + b * p.sdy_b + i0 * p.sdy_n + (long long)h * p.d, p.sdy_n, BN, r_lo, r_hi, p.d, p.vec);
+    load_tile<T, DP, BN>(Q, static_cast<const T*>(p.q) + b * p.sq_b + i0 * p.sq_n + (long long)h * p.d, p.sq_n, r_lo, r_hi, p.d, p.vec);
+    load_tile<T, DP, BN>(dO, static_cast<const T*>(p.dy) + b * p.sdy_b + i0 * p.sdy_n + (long long)h * p.d, p.sdy_n, r_lo, r_hi, p.d, p.vec);
     if (threadIdx.x < BN) {
       const int r = threadIdx.x;
       const long long at = ((long long)b * p.H + h) * p.Nqp + i0 + r;
@@ -403,6 +411,7 @@ template <typename T>
 cudaError_t by_size(const AttnParams& p, bool bwd, cudaStream_t st) {
   if (p.d <= 32) return bwd ? run_bwd<T, 32>(p, st) : run_fwd<T, 32>(p, st);
   if (p.d <= 64) return bwd ? run_bwd<T, 64>(p, st) : run_fwd<T, 64>(p, st);
+  if (p.d <= 96) return bwd ? run_bwd<T, 96>(p, st) : run_fwd<T, 96>(p, st);
   if (p.d <= 128) return bwd ? run_bwd<T, 128>(p, st) : run_fwd<T, 128>(p, st);
   return bwd ? run_bwd<T, 256>(p, st) : run_fwd<T, 256>(p, st);
 }
