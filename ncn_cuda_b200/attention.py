@@ -40,7 +40,7 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[st
         raise ValueError(f"unknown scaling {scaling!r}: one of {SCALINGS}")
     if not (factor >= 1.0 and base > 0 and trained_length > 0 and fast_turns > slow_turns):
         raise ValueError("factor >= 1, base > 0, trained_length > 0 and fast_turns > slow_turns are needed")
-    i = torch.arange(0, rot_dim, 2, dtype=torch.float64)
+    i = torch.arange(0, rot_dim, 2, dtype=torch.float64, device="cpu")
     magnitude = 1.0
     if scaling == "ntk":
         base = base * factor ** (rot_dim / max(rot_dim - 2, 1))
@@ -52,7 +52,28 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[st
         keep = ((turns - slow_turns) / (fast_turns - slow_turns)).clamp(0, 1)
         f = f * keep + f / factor * (1 - keep)
         magnitude = 0.1 * math.log(factor) + 1.0
-    return f.to(device=device), magnitude
+    return (f if device is None else f.to(device=device)), magnitude
+
+
+class _Once(torch.autograd.Function):
+    """Gradients that have no derivative of their own: one that is asked for is an error, not a silent zero."""
+
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tensors[:n]
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("the gradient of an attention operator has no derivative of its own")
+
+
+def _once(grads, *inputs):
+    grads = tuple(grads)
+    if not torch.is_grad_enabled():
+        return grads
+    have = [g for g in grads if g is not None]
+    done = iter(_Once.apply(len(have), *have, *(t for t in inputs if t is not None)))
+    return tuple(None if g is None else next(done) for g in grads)
 
 
 class RotaryFunction(torch.autograd.Function):
@@ -80,11 +101,11 @@ class RotaryFunction(torch.autograd.Function):
         q, k, wq, wk, freqs, positions = ctx.saved_tensors
         if not ctx.norm:
             dx = ops.qk_rotary(dq, dk if ctx.has_k else None, None, None, freqs, positions, *ctx.cfg, inverse=True)
-            return (*dx, None, None, None, None, None, None, None, None, None)
-        dq, dk, dwq, dwk = ops.qk_norm_rotary_bwd(q, k, wq, wk, freqs, positions, dq, dk if ctx.has_k else None, *ctx.cfg)
+            return (*_once(dx, dq, dk), None, None, None, None, None, None, None, None, None)
+        gq, gk, dwq, dwk = ops.qk_norm_rotary_bwd(q, k, wq, wk, freqs, positions, dq, dk if ctx.has_k else None, *ctx.cfg)
         dwq = dwq.to(wq.dtype).reshape(wq.shape)
         dwk = None if dwk is None else dwk.to(wk.dtype).reshape(wk.shape)
-        return dq, dk, dwq, dwk, None, None, None, None, None, None, None
+        return (*_once((gq, gk, dwq, dwk), q, k, wq, wk, dq, dk), None, None, None, None, None, None, None)
 
 
 def _positions(positions):
@@ -135,7 +156,7 @@ class WindowAttentionFunction(torch.autograd.Function):
     def backward(ctx, dy):
         q, k, v, y, state, ctxlen, q_start = ctx.saved_tensors
         dq, dk, dv = ops.window_bwd(q, k, v, y, dy, state, *ctx.cfg, ctxlen=ctxlen, q_start=q_start)
-        return dq, dk, dv, None, None, None, None, None, None, None
+        return (*_once((dq, dk, dv), q, k, v, dy), None, None, None, None, None, None, None)
 
 
 def _window(window, n_sink, scale, q, n_head):
@@ -204,12 +225,13 @@ class NCNWindowAttention(nn.Module):
         self.out = nn.Linear(embed_dim, embed_dim, bias=False)
         self.q_weight = nn.Parameter(torch.ones(d)) if qk_norm else None
         self.k_weight = nn.Parameter(torch.ones(d)) if qk_norm else None
-        self.freqs, self.magnitude = rotary_frequencies(d if rot_dim is None else rot_dim, base, scaling, factor, trained_length)
+        freqs, self.magnitude = rotary_frequencies(d if rot_dim is None else rot_dim, base, scaling, factor, trained_length)
+        self.freqs = freqs if self.qkv.weight.is_meta else freqs.to(self.qkv.weight.device)
 
     def _apply(self, fn, *args, **kwargs):
         # the frequencies go where the weights go, and stay in 64 bits whatever the weights' type becomes
         super()._apply(fn, *args, **kwargs)
-        if self.qkv.weight.device.type != "meta":
+        if not self.qkv.weight.is_meta:
             self.freqs = self.freqs.to(self.qkv.weight.device)
         return self
 

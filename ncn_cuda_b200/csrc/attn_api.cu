@@ -59,7 +59,8 @@ void plan_sinks(AttnParams& p, int T, int TQ) {
   p.sink_tiles = (p.n_sink + T - 1) / T;
   p.sink_rows = p.n_sink < T ? p.n_sink : T;
   p.chunks = (tiles + own - 1) / own;
-  if (p.chunks > 64) p.chunks = 64;
+  const int most = p.sink_tiles < 4 ? 64 : p.sink_tiles < 256 ? 256 / p.sink_tiles : 1;  // (many sink tiles are many items already)
+  if (p.chunks > most) p.chunks = most;
 }
 size_t part_floats(const AttnParams& p) {
   return (size_t)p.B * p.Hk * p.sink_tiles * (p.chunks + 1) * 2 * p.sink_rows * p.d;

@@ -4,6 +4,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
@@ -71,6 +72,8 @@ Tensor per_row(const std::optional<Tensor>& t, const char* name, int64_t B, cons
   if (!t) return Tensor();
   if (t->numel() != B)
     throw py::value_error(std::string(name) + " has " + std::to_string(t->numel()) + " entries for " + std::to_string(B) + " batch rows");
+  if (t->is_floating_point() || t->is_complex() || t->scalar_type() == at::kBool) throw py::type_error(std::string(name) + " holds whole numbers");
+  if (t->scalar_type() == at::kLong) return t->clamp(INT32_MIN, INT32_MAX).to(dev, at::kInt).contiguous();  // ("no limit" stays one)
   return t->to(dev, at::kInt).contiguous();
 }
 const int* int_ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr<int>() : nullptr; }
@@ -86,6 +89,16 @@ bool needs_function(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && !ncn_ext::plain(*t)) return true;
   return false;
+}
+
+// There is no second derivative: what a pass with create_graph gets leads back to the inputs through an error, not to a silent zero.
+variable_list once(variable_list&& grads, Node& node, bool graph) {
+  if (!graph) return std::move(grads);
+  std::shared_ptr<Node> error(new torch::autograd::Error(node.name() + " has no derivative of its own", torch::autograd::edge_list(node.next_edges())),
+                              torch::autograd::deleteNode);
+  for (Tensor& t : grads)
+    if (t.defined()) torch::autograd::set_history(t, error);
+  return std::move(grads);
 }
 
 // ---------------------------------------------------------------- windowed attention
@@ -106,6 +119,7 @@ struct WindowNode : public Node {
   }
   variable_list apply(variable_list&& g) override {
     std::lock_guard<std::mutex> lock(mutex_);
+    const bool graph = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
     if (!g[0].defined()) return variable_list(3);
     const Tensor Q = q.unpack(), K = k.unpack(), V = v.unpack(), Y = y.unpack(shared_from_this()), L = state.unpack();
@@ -127,7 +141,7 @@ struct WindowNode : public Node {
                                 L.const_data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), int_ptr(ctx), int_ptr(st), s,
                                 ws.data_ptr(), bytes, B, Nq, Nk, E, Ek, (int)c.n_head, c.window, c.n_sink, c.start, c.scale, dt,
                                 stream_of(Q)));
-    return {dq, dk, dv};
+    return once({dq, dk, dv}, *this, graph);
   }
 };
 
@@ -262,6 +276,7 @@ struct RotaryNode : public Node {
   }
   variable_list apply(variable_list&& g) override {
     std::lock_guard<std::mutex> lock(mutex_);
+    const bool graph = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
     if (!g[0].defined() && !(g.size() > 1 && g[1].defined())) return variable_list(4);
     const Tensor& any = g[0].defined() ? g[0] : g[1];
@@ -274,7 +289,7 @@ struct RotaryNode : public Node {
     variable_list out(4);
     if (!norm) {
       rotate(gq, gk, Tensor(), Tensor(), f, p, c, true, out[0], out[1]);
-      return out;
+      return once(std::move(out), *this, graph);
     }
     const Tensor Q = q.unpack(), K = has_k ? k.unpack() : Tensor();
     const int64_t B = Q.size(0), N = Q.size(1), E = Q.size(2), Ek = has_k ? K.size(2) : 0, d = E / c.n_head;
@@ -302,7 +317,7 @@ struct RotaryNode : public Node {
     }
     out[2] = dwq.to(opt_wq.device(), c10::typeMetaToScalarType(opt_wq.dtype()));
     if (has_k) out[3] = dwk.to(opt_wk.device(), c10::typeMetaToScalarType(opt_wk.dtype()));
-    return out;
+    return once(std::move(out), *this, graph);
   }
 };
 

@@ -340,6 +340,10 @@ def _per_row(t, name, B, device):
     t = torch.as_tensor(t)
     if t.numel() != B:
         raise ValueError(f"{name} has {t.numel()} entries for {B} batch rows")
+    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        raise TypeError(f"{name} holds whole numbers")
+    if t.dtype == torch.int64:  # ("no limit" stays one)
+        t = t.clamp(-(2**31), 2**31 - 1)
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 

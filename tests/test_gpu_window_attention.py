@@ -372,6 +372,52 @@ def test_decode_captured_and_strided():
 
 
 # ---------------------------------------------------------------- refusals, and calls side by side
+@pytest.mark.parametrize("dtype,d", [(F32, 16), (BF16, 64), (BF16, 12)])
+def test_many_sinks(dtype, d):
+    """More tiles of sinks than the far queries are cut for: fewer pieces each."""
+    q, k, v, dy = make(d, 1, 4000, 4000, 1, 1, d, dtype)
+    check(q, k, v, dy, 1, 8, 3500)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_no_second_derivative(native):
+    q, k, v, dy = make(3, 1, 40, 40, 2, 1, 32, F32)
+    freqs, _ = ncn.rotary_frequencies(32, device="cuda")
+    q, k, v, dy = (t.requires_grad_(True) for t in (q, k, v, dy))
+
+    def apply(f, *args):
+        return f.apply(*args) if native else torch.autograd.Function.apply.__func__(f, *args)
+
+    y = apply(ncn.WindowAttentionFunction, q, k, v, 2, 9, 1, 0.2, None, None, 0)
+    r, _ = apply(ncn.RotaryFunction, q, k, None, None, freqs, None, 2, 0, False, 0.0, 1.0)
+    w = torch.ones(32, device="cuda", requires_grad=True)
+    n, _ = apply(ncn.RotaryFunction, q, k, w, w, freqs, None, 2, 0, False, 1e-6, 1.0)
+    for out in (y, r, n) if native else (y, n):  # (of a rotation the gradient does not depend on what was turned)
+        g, = torch.autograd.grad(out, q, dy, create_graph=True)
+        for loss in (g.sum(), g.sum() + (q * q).sum()):
+            with pytest.raises(RuntimeError, match="derivative of its own"):
+                torch.autograd.grad(loss, q, retain_graph=True)
+
+
+def test_lengths_beyond_32_bits():
+    """A length that means "no limit" stays one; lengths are whole numbers."""
+    q, k, v, dy = make(5, 2, 70, 70, 2, 1, 64, BF16)
+    whole = ncn.fused_window_attention(q, k, v, 2, 9)
+    for most in (2**31 - 1, 2**32, 2**40, 2**63 - 1):
+        ctxlen = torch.full((2,), most, device="cuda")
+        assert torch.equal(whole, ncn.fused_window_attention(q, k, v, 2, 9, ctxlen=ctxlen, q_start=0))
+        assert torch.equal(whole, ops.window_fwd(q, k, v, 2, 9, 0, 0.125, 0, ctxlen=ctxlen)[0])
+        last = ncn.window_attention_decode(q[:, -1:], k, v, ctxlen, 2, 9)
+        assert torch.equal(last, ncn.window_attention_decode(q[:, -1:], k, v, torch.tensor([70, 70]), 2, 9))
+        assert not ncn.fused_window_attention(q, k, v, 2, 9, q_start=ctxlen).any()
+        assert not ncn.fused_window_attention(q, k, v, 2, 9, ctxlen=-ctxlen).any()
+    for bad in (torch.tensor([3.0, 4.0]), torch.tensor([True, False])):
+        for call in (lambda: ncn.fused_window_attention(q, k, v, 2, 9, ctxlen=bad), lambda: ncn.fused_window_attention(q, k, v, 2, 9, q_start=bad),
+                     lambda: ncn.window_attention_decode(q[:, :1], k, v, bad, 2, 9), lambda: ops.window_fwd(q, k, v, 2, 9, 0, 1.0, 0, ctxlen=bad)):
+            with pytest.raises(TypeError, match="whole numbers"):
+                call()
+
+
 def test_refusals_on_the_device():
     q, k, v, _ = make(1, 2, 8, 8, 4, 2, 32, BF16)
     freqs, _ = ncn.rotary_frequencies(32, device="cuda")

@@ -68,6 +68,8 @@ def test_sizes_of_buffers():
     assert lib.ncn_window_bwd_workspace_bytes(2, 130, 130, 256, 64, 4, 16, 0, 1) == 2 * 4 * 256 * 4       # no sinks
     assert lib.ncn_window_bwd_workspace_bytes(2, 130, 130, 256, 64, 4, 16, 5, 1) > 2 * 4 * 256 * 4
     assert lib.ncn_window_bwd_workspace_bytes(2, 130, 130, 256, 100, 4, 16, 5, 1) == 0
+    # many sinks: in proportion to dk and dv in fp32 (2 x 2 of them and 256 pieces of 128 x 128), not to their pieces times the tiles
+    assert lib.ncn_window_bwd_workspace_bytes(1, 131072, 131072, 128, 128, 1, 1024, 65536, 1) <= (4 * 131072 + 2 * 256 * 128 + 131072) * 128 * 4
     assert lib.ncn_qk_norm_rotary_workspace_bytes(2, 3, 64, 4) == 2 * 3 * 4 * 2 * 16 * 4
     assert lib.ncn_qk_norm_rotary_workspace_bytes(1 << 20, 1 << 20, 64, 4) == 8192 * 2 * 16 * 4
 
@@ -126,3 +128,7 @@ def test_layer_arguments():
     layer.to(torch.bfloat16)
     assert layer.qkv.weight.dtype == torch.bfloat16 and layer.freqs.dtype == torch.float64 and layer.freqs.shape == (4,)
     assert ctypes.sizeof(ctypes.c_int64) == 8
+    with torch.device("meta"):
+        layer = ncn.NCNWindowAttention(64, 4, 8)
+    assert layer.qkv.weight.is_meta and layer.freqs.device.type == "cpu"
+    assert layer.to_empty(device="cpu").freqs.dtype == torch.float64
