@@ -1,6 +1,9 @@
 // Windowed attention of the last few positions of each row over a cache: the form for single tokens.
 //
-// Bound by reading the visible keys and values once.  A CTA of 8 warps takes the queries of one key/value head (the heads of its
+// Bound by reading the visible keys and values once (64 rows, windows of 4096, 8 heads of 128: 1.08 GB in 180 us, 6.0 of the 6.46 TB/s
+// that a plain copy reaches); one row's time is a launch, the latency of its loads and the joins (7 us).
+//
+// A CTA of 8 warps takes the queries of one key/value head (the heads of its
 // group times the new positions, up to 16 rows at a time); the visible keys, sinks first and the window behind them, are dealt out to the
 // warps of a cluster of CTAs in blocks, every warp keeps a running softmax of its own, and the parts are joined through shared
 // memory, first in the CTA, then in the cluster over distributed shared memory: one launch, no workspace, and one order of sums.

@@ -12,6 +12,16 @@
 //
 // The backward is two kernels, one that owns queries and one that owns keys.  It computes the scores twice, 7 products for 5, and in
 // return no sum depends on the order in which CTAs finish.
+//
+// Rounded to bf16: the weights P and the gradients dS, as operands of the second products (each term off by at
+// most 2^-8, like the results' own rounding: results end up about 1.4 times as far from the exact ones as that alone puts them).  Scores,
+// softmax sums, delta and all sums over keys or queries are fp32.
+//
+// Measured (2 x 4096 positions, 16 heads of 128 on 4 of keys, windows of 1024, 4 sinks): forward 89 us, dq 126, dk and dv 123, 680 to 980
+// TFLOP/s over the visible pairs; 16384 positions, windows of 4096: forward 428 us, 1120 TFLOP/s (1688 is what plain matrix products
+// reach).  Per tile the bound is the exchange between the two sides: 3000 cycles per pair of tiles against 2048 of the products
+// alone (score to weight to product, each waiting for the one before).  For short windows it is the CTA: first loads, epilogue
+// and uneven ends take some 10 us of each, and 256 or 512 of them on 148 SMs leave the last round part empty.
 #include <cuda.h>
 
 #include "attn_tensor.h"

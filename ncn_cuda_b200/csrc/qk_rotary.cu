@@ -4,7 +4,12 @@
 //   (a, b) pair i of u:  a' = M (a cos - b sin),  b' = M (b cos + a sin),  angle = position * frequency_i
 // Backward: g = the cotangent rotated by the opposite angle;  dw = sum g x r,  dx = r (g w - x r mean(g w x r)).
 //
-// One pass over the data: 2 tensors forward, 3 backward, which is what bounds it.  Angles are formed in 64 bits as turns
+// One pass over the data: 2 tensors forward, 3 backward, which is what bounds it.  Measured (bf16, 32768 positions, 32 + 8 heads of
+// 128): 122 us forward, 194 backward with norms, 5.5 and 5.2 of the 6.46 TB/s that a plain copy reaches, with three quarters of the
+// instruction slots in use.  Teams that keep a position and walk its heads need fewer instructions but were slower (131, 207: their
+// reads lie 10 KB apart), and so were bulk prefetches of the next span into L2 (139, 228).
+//
+// Angles are formed in 64 bits as turns
 // (position * frequency / 2 pi minus the nearest whole number), so that far positions lose nothing; what is left is below half a
 // turn and goes through sincospi in 32 bits.  A sine and cosine cost more instructions than everything else of a pair of
 // features: they are formed once per position, into shared memory, for all heads.
