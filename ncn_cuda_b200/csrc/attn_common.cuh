@@ -155,6 +155,8 @@ __device__ __forceinline__ float ex2(float x) {
 // launchers
 cudaError_t launch_attn_simt_fwd(const AttnParams& p, int dtype, cudaStream_t st);
 cudaError_t launch_attn_simt_bwd(const AttnParams& p, int dtype, cudaStream_t st);
+cudaError_t launch_attn_split_fwd(const AttnParams& p, cudaStream_t st);
+cudaError_t launch_attn_split_bwd(const AttnParams& p, cudaStream_t st);  // (but for the sum of the sinks' parts)
 cudaError_t launch_attn_sink_sum(const AttnParams& p, int dtype, int tile, cudaStream_t st);
 cudaError_t launch_attn_decode(const AttnParams& p, int dtype, int sms, cudaStream_t st);
 

@@ -407,6 +407,7 @@ cudaError_t run_bwd(const AttnParams& p, cudaStream_t st) {
   const int items = (p.Nk + kOwn - 1) / kOwn + p.sink_tiles * p.chunks;
   return launch_behind(attn_simt_dkv_kernel<T, DP>, dim3((unsigned)(items * p.Hk * p.B)), 256, smem_dkv<T, DP>(), st, p);
 }
+bool split_covers(const AttnParams& p, int dtype) { return dtype == DT_F32 && p.d > 16 && p.d <= 128; }
 template <typename T>
 cudaError_t by_size(const AttnParams& p, bool bwd, cudaStream_t st) {
   if (p.d <= 32) return bwd ? run_bwd<T, 32>(p, st) : run_fwd<T, 32>(p, st);
@@ -419,10 +420,13 @@ cudaError_t by_size(const AttnParams& p, bool bwd, cudaStream_t st) {
 }  // namespace
 
 cudaError_t launch_attn_simt_fwd(const AttnParams& p, int dtype, cudaStream_t st) {
+  if (split_covers(p, dtype)) return launch_attn_split_fwd(p, st);
   return dtype == DT_BF16 ? by_size<__nv_bfloat16>(p, false, st) : by_size<float>(p, false, st);
 }
 cudaError_t launch_attn_simt_bwd(const AttnParams& p, int dtype, cudaStream_t st) {
-  cudaError_t e = dtype == DT_BF16 ? by_size<__nv_bfloat16>(p, true, st) : by_size<float>(p, true, st);
+  cudaError_t e = split_covers(p, dtype) ? launch_attn_split_bwd(p, st)
+                  : dtype == DT_BF16     ? by_size<__nv_bfloat16>(p, true, st)
+                                         : by_size<float>(p, true, st);
   if (e != cudaSuccess || p.chunks == 0) return e;
   return launch_attn_sink_sum(p, dtype, kOwn, st);
 }
