@@ -216,7 +216,8 @@ size_t ncn_ckpt_bytes(int64_t B, int64_t N, int64_t E, int L, int ckpt_every, in
  * values have Ek / d heads, each shared by n_head * d / Ek consecutive heads of the queries.  Inputs may be views: `strides` (a host
  * array, or null for contiguous tensors) gives {row, position} strides in elements of q, k, v (and of dy in the backward); the
  * features of a position are next to each other.  Results are contiguous.  d up to 256 (attention), 512 (rotation).  bf16 with d a
- * multiple of 8 up to 128, tensors on 16-byte boundaries and strides that are multiples of 8 runs on the tensor cores, the rest on the FMA pipes.
+ * multiple of 8 up to 128, tensors on 16-byte boundaries and strides that are multiples of 8 runs on the tensor cores; fp32 with d from 17 to
+ * 128 too, three products for one (an infinity, or a value within 2^-12 of the largest, gives NaN there); the rest on the FMA pipes.
  *
  * Windowed attention.  Query i of row b is at position p = start_b + i, key j at position j, ctx_b = clamp(ctxlen[b], 0, Nk):
  *   query i sees key j  where  j < ctx_b,  j <= p < ctx_b  and  (p - j < window or j < n_sink)

@@ -1,5 +1,5 @@
-// Windowed attention on the FMA pipes: fp32 storage (whose results keep 32-bit accuracy, which the tensor cores' formats do not
-// give), and bf16 with head sizes or alignments that the tensor-core kernels do not take.
+// Windowed attention on the FMA pipes: fp32 with heads of more than 128 or at most 16 features, and bf16 with head sizes or alignments that
+// the tensor-core kernels do not take.  (fp32 between these: attn_split.cu.)
 //
 // A CTA of 256 threads owns 64 rows (queries; in the backward of the keys: keys) and walks the tiles of the other side.  Thread
 // (ty, tx) of 16 x 16 holds rows 4 ty .. 4 ty + 3.  Tiles are fp32 in shared memory whatever the storage type; a row is DP + 4
@@ -7,10 +7,10 @@
 // 32, 64, 96, 128 or 256: without 96, heads of 72 to 96 did a third more products on zeros.
 //
 // What bounds it: the reads of shared memory.  A product over 4 features takes a thread 8 reads of 16 bytes, which return to a
-// warp in 32 cycles, for 64 FMAs, which take 16: half the FMA rate (36 of 72 TFLOP/s) is the most this split can give.  Measured,
-// 2 x 4096 positions of 8 heads, windows of 1024: heads of 128 forward 928 us (32.4 TFLOP/s), dq 1332 (33.9), dk and dv 1761
-// (34.2); heads of 64 453, 649, 862 us (33 to 35).  Tiles of 8 rows a thread would lower the reads by a quarter, but with heads
-// of 128 the backward's four tiles then no longer fit in shared memory.
+// warp in 32 cycles, for 64 FMAs, which take 16: half the FMA rate (36 of 72 TFLOP/s) is the most this split can give.  Measured:
+// fp32, heads of 128, 2 x 4096 positions of 8 heads, windows of 1024, forward 928 us (32.4 TFLOP/s), dq 1332 (33.9), dk and dv
+// 1761 (34.2); bf16, heads of 256, 2 x 2048 positions, windows of 512: 556, 833, 1031 us (27 to 29).  Tiles of 8 rows a thread would
+// lower the reads by a quarter, but with large heads the backward's four tiles then no longer fit in shared memory.
 #include "attn_common.cuh"
 #include "ncn_common.cuh"
 
@@ -407,13 +407,16 @@ cudaError_t run_bwd(const AttnParams& p, cudaStream_t st) {
   const int items = (p.Nk + kOwn - 1) / kOwn + p.sink_tiles * p.chunks;
   return launch_behind(attn_simt_dkv_kernel<T, DP>, dim3((unsigned)(items * p.Hk * p.B)), 256, smem_dkv<T, DP>(), st, p);
 }
+// (With few features the products' error of 2^-22 would stand out against their sum's.)
 bool split_covers(const AttnParams& p, int dtype) { return dtype == DT_F32 && p.d > 16 && p.d <= 128; }
 template <typename T>
 cudaError_t by_size(const AttnParams& p, bool bwd, cudaStream_t st) {
   if (p.d <= 32) return bwd ? run_bwd<T, 32>(p, st) : run_fwd<T, 32>(p, st);
-  if (p.d <= 64) return bwd ? run_bwd<T, 64>(p, st) : run_fwd<T, 64>(p, st);
-  if (p.d <= 96) return bwd ? run_bwd<T, 96>(p, st) : run_fwd<T, 96>(p, st);
-  if (p.d <= 128) return bwd ? run_bwd<T, 128>(p, st) : run_fwd<T, 128>(p, st);
+  if constexpr (sizeof(T) == 2) {
+    if (p.d <= 64) return bwd ? run_bwd<T, 64>(p, st) : run_fwd<T, 64>(p, st);
+    if (p.d <= 96) return bwd ? run_bwd<T, 96>(p, st) : run_fwd<T, 96>(p, st);
+    if (p.d <= 128) return bwd ? run_bwd<T, 128>(p, st) : run_fwd<T, 128>(p, st);
+  }
   return bwd ? run_bwd<T, 256>(p, st) : run_fwd<T, 256>(p, st);
 }
 

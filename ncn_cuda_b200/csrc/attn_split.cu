@@ -2,14 +2,19 @@
 //
 //   x = hi + lo, hi: x rounded to 11 bits, lo: what is left (12 bits and a sign, of which the products use 11)
 //   a b = hi hi + (hi lo + lo hi), the second sum in accumulators of its own; lo lo, 2^-22 of the product at most, is left out
-// A product is off by about 2^-23 of its size, as far as fp32 multiplications and additions one after the other are.  The
-// products' units may cut where fp32 additions round: a sum therefore runs over one tile in them, and tiles are added in fp32.
+// A product is off by 2^-20.4 of its size at most (2^-22 for each lo that loses its last bit and for lo lo) and by 2^-24 as a rule, as
+// far as fp32 additions one after the other are: results are 1.0 to 1.7 times as far from the exact ones as with fp32 products.
+// The matrix unit may cut where fp32 additions round: a sum therefore runs over one tile in it, and tiles are added in fp32.
 //
 // A CTA of 4 warps owns 64 rows (queries; in the backward of the keys: keys), 16 a warp, and walks the tiles of the other side in shared
 // memory; two or more CTAs fit on an SM.  Scores never leave registers: the accumulators' columns 2 c and 2 c + 1 of a lane are the
 // entries c and c + 4 of the next product's left operand, if its rows are taken in that order (the order of a sum's terms is free).
 // A row in shared memory is DP + 4 floats: the 32 lanes of an operand's load hit 32 different banks both ways.  While one tile of
 // a pair is worked on, the other's successor is on its way (cp.async).
+//
+// Measured, 2 x 4096 positions of 8 heads, windows of 1024: heads of 128 forward 616 us (48.8 TFLOP/s), dq 949 (47.5), dk and dv 1262
+// (47.7); heads of 64 317, 462, 624 (48); on the FMA pipes 928, 1332, 1761 and 453, 649, 862.  The matrix unit is 50 to 56 % busy (three
+// products: 275 TFLOP/s of tf32 would be 92 here); more CTAs, smaller tiles and more independent accumulators change nothing.
 #include "attn_common.cuh"
 #include "ncn_common.cuh"
 
@@ -17,8 +22,13 @@ namespace ncn {
 namespace {
 
 constexpr int kOwn = 64, kCta = 128;
-// rows of the other side's tiles: the backward holds two tiles of its own, and 32 let a second CTA fit beside it where heads are large
+// Rows of the other side's tiles: the backward holds two tiles of its own, and 32 let a second CTA fit beside it where heads are large.
+// CTAs per SM that the registers leave room for.  (Heads of 128 forward with 32 rows and three CTAs 642 us, as below 610; heads of
+// 64 backward with 32 rows and three CTAs 478 + 641, as below 461 + 612.)
+constexpr int kFwdRows = 64;
 template <int DP> constexpr int bwd_rows() { return DP > 64 ? 32 : 64; }
+template <int DP> constexpr int fwd_ctas() { return DP > 96 ? 2 : 3; }
+template <int DP> constexpr int bwd_ctas() { return DP > 32 ? 2 : 3; }
 
 struct Parts {
   uint32_t hi, lo;
@@ -30,7 +40,7 @@ __device__ __forceinline__ Parts split(float x) {
   return p;
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -81,13 +91,15 @@ __device__ __forceinline__ void rows_by_rows(const float* A, const float* B, flo
       const Parts p = split(a_at[k + (i & 1) * 8 * (DP + 4) + (i >> 1) * 4]);
       ah[i] = p.hi, al[i] = p.lo;
     }
+    Parts b[NB][2];  // (products that follow each other go to different accumulators)
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const Parts b0 = split(b_at[8 * n * (DP + 4) + k]), b1 = split(b_at[8 * n * (DP + 4) + k + 4]);
-      mma(small[n], al, b0.hi, b1.hi);
-      mma(s[n], ah, b0.hi, b1.hi);
-      mma(small[n], ah, b0.lo, b1.lo);
-    }
+    for (int n = 0; n < NB; ++n) b[n][0] = split(b_at[8 * n * (DP + 4) + k]), b[n][1] = split(b_at[8 * n * (DP + 4) + k + 4]);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) mma(small[n], al, b[n][0].hi, b[n][1].hi);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) mma(s[n], ah, b[n][0].hi, b[n][1].hi);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) mma(small[n], ah, b[n][0].lo, b[n][1].lo);
   }
 #pragma unroll
   for (int n = 0; n < NB; ++n)
@@ -110,16 +122,16 @@ __device__ __forceinline__ void add_rows_by_cols(const float (&w)[KB][4], const 
     }
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) {
-    float big[4] = {}, small[4] = {};
+    float big[4] = {}, small[4] = {}, other[4] = {};
 #pragma unroll
     for (int k = 0; k < KB; ++k) {
       const Parts b0 = split(at[8 * k * (DP + 4) + 8 * n]), b1 = split(at[(8 * k + 1) * (DP + 4) + 8 * n]);
       mma(small, wl[k], b0.hi, b1.hi);
       mma(big, wh[k], b0.hi, b1.hi);
-      mma(small, wh[k], b0.lo, b1.lo);
+      mma(other, wh[k], b0.lo, b1.lo);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[n][i] = fmaf(acc[n][i], i < 2 ? keep0 : keep1, big[i] + small[i]);
+    for (int i = 0; i < 4; ++i) acc[n][i] = fmaf(acc[n][i], i < 2 ? keep0 : keep1, big[i] + (small[i] + other[i]));
   }
 }
 
@@ -134,9 +146,9 @@ __device__ __forceinline__ float sum4(float x) {
 }
 
 template <int DP>
-__global__ void __launch_bounds__(kCta) attn_split_fwd_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kCta, fwd_ctas<DP>()) attn_split_fwd_kernel(const AttnParams p) {
   wait_for_inputs();
-  constexpr int BN = 64, NB = BN / 8;
+  constexpr int BN = kFwdRows, NB = BN / 8;
   extern __shared__ __align__(16) float sm[];
   float *Q = sm, *K = Q + kOwn * (DP + 4), *V = K + BN * (DP + 4);
   const Block at_block = block_of(p.H, (p.Nq + kOwn - 1) / kOwn);
@@ -227,7 +239,7 @@ __global__ void __launch_bounds__(kCta) attn_split_fwd_kernel(const AttnParams p
 
 // Gradient of the queries; also leaves delta = sum(dy * y) of its rows for the backward of the keys.
 template <int DP>
-__global__ void __launch_bounds__(kCta) attn_split_dq_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kCta, bwd_ctas<DP>()) attn_split_dq_kernel(const AttnParams p) {
   wait_for_inputs();
   constexpr int BN = bwd_rows<DP>(), NB = BN / 8;
   extern __shared__ __align__(16) float sm[];
@@ -317,7 +329,7 @@ __global__ void __launch_bounds__(kCta) attn_split_dq_kernel(const AttnParams p)
 // Gradients of the keys and values.  The heads of a group are walked one after the other by the same CTA, so that their sum has
 // one order.
 template <int DP>
-__global__ void __launch_bounds__(kCta) attn_split_dkv_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kCta, bwd_ctas<DP>()) attn_split_dkv_kernel(const AttnParams p) {
   wait_for_inputs();
   constexpr int BN = bwd_rows<DP>(), NB = BN / 8;
   extern __shared__ __align__(16) float sm[];
@@ -419,7 +431,7 @@ __global__ void __launch_bounds__(kCta) attn_split_dkv_kernel(const AttnParams p
 template <int DP>
 cudaError_t run_fwd(const AttnParams& p, cudaStream_t st) {
   static SmemGrant grant;
-  constexpr size_t smem = sizeof(float) * (kOwn + 128) * (DP + 4);
+  constexpr size_t smem = sizeof(float) * (kOwn + 2 * kFwdRows) * (DP + 4);
   const cudaError_t e = grant_smem(grant, attn_split_fwd_kernel<DP>, smem);
   if (e != cudaSuccess) return e;
   return launch_behind(attn_split_fwd_kernel<DP>, dim3((unsigned)((p.Nq + kOwn - 1) / kOwn * p.H * p.B)), kCta, smem, st, p);

@@ -371,6 +371,22 @@ def test_decode_captured_and_strided():
     assert torch.equal(y, check_decode(q, kc, vc, H, 300, 4, ctxlen))
 
 
+@pytest.mark.parametrize("d", [24, 50, 64, 100, 128])
+def test_fp32_features_of_all_sizes(d):
+    """fp32 heads of 17 to 128 features go through products of two parts each: small features beside large ones keep their bits."""
+    q, k, v, dy = make(d, 1, 200, 200, 2, 1, d, F32)
+    g = torch.Generator(device="cuda").manual_seed(d)
+    e = torch.randint(-30, 31, (2, 1, 1, d), generator=g, device="cuda").float()
+    q, dy = q * torch.exp2(e[0]).repeat(1, 1, 2), dy * torch.exp2(-e[1]).repeat(1, 1, 2)
+    k, v = k * torch.exp2(-e[0]), v * torch.exp2(e[1])
+    check(q, k, v, dy, 2, 60, 3)
+
+
+def test_fp32_many_sinks_and_chunks():
+    q, k, v, dy = make(8, 2, 700, 1500, 4, 2, 40, F32)
+    check(q, k, v, dy, 4, 30, 900, ctxlen=torch.tensor([1500, 1033], device="cuda"))
+
+
 # ---------------------------------------------------------------- refusals, and calls side by side
 @pytest.mark.parametrize("dtype,d", [(F32, 16), (BF16, 64), (BF16, 12)])
 def test_many_sinks(dtype, d):
