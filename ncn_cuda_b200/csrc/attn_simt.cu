@@ -4,7 +4,7 @@
 // A CTA of 256 threads owns 64 rows (queries; in the backward of the keys: keys) and walks the tiles of the other side.  Thread
 // (ty, tx) of 16 x 16 holds rows 4 ty .. 4 ty + 3.  Tiles are fp32 in shared memory whatever the storage type; a row is DP + 4
 // floats, so that eight lanes that read eight rows 16 bytes at a time hit 32 different banks.  DP is the head size, rounded up to
-// 32, 64, 96, 128 or 256: without 96, heads of 72 to 96 did a third more products on zeros.
+// 32, 64, 96, 128 or 256 (fp32: 32 or 256): without 96, heads of 72 to 96 did a third more products on zeros.
 //
 // What bounds it: the reads of shared memory.  A product over 4 features takes a thread 8 reads of 16 bytes, which return to a
 // warp in 32 cycles, for 64 FMAs, which take 16: half the FMA rate (36 of 72 TFLOP/s) is the most this split can give.  Measured:

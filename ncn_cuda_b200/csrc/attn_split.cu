@@ -9,11 +9,11 @@
 // A CTA of 4 warps owns 64 rows (queries; in the backward of the keys: keys), 16 a warp, and walks the tiles of the other side in shared
 // memory; two or more CTAs fit on an SM.  Scores never leave registers: the accumulators' columns 2 c and 2 c + 1 of a lane are the
 // entries c and c + 4 of the next product's left operand, if its rows are taken in that order (the order of a sum's terms is free).
-// A row in shared memory is DP + 4 floats: the 32 lanes of an operand's load hit 32 different banks both ways.  While one tile of
+// A row in shared memory is DP + 4 floats (DP: the head size rounded up to 32, 48, 64, 80, 96 or 128): the 32 lanes of an operand's load hit 32 different banks both ways.  While one tile of
 // a pair is worked on, the other's successor is on its way (cp.async).
 //
 // Measured, 2 x 4096 positions of 8 heads, windows of 1024: heads of 128 forward 616 us (48.8 TFLOP/s), dq 949 (47.5), dk and dv 1262
-// (47.7); heads of 64 317, 462, 624 (48); on the FMA pipes 928, 1332, 1761 and 453, 649, 862.  The matrix unit is 50 to 56 % busy (three
+// (47.7); heads of 80 401, 634, 828 (in tiles of 96 features 472, 733, 983); heads of 64 317, 462, 624 (48); on the FMA pipes 928, 1332, 1761 and 453, 649, 862.  The matrix unit is 50 to 56 % busy (three
 // products: 275 TFLOP/s of tf32 would be 92 here); more CTAs, smaller tiles and more independent accumulators change nothing.
 #include "attn_common.cuh"
 #include "ncn_common.cuh"
@@ -453,10 +453,20 @@ cudaError_t run_bwd(const AttnParams& p, cudaStream_t st) {
 }  // namespace
 
 cudaError_t launch_attn_split_fwd(const AttnParams& p, cudaStream_t st) {
-  return p.d <= 32 ? run_fwd<32>(p, st) : p.d <= 64 ? run_fwd<64>(p, st) : p.d <= 96 ? run_fwd<96>(p, st) : run_fwd<128>(p, st);
+  return p.d <= 32   ? run_fwd<32>(p, st)
+         : p.d <= 48 ? run_fwd<48>(p, st)
+         : p.d <= 64 ? run_fwd<64>(p, st)
+         : p.d <= 80 ? run_fwd<80>(p, st)
+         : p.d <= 96 ? run_fwd<96>(p, st)
+                     : run_fwd<128>(p, st);
 }
 cudaError_t launch_attn_split_bwd(const AttnParams& p, cudaStream_t st) {
-  return p.d <= 32 ? run_bwd<32>(p, st) : p.d <= 64 ? run_bwd<64>(p, st) : p.d <= 96 ? run_bwd<96>(p, st) : run_bwd<128>(p, st);
+  return p.d <= 32   ? run_bwd<32>(p, st)
+         : p.d <= 48 ? run_bwd<48>(p, st)
+         : p.d <= 64 ? run_bwd<64>(p, st)
+         : p.d <= 80 ? run_bwd<80>(p, st)
+         : p.d <= 96 ? run_bwd<96>(p, st)
+                     : run_bwd<128>(p, st);
 }
 
 }  // namespace ncn
