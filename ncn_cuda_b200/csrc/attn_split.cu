@@ -23,8 +23,8 @@ namespace {
 
 constexpr int kOwn = 64, kCta = 128;
 // Rows of the other side's tiles: the backward holds two tiles of its own, and 32 let a second CTA fit beside it where heads are large.
-// CTAs per SM that the registers leave room for.  (Heads of 128 forward with 32 rows and three CTAs 642 us, as below 610; heads of
-// 64 backward with 32 rows and three CTAs 478 + 641, as below 461 + 612.)
+// CTAs per SM that the registers leave room for.  (Heads of 128 forward with 32 rows and three CTAs 642 us, as below 616; heads of
+// 64 backward with 32 rows and three CTAs 478 + 641, as below 462 + 624.)
 constexpr int kFwdRows = 64;
 template <int DP> constexpr int bwd_rows() { return DP > 64 ? 32 : 64; }
 template <int DP> constexpr int fwd_ctas() { return DP > 96 ? 2 : 3; }
