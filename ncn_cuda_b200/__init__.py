@@ -9,6 +9,7 @@ from .attention import (
     NCNWindowAttention,
     RotaryFunction,
     WindowAttentionFunction,
+    WindowDecodeFunction,
     fused_qk_norm_rotary,
     fused_rotary,
     fused_window_attention,
@@ -36,6 +37,6 @@ __all__ = [
     "NCNNetTestCuda", "RefTorchNaive", "ref_naive_fwd", "group_pos_to_index_v2", "NCNFunctionPytorch",
     "RefInvTorchNaive", "NCNResidualStack", "allreduce_weight_grads", "shard_rows", "NCNContextFunction",
     "fused_ncn_cuda_ctxlen",
-    "set_stage_backward", "NCNWindowAttention", "RotaryFunction", "WindowAttentionFunction", "fused_qk_norm_rotary", "fused_rotary",
+    "set_stage_backward", "NCNWindowAttention", "RotaryFunction", "WindowAttentionFunction", "WindowDecodeFunction", "fused_qk_norm_rotary", "fused_rotary",
     "fused_window_attention", "rotary_frequencies", "window_attention_decode",
 ]

@@ -159,6 +159,26 @@ class WindowAttentionFunction(torch.autograd.Function):
         return (*_once((dq, dk, dv), q, k, v, dy), None, None, None, None, None, None, None)
 
 
+class WindowDecodeFunction(torch.autograd.Function):
+    """Windowed attention over a cache; `apply` goes to the native form, as in RotaryFunction.  It has no gradient: the Function is there
+    for calls that are traced, and refuses transforms and forward gradients as any custom Function does."""
+
+    @classmethod
+    def apply(cls, *args):
+        if cls is not WindowDecodeFunction:
+            return super().apply(*args)
+        out = _lib.native().window_decode(*args)
+        return super().apply(*args) if out is None else out
+
+    @staticmethod
+    def forward(ctx, q, k_cache, v_cache, ctxlen, n_head, window, n_sink, scale):
+        return ops.window_decode(q, k_cache, v_cache, ctxlen, n_head, window, n_sink, scale)
+
+    @staticmethod
+    def backward(ctx, dy):
+        raise RuntimeError("window_attention_decode has no gradient: use fused_window_attention")
+
+
 def _window(window, n_sink, scale, q, n_head):
     window = ops.NO_WINDOW if window is None else int(window)
     if window < 1 or n_sink < 0:
@@ -200,7 +220,7 @@ def window_attention_decode(q, k_cache, v_cache, ctxlen, n_head, window, n_sink=
     window, scale = _window(window, n_sink, scale, q, n_head)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_cache, v_cache)):
         raise RuntimeError("window_attention_decode has no gradient: use fused_window_attention, or torch.no_grad()")
-    return _lib.native().window_decode(q, k_cache, v_cache, torch.as_tensor(ctxlen), n_head, window, n_sink, scale)
+    return WindowDecodeFunction.apply(q, k_cache, v_cache, torch.as_tensor(ctxlen), n_head, window, n_sink, scale)
 
 
 class NCNWindowAttention(nn.Module):

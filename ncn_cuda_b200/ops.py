@@ -393,6 +393,23 @@ def window_bwd(q, k, v, y, dy, state, n_head, window, n_sink, scale, start, ctxl
     return dq, dk, dv
 
 
+def window_decode(q, k, v, ctxlen, n_head, window, n_sink, scale):
+    """Returns y: the last positions of each row over caches k and v."""
+    lib = _lib.load()
+    _check_qkv(q, k, v, n_head)
+    (B, Nq, E), (_, S, Ek) = q.shape, k.shape
+    ctxlen = _per_row(ctxlen, "ctxlen", B, q.device)
+    (q, k, v), strides = _strided(q, k, v)
+    y = torch.empty_like(q, memory_format=torch.contiguous_format)
+    with _on(q.device):
+        rc = lib.ncn_window_decode(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(), _ptr(ctxlen), strides, B, Nq, S, E, Ek, n_head, window, n_sink, scale,
+            _dtype_code(q), _stream(),
+        )
+    _lib.check("ncn_window_decode", rc)
+    return y
+
+
 def _rotary_args(q, k, freqs, positions, n_head):
     _check_inputs(q)
     B, N, E = q.shape

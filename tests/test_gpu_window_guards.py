@@ -1,0 +1,87 @@
+"""Attention operators at the edges of what they take: traced and transformed calls, scores that overflow, places that nobody sees, views
+off the 16-byte grid, mixed precision, many rows."""
+import math
+
+import pytest
+import torch
+
+import ncn_cuda_b200 as ncn
+from ncn_cuda_b200 import ops
+from tests import window_oracle as O
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def make(seed, B, Nq, Nk, H, Hk, d, dtype):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda n, h: torch.randn(B, n, h * d, generator=g, device="cuda").to(dtype)  # noqa: E731
+    return r(Nq, H), r(Nk, Hk), r(Nk, Hk), r(Nq, H)
+
+
+# ---------------------------------------------------------------- calls that are traced or transformed
+def _call(kind):
+    """-> a call of tensors alone, and its tensors"""
+    q, k, v, _ = make(1, 2, 40, 40, 2, 1, 32, F32)
+    freqs, _ = ncn.rotary_frequencies(32, device="cuda")
+    lengths = torch.tensor([40, 21], device="cuda")
+    w = torch.ones(32, device="cuda")
+    if kind == "window":
+        return lambda a, b, c: ncn.fused_window_attention(a, b, c, 2, 9, n_sink=1, ctxlen=lengths), [q, k, v]
+    if kind == "rotary":
+        return lambda a, b: ncn.fused_rotary(a, b, freqs, 2), [q, k]
+    if kind == "norm_rotary":
+        return lambda a, b, c, e: ncn.fused_qk_norm_rotary(a, b, c, e, freqs, 2, positions=3), [q, k, w, w]
+    return lambda a, b, c: ncn.window_attention_decode(a, b, c, lengths, 2, 9, n_sink=1), [q[:, :2].contiguous(), k, v]
+
+
+@pytest.mark.parametrize("kind", ["window", "rotary", "norm_rotary", "decode"])
+def test_a_traced_call_computes(kind):
+    call, args = _call(kind)
+    with torch.no_grad():
+        traced = torch.jit.trace(call, tuple(args), check_trace=False)
+        other = [a.flip(1) if a.dim() == 3 else 2 * a for a in args]
+        got, want = traced(*other), call(*other)
+    for p, q in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+        assert torch.equal(p, q)
+
+
+def test_a_traced_step_computes():
+    torch.manual_seed(1)
+    layer = ncn.NCNWindowAttention(64, 2, 9, n_sink=1, n_kv_head=1).cuda().requires_grad_(False)
+    x, other = torch.randn(2, 2, 1, 64, device="cuda")
+    lengths = torch.tensor([1, 1], device="cuda")
+
+    def step(x, k, v):
+        return layer.step(x, (k, v), lengths)
+
+    traced = torch.jit.trace(step, (x, *layer.new_cache(2, 8)), check_trace=False)
+    assert torch.equal(traced(other, *layer.new_cache(2, 8)), step(other, *layer.new_cache(2, 8)))
+
+
+@pytest.mark.parametrize("kind", ["window", "rotary", "norm_rotary", "decode"])
+def test_transforms_are_refused(kind):
+    """No forward-mode rule and no vmap rule: a dual tensor or a functorch transform is an error, never a lost tangent."""
+    import torch.autograd.forward_ad as fwAD
+
+    call, args = _call(kind)
+    for i in range(len(args)):
+        with fwAD.dual_level(), pytest.raises(NotImplementedError, match="jvp"):
+            call(*[fwAD.make_dual(t, torch.ones_like(t)) if i == k else t for k, t in enumerate(args)])
+    with pytest.raises(RuntimeError, match="setup_context"):
+        torch.func.vmap(lambda a: call(a, *args[1:]))(torch.stack([args[0], args[0]]))
+    with torch.no_grad():  # with the level left, the same tensors are taken
+        call(*args)
+
+
+def test_function_form_of_decode_agrees():
+    for dtype, d in ((BF16, 64), (F32, 40), (BF16, 20)):
+        q, k, v, _ = make(9, 3, 2, 130, 4, 1, d, dtype)
+        args = (torch.tensor([130, 77, 0], device="cuda"), 4, 20, 3, 0.125)
+        a = ncn.WindowDecodeFunction.apply(q, k, v, *args)
+        b = torch.autograd.Function.apply.__func__(ncn.WindowDecodeFunction, q, k, v, *args)
+        assert torch.equal(a, b)
+    with pytest.raises(TypeError, match="whole numbers"):
+        ops.window_decode(q, k, v, torch.tensor([1.0, 2.0, 3.0]), 4, 20, 3, 0.125)
+    with pytest.raises(ValueError, match="ctxlen has 2"):
+        ops.window_decode(q, k, v, torch.tensor([1, 2]), 4, 20, 3, 0.125)
