@@ -222,6 +222,7 @@ size_t ncn_ckpt_bytes(int64_t B, int64_t N, int64_t E, int L, int ckpt_every, in
  * Windowed attention.  Query i of row b is at position p = start_b + i, key j at position j, ctx_b = clamp(ctxlen[b], 0, Nk):
  *   query i sees key j  where  j < ctx_b,  j <= p < ctx_b  and  (p - j < window or j < n_sink)
  *   y = softmax over the visible keys of (scale q . k), times v
+ * A query that sees keys, all of whose scores are minus infinity (products that overflow), gives NaN, as the formula does.
  * A query that sees nothing (padding behind ctx_b, a position below zero) gives zeros and no gradient; what k, v, q and dy hold in such
  * places is not used, NaN included.  (Keys that one query sees and a neighbour does not may share a tile: a NaN or infinity in such a
  * key's v reaches, in the forward and backward, queries up to 256 positions from those that see it.)  ctxlen (int32 [B] on the device) null: Nk.

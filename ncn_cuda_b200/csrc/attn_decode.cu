@@ -42,7 +42,7 @@ __device__ __forceinline__ int block_start(const KeyBlocks& k, int i, int size, 
 
 // Joins what the warps of a cluster hold.  Os[kWarps][R][DP], ms (log2 units) and ls [kWarps][R] in shared memory.
 template <typename T, int R, int DP>
-__device__ __forceinline__ void join(const AttnParams& p, float* Os, float* ms, float* ls, int rows, int row0, int hk, int b) {
+__device__ __forceinline__ void join(const AttnParams& p, float* Os, float* ms, float* ls, int rows, int row0, int hk, int b, int start) {
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   __syncthreads();
@@ -81,7 +81,7 @@ __device__ __forceinline__ void join(const AttnParams& p, float* Os, float* ms, 
     }
     if (c < p.d) {
       const int row = row0 + r, h = hk * p.G + row / p.Nq, i = row % p.Nq;
-      put(static_cast<T*>(p.y) + ((long long)b * p.Nq + i) * p.H * p.d + (long long)h * p.d + c, L == 0.f ? 0.f : sum / L);
+      put(static_cast<T*>(p.y) + ((long long)b * p.Nq + i) * p.H * p.d + (long long)h * p.d + c, start + i >= 0 ? sum / L : 0.f);  // (scores that are all minus infinity: 0 / 0)
     }
   }
   cluster.sync();  // nobody leaves while its memory is read
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kWarps * 32, TILES == 1 ? 2 : 1) attn_decode_k
           *reinterpret_cast<float4*>(Os + (warp * R + r) * DP + 64 * t + 8 * g8 + 2 * e) =
               make_float4(o[u][t * 4 + e][x], o[u][t * 4 + e][2 + x], o[u][t * 4 + e + 1][x], o[u][t * 4 + e + 1][2 + x]);
     }
-  join<bf16, R, DP>(p, Os, ms, ls, rows, row0, hk, b);
+  join<bf16, R, DP>(p, Os, ms, ls, rows, row0, hk, b, g.start);
 }
 
 // fp32, and bf16 heads that the kernel above does not take.  Eight lanes per key, DP / 8 features each; a warp has four keys at a
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_decode_any_kernel(const Attn
       for (int e = 0; e < F; ++e) Os[(warp * R + r) * DP + feature(e)] = o[r][e];
     }
   }
-  join<T, R, DP>(p, Os, ms, ls, rows, row0, hk, b);
+  join<T, R, DP>(p, Os, ms, ls, rows, row0, hk, b, g.start);
 }
 
 // CTAs of a cluster: enough that the SMs have a CTA each, no more than the keys feed, blocks of `size` keys to a warp.  (64 rows of a cache

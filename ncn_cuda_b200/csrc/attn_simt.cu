@@ -190,16 +190,18 @@ __global__ void __launch_bounds__(256) attn_simt_fwd_kernel(const AttnParams p) 
   for (int i = 0; i < 4; ++i) {
     const int qi = i0 + 4 * ty + i;
     if (qi >= p.Nq) continue;
-    const float inv = l[i] > 0.f || l[i] != l[i] ? 1.f / l[i] : 0.f;
+    const int pos = g.start + qi;
+    const bool some = pos >= 0 && pos < g.ctx;  // (it sees its own place; scores that are all minus infinity leave l = 0, and NaN)
+    const float inv = 1.f / l[i];
     const long long at = ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
     T *y = static_cast<T*>(p.y) + at, *rest = sizeof(T) == 2 && p.rest ? reinterpret_cast<T*>(p.rest) + at : nullptr;
 #pragma unroll
     for (int e = 0; e < DP / 16; ++e) {
       const int c = feature_of<DP>(e);
-      if (c < p.d) put_rest(y + c, rest ? rest + c : nullptr, o[i][e] * inv);
+      if (c < p.d) put_rest(y + c, rest ? rest + c : nullptr, some ? o[i][e] * inv : 0.f);
     }
     if (p.lse && tx == 0)
-      p.lse[((long long)b * p.H + h) * p.Nqp + qi] = l[i] == 0.f ? INFINITY : m[i] * p.scale_log2 + log2f(l[i]);
+      p.lse[((long long)b * p.H + h) * p.Nqp + qi] = some ? m[i] * p.scale_log2 + log2f(l[i]) : INFINITY;
   }
 }
 

@@ -224,16 +224,18 @@ __global__ void __launch_bounds__(kCta, fwd_ctas<DP>()) attn_split_fwd_kernel(co
   for (int r = 0; r < 2; ++r) {
     const int qi = i0 + 16 * warp + g8 + 8 * r;
     if (qi >= p.Nq) continue;
-    const float inv = l[r] > 0.f || l[r] != l[r] ? 1.f / l[r] : 0.f;
+    const int pos = g.start + qi;
+    const bool some = pos >= 0 && pos < g.ctx;  // (it sees its own place; scores that are all minus infinity leave l = 0, and NaN)
+    const float inv = 1.f / l[r];
     float* y = static_cast<float*>(p.y) + ((long long)b * p.Nq + qi) * p.H * p.d + (long long)h * p.d;
 #pragma unroll
     for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int c = 8 * n + 2 * c4 + i;
-        if (c < p.d) y[c] = o[n][2 * r + i] * inv;
+        if (c < p.d) y[c] = some ? o[n][2 * r + i] * inv : 0.f;
       }
-    if (p.lse && c4 == 0) p.lse[((long long)b * p.H + h) * p.Nqp + qi] = l[r] == 0.f ? INFINITY : m[r] * p.scale_log2 + log2f(l[r]);
+    if (p.lse && c4 == 0) p.lse[((long long)b * p.H + h) * p.Nqp + qi] = some ? m[r] * p.scale_log2 + log2f(l[r]) : INFINITY;
   }
 }
 

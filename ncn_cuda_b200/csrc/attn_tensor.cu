@@ -265,11 +265,11 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 // Exponentials.  The special-function pipe gives 16 per SM and cycle, 1024 cycles per tile of 128 x 128, as long as both products of heads
 // of 128 take; so some pairs (kOnFma of 8; 2 and 3 measured best, 0 and 4 two to four per cent slower) are computed on the FMA pipe instead, two at a time: 2^x = 2^n 2^f, n the nearest whole number,
 // |f| <= 1/2, 2^f by the polynomial of degree 4 of least relative error (Remez exchange; 2.6e-6 = 2^-18.6, a thousandth of the weights'
-// rounding to bf16).  Below 2^-120 the result is 2^-120 rather than less: masks are laid over the weights, not the scores.  NaN stays NaN.
+// rounding to bf16).  From -127 down 2^n has the bits of zero, and so has the result, minus infinity's too.  NaN stays NaN.
 constexpr int kOnFma = 2;
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-120.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-120.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
   constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it leaves the nearest whole number in the low bits
   const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
   const float2 n = __fadd2_rn(t, make_float2(-kRound, -kRound));
@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
       asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
       l += *other_row;
       // (padding between rows that see a whole tile has had no mask)
-      const bool some = mine > 0 && pos >= 0 && pos < end && !(l == 0.f);
+      const bool some = mine > 0 && pos >= 0 && pos < end;  // (scores that are all minus infinity leave l = 0, and NaN)
       const float inv = some ? 1.f / l : 0.f;
       if (p.lse && half == 0 && qi < p.Nq) p.lse[((long long)b * p.H + h) * p.Nqp + qi] = some ? ref + log2f(l) : INFINITY;
       // through the place of the tile's queries, 4 KB of it to a warp (2 KB in heads of 64): the last of its products has read them (with no

@@ -85,3 +85,50 @@ def test_function_form_of_decode_agrees():
         ops.window_decode(q, k, v, torch.tensor([1.0, 2.0, 3.0]), 4, 20, 3, 0.125)
     with pytest.raises(ValueError, match="ctxlen has 2"):
         ops.window_decode(q, k, v, torch.tensor([1, 2]), 4, 20, 3, 0.125)
+
+
+# ---------------------------------------------------------------- scores of minus infinity
+BIG = 2.0**66  # BIG * -BIG overflows in 32 bits
+
+FORMS = [(BF16, 64), (BF16, 128), (BF16, 20), (BF16, 160), (F32, 64), (F32, 16), (F32, 160)]
+
+
+def overflowing(dtype, d, N, sinks):
+    """The scores of keys 0 .. sinks - 1 overflow to minus infinity for every query; their values are large."""
+    q, k, v, dy = make(d, 2, N, N, 2, 1, d, dtype)
+    q[..., ::d], k[..., 0] = BIG, 0.0
+    k[:, :sinks, 0] = -BIG
+    v[:, :sinks] = 1e35
+    return q, k, v, dy
+
+
+@pytest.mark.parametrize("dtype,d", FORMS)
+def test_scores_of_minus_infinity_weigh_nothing(dtype, d):
+    """Sinks whose scores are minus infinity: a query that sees other keys too is answered from these alone, one that sees none gets
+    what the formula gives, NaN.  (Sinks in places 0 and 1, so that past the window the answer is the one without sinks.)"""
+    N, window, sinks = 300, 60, 2
+    q, k, v, dy = overflowing(dtype, d, N, sinks)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    y = ncn.fused_window_attention(*leaves, 2, window, n_sink=sinks)
+    want = O.attention(q, k, v, 2, window, 0, 1 / math.sqrt(d), N, 0, dy)
+    far = window + sinks
+    O.close("y", y.detach()[:, far:], tuple(t[:, far:] for t in want["y"]))
+    assert y[:, :sinks].isnan().all() and y[:, sinks:].isfinite().all()
+    dq, dk, dv = torch.autograd.grad(y, leaves, dy)
+    O.close("dq", dq[:, far:], tuple(t[:, far:] for t in want["dq"]))
+    assert dq[:, :sinks].isnan().all()
+    # keys that no row of NaN sees
+    assert dk[:, sinks:].isfinite().all() and dv[:, sinks:].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype,d", FORMS)
+def test_decode_with_scores_of_minus_infinity(dtype, d):
+    N, window, sinks = 300, 60, 2
+    q, k, v, _ = overflowing(dtype, d, N, sinks)
+    one = q[:, :1]
+    y = ncn.window_attention_decode(one, k, v, torch.tensor([N, 2]), 2, window, n_sink=sinks)
+    want = O.attention(one, k, v, 2, window, 0, 1 / math.sqrt(d), N, N - 1)["y"]
+    O.close("y", y[:1], tuple(t[:1] for t in want))
+    assert y[1].isnan().all()
+    y = ncn.window_attention_decode(q[:, :2], k, v, torch.tensor([1, 0]), 2, window, n_sink=sinks)
+    assert (y[0, 0] == 0).all() and y[0, 1].isnan().all() and (y[1] == 0).all()  # a position below zero; one key; none
