@@ -223,8 +223,8 @@ size_t ncn_ckpt_bytes(int64_t B, int64_t N, int64_t E, int L, int ckpt_every, in
  *   query i sees key j  where  j < ctx_b,  j <= p < ctx_b  and  (p - j < window or j < n_sink)
  *   y = softmax over the visible keys of (scale q . k), times v
  * A query that sees keys, all of whose scores are minus infinity (products that overflow), gives NaN, as the formula does.
- * A query that sees nothing (padding behind ctx_b, a position below zero) gives zeros and no gradient; what k, v, q and dy hold in such
- * places is not used, NaN included.  (Keys that one query sees and a neighbour does not may share a tile: a NaN or infinity in such a
+ * A query that sees nothing (padding behind ctx_b, a position below zero) gives zeros and no gradient; what q and dy hold in such
+ * places, and k and v in places that no query of the row sees (behind ctx_b, behind the last query, in front of the window), is not used, NaN included.  (Keys that one query sees and a neighbour does not may share a tile: a NaN or infinity in such a
  * key's v reaches, in the forward and backward, queries up to 256 positions from those that see it.)  ctxlen (int32 [B] on the device) null: Nk.
  * q_start (int32 [B] on the device) null: start for every row.  window >= 1, n_sink >= 0, scale > 0. */
 

@@ -42,6 +42,29 @@ __device__ __forceinline__ RowGeom row_geom(const AttnParams& p, int b) {
   return g;
 }
 
+// Keys of a row that some query of the call sees: from `first` to `end`, and sinks before that.  What lies in other places (a cache behind
+// the last query, in front of the window) may be anything, NaN included: where the weights' zeros would meet it in a product it is
+// read as zero.
+struct SeenKeys {
+  int sinks, first, end;
+  __device__ __forceinline__ bool has(int key) const { return key < end && (key >= first || key < sinks); }
+  // whether one of keys k0 .. k0 + n - 1 (of Nk) is not seen
+  __device__ __forceinline__ bool lacks(int k0, int n, int Nk) const {
+    const int k1 = min(k0 + n, Nk);
+    return k1 > end || max(k0, sinks) < min(k1, first);
+  }
+};
+__device__ __forceinline__ SeenKeys seen_keys(const AttnParams& p, const RowGeom& g) {
+  return SeenKeys{p.n_sink, max(g.start, 0) - p.window + 1, min(g.ctx, g.start + p.Nq)};
+}
+// Rows of a tile that are read: [lo, hi) without [gap_lo, gap_hi)
+struct Rows {
+  int lo, hi, gap_lo, gap_hi;
+  __device__ __forceinline__ bool has(int r) const { return r >= lo && r < hi && !(r >= gap_lo && r < gap_hi); }
+};
+__device__ __forceinline__ Rows rows_between(int lo, int hi) { return Rows{lo, hi, 0, 0}; }
+__device__ __forceinline__ Rows rows_seen(const SeenKeys& s, int k0) { return Rows{0, s.end - k0, s.sinks - k0, s.first - k0}; }
+
 // A CTA's place: heads next to each other, so that a group reads its keys and values out of L2; then the tiles of a row; then rows.
 // last_first counts the tiles from the last, which see the most keys.  One-dimensional, as batches may have more rows than the
 // other two dimensions of a grid hold.

@@ -20,10 +20,10 @@ namespace {
 constexpr int kOwn = 64;
 template <int DP> constexpr int other_rows() { return DP > 128 ? 32 : 64; }
 
-// ROWS x d of `src` (row stride in elements) -> fp32 tile [ROWS][DP + 4]; rows outside [r_lo, r_hi) and features beyond d are zero.
+// ROWS x d of `src` (row stride in elements) -> fp32 tile [ROWS][DP + 4]; rows that `rows` does not have and features beyond d are zero.
 // All of a thread's loads are under way at once: one after the other they took longer than the tile's arithmetic.
 template <typename T, int DP, int ROWS>
-__device__ __forceinline__ void load_tile(float* dst, const T* src, long long stride, int r_lo, int r_hi, int d, int vec) {
+__device__ __forceinline__ void load_tile(float* dst, const T* src, long long stride, Rows rows, int d, int vec) {
   constexpr int V = 16 / sizeof(T), PER = DP / V, COUNT = ROWS * PER, EACH = (COUNT + 255) / 256;
   if (vec) {
     uint4 raw[EACH];
@@ -31,7 +31,7 @@ __device__ __forceinline__ void load_tile(float* dst, const T* src, long long st
     for (int i = 0; i < EACH; ++i) {
       const int e = threadIdx.x + 256 * i, r = e / PER, c = e % PER * V;
       raw[i] = make_uint4(0, 0, 0, 0);
-      if (e < COUNT && r >= r_lo && r < r_hi && c < d) raw[i] = *reinterpret_cast<const uint4*>(src + r * stride + c);  // (d is a multiple of V)
+      if (e < COUNT && rows.has(r) && c < d) raw[i] = *reinterpret_cast<const uint4*>(src + r * stride + c);  // (d is a multiple of V)
     }
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
@@ -44,7 +44,7 @@ __device__ __forceinline__ void load_tile(float* dst, const T* src, long long st
   } else {
     for (int e = threadIdx.x; e < ROWS * DP; e += 256) {
       const int r = e / DP, c = e % DP;
-      dst[r * (DP + 4) + c] = r >= r_lo && r < r_hi && c < d ? to_f(src[r * stride + c]) : 0.f;
+      dst[r * (DP + 4) + c] = rows.has(r) && c < d ? to_f(src[r * stride + c]) : 0.f;
     }
   }
 }
@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(256) attn_simt_fwd_kernel(const AttnParams p) 
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const RowGeom g = row_geom(p, b);
   const KeyTiles kt = key_tiles<BN>(p, g, i0, i0 + kOwn);
+  const SeenKeys seen = seen_keys(p, g);
   const T* q = static_cast<const T*>(p.q) + b * p.sq_b + i0 * p.sq_n + (long long)h * p.d;
   const T* k = static_cast<const T*>(p.k) + b * p.sk_b + (long long)hk * p.d;
   const T* v = static_cast<const T*>(p.v) + b * p.sv_b + (long long)hk * p.d;
@@ -147,12 +148,12 @@ __global__ void __launch_bounds__(256) attn_simt_fwd_kernel(const AttnParams p) 
     for (int e = 0; e < DP / 16; ++e) o[i][e] = 0.f;
   }
   const int n = kt.count();
-  if (n) load_tile<T, DP, kOwn>(Q, q, p.sq_n, 0, p.Nq - i0, p.d, p.vec);
+  if (n) load_tile<T, DP, kOwn>(Q, q, p.sq_n, rows_between(0, p.Nq - i0), p.d, p.vec);
   for (int it = 0; it < n; ++it) {
     const int k0 = kt.tile(it) * BN;
     __syncthreads();
-    load_tile<T, DP, BN>(K, k + k0 * p.sk_n, p.sk_n, 0, g.ctx - k0, p.d, p.vec);
-    load_tile<T, DP, BN>(V, v + k0 * p.sv_n, p.sv_n, 0, g.ctx - k0, p.d, p.vec);
+    load_tile<T, DP, BN>(K, k + k0 * p.sk_n, p.sk_n, rows_seen(seen, k0), p.d, p.vec);
+    load_tile<T, DP, BN>(V, v + k0 * p.sv_n, p.sv_n, rows_seen(seen, k0), p.d, p.vec);
     __syncthreads();
     float s[4][CJ] = {};
     rows_by_rows<DP, CJ>(Q, K, s);
@@ -217,13 +218,14 @@ __global__ void __launch_bounds__(256) attn_simt_dq_kernel(const AttnParams p) {
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const RowGeom g = row_geom(p, b);
   const KeyTiles kt = key_tiles<BN>(p, g, i0, i0 + kOwn);
+  const SeenKeys seen = seen_keys(p, g);
   const T* q = static_cast<const T*>(p.q) + b * p.sq_b + i0 * p.sq_n + (long long)h * p.d;
   const T* dy = static_cast<const T*>(p.dy) + b * p.sdy_b + i0 * p.sdy_n + (long long)h * p.d;
   const T* k = static_cast<const T*>(p.k) + b * p.sk_b + (long long)hk * p.d;
   const T* v = static_cast<const T*>(p.v) + b * p.sv_b + (long long)hk * p.d;
   const int r_lo = max(0, -(g.start + i0)), r_hi = min(p.Nq, g.ctx - g.start) - i0;  // rows that are not padding
-  load_tile<T, DP, kOwn>(Q, q, p.sq_n, r_lo, r_hi, p.d, p.vec);
-  load_tile<T, DP, kOwn>(dO, dy, p.sdy_n, r_lo, r_hi, p.d, p.vec);
+  load_tile<T, DP, kOwn>(Q, q, p.sq_n, rows_between(r_lo, r_hi), p.d, p.vec);
+  load_tile<T, DP, kOwn>(dO, dy, p.sdy_n, rows_between(r_lo, r_hi), p.d, p.vec);
   __syncthreads();
   float acc[4][DP / 16] = {}, lse[4], delta[4];
 #pragma unroll
@@ -248,8 +250,8 @@ __global__ void __launch_bounds__(256) attn_simt_dq_kernel(const AttnParams p) {
   for (int it = 0; it < n; ++it) {
     const int k0 = kt.tile(it) * BN;
     __syncthreads();
-    load_tile<T, DP, BN>(K, k + k0 * p.sk_n, p.sk_n, 0, g.ctx - k0, p.d, p.vec);
-    load_tile<T, DP, BN>(V, v + k0 * p.sv_n, p.sv_n, 0, g.ctx - k0, p.d, p.vec);
+    load_tile<T, DP, BN>(K, k + k0 * p.sk_n, p.sk_n, rows_seen(seen, k0), p.d, p.vec);
+    load_tile<T, DP, BN>(V, v + k0 * p.sv_n, p.sv_n, rows_seen(seen, k0), p.d, p.vec);
     __syncthreads();
     float s[4][CJ] = {}, dp[4][CJ] = {};
     rows_by_rows<DP, CJ>(Q, K, s);
@@ -293,20 +295,20 @@ __global__ void __launch_bounds__(256) attn_simt_dkv_kernel(const AttnParams p) 
   const int hk = at_block.head, b = at_block.b, ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const RowGeom g = row_geom(p, b);
   const KeyItem it = key_item<kOwn, BN>(p, g, at_block.first_last);
-  const int k0 = it.tile * kOwn;
+  const int k0 = it.tile * kOwn, end = min(g.ctx, g.start + p.Nq);  // (of the queries: the last tile's rows behind them see nothing)
   const T* k = static_cast<const T*>(p.k) + b * p.sk_b + k0 * p.sk_n + (long long)hk * p.d;
   const T* v = static_cast<const T*>(p.v) + b * p.sv_b + k0 * p.sv_n + (long long)hk * p.d;
   float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
   if (it.begin < it.end) {
-    load_tile<T, DP, kOwn>(K, k, p.sk_n, 0, g.ctx - k0, p.d, p.vec);
-    load_tile<T, DP, kOwn>(V, v, p.sv_n, 0, g.ctx - k0, p.d, p.vec);
+    load_tile<T, DP, kOwn>(K, k, p.sk_n, rows_between(0, g.ctx - k0), p.d, p.vec);
+    load_tile<T, DP, kOwn>(V, v, p.sv_n, rows_between(0, g.ctx - k0), p.d, p.vec);
   }
   for (int e = it.begin; e < it.end; ++e) {
     const int h = hk * p.G + e / it.tiles, i0 = (it.first + e % it.tiles) * BN;
     const int r_lo = max(0, -(g.start + i0)), r_hi = min(p.Nq, g.ctx - g.start) - i0;
     __syncthreads();
-    load_tile<T, DP, BN>(Q, static_cast<const T*>(p.q) + b * p.sq_b + i0 * p.sq_n + (long long)h * p.d, p.sq_n, r_lo, r_hi, p.d, p.vec);
-    load_tile<T, DP, BN>(dO, static_cast<const T*>(p.dy) + b * p.sdy_b + i0 * p.sdy_n + (long long)h * p.d, p.sdy_n, r_lo, r_hi, p.d, p.vec);
+    load_tile<T, DP, BN>(Q, static_cast<const T*>(p.q) + b * p.sq_b + i0 * p.sq_n + (long long)h * p.d, p.sq_n, rows_between(r_lo, r_hi), p.d, p.vec);
+    load_tile<T, DP, BN>(dO, static_cast<const T*>(p.dy) + b * p.sdy_b + i0 * p.sdy_n + (long long)h * p.d, p.sdy_n, rows_between(r_lo, r_hi), p.d, p.vec);
     if (threadIdx.x < BN) {
       const int r = threadIdx.x;
       const long long at = ((long long)b * p.H + h) * p.Nqp + i0 + r;
@@ -326,7 +328,7 @@ __global__ void __launch_bounds__(256) attn_simt_dkv_kernel(const AttnParams p) 
       for (int j = 0; j < CJ; ++j) {
         const int c = tx + 16 * j;
         float w = ex2(fmaf(s[i][j], p.scale_log2, -lse_s[c])), t = w * (dp[i][j] - del_s[c]);
-        if (!all && !sees(p, g.ctx, g.start + i0 + c, key)) w = t = 0.f;
+        if (!all && !sees(p, end, g.start + i0 + c, key)) w = t = 0.f;
         P[(4 * ty + i) * (BN + 4) + c] = w;
         S[(4 * ty + i) * (BN + 4) + c] = t;
       }

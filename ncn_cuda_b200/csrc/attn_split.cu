@@ -46,23 +46,23 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// ROWS x d of `src` -> tile [ROWS][DP + 4], asynchronously where rows may be read 16 bytes at a time; rows outside [r_lo, r_hi) and
-// features beyond d are zero.
+// ROWS x d of `src` -> tile [ROWS][DP + 4], asynchronously where rows may be read 16 bytes at a time; rows that `rows` does not
+// have and features beyond d are zero.
 template <int DP, int ROWS>
-__device__ __forceinline__ void send_for(float* dst, const float* src, long long stride, int r_lo, int r_hi, int d, int vec) {
+__device__ __forceinline__ void send_for(float* dst, const float* src, long long stride, Rows rows, int d, int vec) {
   constexpr int PER = DP / 4;
   if (vec) {
 #pragma unroll 4
     for (int e = threadIdx.x; e < ROWS * PER; e += kCta) {
       const int r = e / PER, c = e % PER * 4;
-      const bool ok = r >= r_lo && r < r_hi && c < d;
+      const bool ok = rows.has(r) && c < d;
       const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst + r * (DP + 4) + c);
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(ok ? src + r * stride + c : src), "r"(ok ? 16 : 0) : "memory");
     }
   } else {
     for (int e = threadIdx.x; e < ROWS * DP; e += kCta) {
       const int r = e / DP, c = e % DP;
-      dst[r * (DP + 4) + c] = r >= r_lo && r < r_hi && c < d ? src[r * stride + c] : 0.f;
+      dst[r * (DP + 4) + c] = rows.has(r) && c < d ? src[r * stride + c] : 0.f;
     }
   }
 }
@@ -156,23 +156,24 @@ __global__ void __launch_bounds__(kCta, fwd_ctas<DP>()) attn_split_fwd_kernel(co
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g8 = lane / 4, c4 = lane % 4;
   const RowGeom g = row_geom(p, b);
   const KeyTiles kt = key_tiles<BN>(p, g, i0, i0 + kOwn);
+  const SeenKeys seen = seen_keys(p, g);
   const float* q = static_cast<const float*>(p.q) + b * p.sq_b + i0 * p.sq_n + (long long)h * p.d;
   const float* k = static_cast<const float*>(p.k) + b * p.sk_b + (long long)hk * p.d;
   const float* v = static_cast<const float*>(p.v) + b * p.sv_b + (long long)hk * p.d;
   auto send_keys = [&](int it) {
     const int k0 = kt.tile(it) * BN;
-    send_for<DP, BN>(K, k + k0 * p.sk_n, p.sk_n, 0, g.ctx - k0, p.d, p.vec);
+    send_for<DP, BN>(K, k + k0 * p.sk_n, p.sk_n, rows_seen(seen, k0), p.d, p.vec);
   };
   auto send_values = [&](int it) {
     const int k0 = kt.tile(it) * BN;
-    send_for<DP, BN>(V, v + k0 * p.sv_n, p.sv_n, 0, g.ctx - k0, p.d, p.vec);
+    send_for<DP, BN>(V, v + k0 * p.sv_n, p.sv_n, rows_seen(seen, k0), p.d, p.vec);
   };
   float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
   const int n_tiles = kt.count();
   if (n_tiles) {
-    send_for<DP, kOwn>(Q, q, p.sq_n, 0, p.Nq - i0, p.d, p.vec);
+    send_for<DP, kOwn>(Q, q, p.sq_n, rows_between(0, p.Nq - i0), p.d, p.vec);
     send_keys(0);
     sent();
     send_values(0);
@@ -251,6 +252,7 @@ __global__ void __launch_bounds__(kCta, bwd_ctas<DP>()) attn_split_dq_kernel(con
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g8 = lane / 4, c4 = lane % 4, row0 = 16 * warp;
   const RowGeom g = row_geom(p, b);
   const KeyTiles kt = key_tiles<BN>(p, g, i0, i0 + kOwn);
+  const SeenKeys seen = seen_keys(p, g);
   const float* q = static_cast<const float*>(p.q) + b * p.sq_b + i0 * p.sq_n + (long long)h * p.d;
   const float* dy = static_cast<const float*>(p.dy) + b * p.sdy_b + i0 * p.sdy_n + (long long)h * p.d;
   const float* k = static_cast<const float*>(p.k) + b * p.sk_b + (long long)hk * p.d;
@@ -258,15 +260,15 @@ __global__ void __launch_bounds__(kCta, bwd_ctas<DP>()) attn_split_dq_kernel(con
   const int r_lo = max(0, -(g.start + i0)), r_hi = min(p.Nq, g.ctx - g.start) - i0;  // rows that are not padding
   auto send_keys = [&](int it) {
     const int k0 = kt.tile(it) * BN;
-    send_for<DP, BN>(K, k + k0 * p.sk_n, p.sk_n, 0, g.ctx - k0, p.d, p.vec);
+    send_for<DP, BN>(K, k + k0 * p.sk_n, p.sk_n, rows_seen(seen, k0), p.d, p.vec);
   };
   auto send_values = [&](int it) {
     const int k0 = kt.tile(it) * BN;
-    send_for<DP, BN>(V, v + k0 * p.sv_n, p.sv_n, 0, g.ctx - k0, p.d, p.vec);
+    send_for<DP, BN>(V, v + k0 * p.sv_n, p.sv_n, rows_seen(seen, k0), p.d, p.vec);
   };
   const int n_tiles = kt.count();
-  send_for<DP, kOwn>(dO, dy, p.sdy_n, r_lo, r_hi, p.d, p.vec);
-  send_for<DP, kOwn>(Q, q, p.sq_n, r_lo, r_hi, p.d, p.vec);
+  send_for<DP, kOwn>(dO, dy, p.sdy_n, rows_between(r_lo, r_hi), p.d, p.vec);
+  send_for<DP, kOwn>(Q, q, p.sq_n, rows_between(r_lo, r_hi), p.d, p.vec);
   if (n_tiles) send_values(0);
   sent();
   if (n_tiles) send_keys(0);
@@ -341,7 +343,7 @@ __global__ void __launch_bounds__(kCta, bwd_ctas<DP>()) attn_split_dkv_kernel(co
   const int hk = at_block.head, b = at_block.b, lane = threadIdx.x % 32, warp = threadIdx.x / 32, g8 = lane / 4, c4 = lane % 4, row0 = 16 * warp;
   const RowGeom g = row_geom(p, b);
   const KeyItem it = key_item<kOwn, BN>(p, g, at_block.first_last);
-  const int k0 = it.tile * kOwn;
+  const int k0 = it.tile * kOwn, end = min(g.ctx, g.start + p.Nq);  // (of the queries: the last tile's rows behind them see nothing)
   const float* k = static_cast<const float*>(p.k) + b * p.sk_b + k0 * p.sk_n + (long long)hk * p.d;
   const float* v = static_cast<const float*>(p.v) + b * p.sv_b + k0 * p.sv_n + (long long)hk * p.d;
   auto place = [&](int e, int& h, int& i0, int& r_lo, int& r_hi) {
@@ -351,12 +353,12 @@ __global__ void __launch_bounds__(kCta, bwd_ctas<DP>()) attn_split_dkv_kernel(co
   auto send_queries = [&](int e) {
     int h, i0, r_lo, r_hi;
     place(e, h, i0, r_lo, r_hi);
-    send_for<DP, BN>(Q, static_cast<const float*>(p.q) + b * p.sq_b + i0 * p.sq_n + (long long)h * p.d, p.sq_n, r_lo, r_hi, p.d, p.vec);
+    send_for<DP, BN>(Q, static_cast<const float*>(p.q) + b * p.sq_b + i0 * p.sq_n + (long long)h * p.d, p.sq_n, rows_between(r_lo, r_hi), p.d, p.vec);
   };
   auto send_cotangents = [&](int e, int buffer) {  // and what belongs to their rows
     int h, i0, r_lo, r_hi;
     place(e, h, i0, r_lo, r_hi);
-    send_for<DP, BN>(dO, static_cast<const float*>(p.dy) + b * p.sdy_b + i0 * p.sdy_n + (long long)h * p.d, p.sdy_n, r_lo, r_hi, p.d, p.vec);
+    send_for<DP, BN>(dO, static_cast<const float*>(p.dy) + b * p.sdy_b + i0 * p.sdy_n + (long long)h * p.d, p.sdy_n, rows_between(r_lo, r_hi), p.d, p.vec);
     if (threadIdx.x < BN) {
       const int r = threadIdx.x;
       const long long at = ((long long)b * p.H + h) * p.Nqp + i0 + r;
@@ -371,8 +373,8 @@ __global__ void __launch_bounds__(kCta, bwd_ctas<DP>()) attn_split_dkv_kernel(co
 #pragma unroll
     for (int i = 0; i < 4; ++i) dk[n][i] = dv[n][i] = 0.f;
   if (it.begin < it.end) {
-    send_for<DP, kOwn>(K, k, p.sk_n, 0, g.ctx - k0, p.d, p.vec);
-    send_for<DP, kOwn>(V, v, p.sv_n, 0, g.ctx - k0, p.d, p.vec);
+    send_for<DP, kOwn>(K, k, p.sk_n, rows_between(0, g.ctx - k0), p.d, p.vec);
+    send_for<DP, kOwn>(V, v, p.sv_n, rows_between(0, g.ctx - k0), p.d, p.vec);
     send_cotangents(it.begin, it.begin & 1);
     sent();
     send_queries(it.begin);
@@ -395,7 +397,7 @@ __global__ void __launch_bounds__(kCta, bwd_ctas<DP>()) attn_split_dkv_kernel(co
       for (int i = 0; i < 4; ++i) {
         const int c = 8 * n + 2 * c4 + (i & 1);
         float w = ex2(fmaf(s[n][i], p.scale_log2, -lse[c])), t = w * (dp[n][i] - delta[c]);
-        if (!all && !sees(p, g.ctx, g.start + i0 + c, key + (i >> 1) * 8)) w = t = 0.f;
+        if (!all && !sees(p, end, g.start + i0 + c, key + (i >> 1) * 8)) w = t = 0.f;
         s[n][i] = w, dp[n][i] = t;
       }
     add_rows_by_cols<DP, NB>(s, dO, 1.f, 1.f, dv);

@@ -7,8 +7,8 @@
 // TMA unit; the same tile serves as an operand along its features (scores) and along its positions (second products).
 // Heads whose size is not 64 or 128 are filled up with zeros by the TMA unit.
 //
-// Rows of padding (behind ctxlen) may hold anything, NaN included: scores are masked by selection, and the rows that a second
-// product would multiply by zero weights are cleared in shared memory first.
+// Rows of padding (behind ctxlen) and places that no query of the call sees may hold anything, NaN included: scores are masked by
+// selection, and the rows that a second product would multiply by zero weights are cleared in shared memory first.
 //
 // The backward is two kernels, one that owns queries and one that owns keys.  It computes the scores twice, 7 products for 5, and in
 // return no sum depends on the order in which CTAs finish.
@@ -236,14 +236,14 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
 #pragma unroll
   for (int c = 0; c < DP / 64; ++c) tma_load(dst + c * kBlockBytes, map, c * 64, head, row, b, bar);
 }
-// Clears the rows outside [lo, hi) of a tile; a whole warp.  The thread that issues the products has seen the tile arrive, asks for it
+// Clears the rows of a tile that `keep` does not name; a whole warp.  The thread that issues the products has seen the tile arrive, asks for it
 // (`go`) and waits (`cleared`) before it goes on: one tile at a time, so neither can be a phase ahead.
-template <int DP>
-__device__ __forceinline__ void clear_rows(uint32_t tile, int lo, int hi, uint64_t* cleared) {
+template <int DP, typename Keep>
+__device__ __forceinline__ void clear_rows(uint32_t tile, Keep keep, uint64_t* cleared) {
   const int lane = threadIdx.x % 32;
   for (int e = lane; e < kT * DP / 8; e += 32) {
     const int r = e % (kT * 8) / 8;
-    if (r < lo || r >= hi)
+    if (!keep(r))
       asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + e / (kT * 8) * kBlockBytes + e % (kT * 8) * 16), "r"(0) : "memory");
   }
   fence_proxy_async();
@@ -427,8 +427,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
   const RowGeom g = row_geom(p, b);
   const KeyTiles all = key_tiles<kT>(p, g, i0, first_of(1) + kT);
   const int n = all.count();
-  // the last tile may end in padding, whose values would meet weights of zero
-  const bool clear = n > 0 && g.ctx < p.Nk && all.tile(n - 1) * kT + kT > g.ctx;
+  // tiles with places that nobody sees (the last one may end in padding), whose values would meet weights of zero
+  const SeenKeys seen = seen_keys(p, g);
+  auto unseen = [&](int j) { return seen.lacks(all.tile(j) * kT, kT, p.Nk); };
   const int at_once = min(2 * n, SLOTS);
   auto load = [&](int i) {
     const auto to = ring.place(i);
@@ -464,7 +465,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
     }
     __syncwarp();
   } else if (warp == 18) {
-    if (clear && wait(go, 0)) clear_rows<DP>(ring.at(ring.place(2 * n - 1)), 0, g.ctx - all.tile(n - 1) * kT, cleared);
+    uint32_t clears = 0;
+    for (int j = 0; j < n; ++j) {
+      if (!unseen(j)) continue;
+      if (!wait(go, clears++ & 1)) break;
+      const int k0 = all.tile(j) * kT;
+      clear_rows<DP>(ring.at(ring.place(2 * j + 1)), [&](int r) { return seen.has(k0 + r); }, cleared);
+    }
   } else if (warp == 16) {
     if (n > 0 && elect_one()) {
       // what tile x needs of the list: entries below ns, and lo .. hi
@@ -476,7 +483,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
         hi[x] = kt.t1 >= kt.t0 ? all.entry(kt.t1) : -1;
         last[x] = max(ns[x] - 1, hi[x]);
       }
-      uint32_t phase[2] = {0, 0};
+      uint32_t phase[2] = {0, 0}, clears = 0;
       bool begun[2] = {false, false};
       typename Ring<SLOTS>::Place k_at, v_at;
       v_at.next();
@@ -495,7 +502,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_tensor_fwd_kernel(const _
       }
 #pragma unroll 1
       for (int j = 0; ok && j < n; ++j) {
-        ok = ring.wait_full(wait, v_at) && (j + 1 < n ? ring.wait_full(wait, k_at) : !clear || have_cleared(wait, go, cleared, 0));
+        ok = ring.wait_full(wait, v_at) && (!unseen(j) || have_cleared(wait, go, cleared, clears++ & 1)) && (j + 1 >= n || ring.wait_full(wait, k_at));
         if (!ok) break;
         const uint32_t vs = ring.at(v_at);
 #pragma unroll
@@ -710,8 +717,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
   const KeyTiles kt = key_tiles<kT>(p, g, i0, i0 + kT);
   const int n = kt.count();
 
-  // the last tile may end in padding: keys that would meet a dS of zero
-  const bool clear = n > 0 && g.ctx < p.Nk && kt.tile(n - 1) * kT + kT > g.ctx;
+  // tiles with places that nobody sees: keys that would meet a dS of zero
+  const SeenKeys seen = seen_keys(p, g);
+  auto unseen = [&](int j) { return seen.lacks(kt.tile(j) * kT, kT, p.Nk); };
   // (as in the forward: the first tiles are sent for before the warps meet)
   const int at_once = min(2 * n + 2, SLOTS);
   auto load = [&](int i) {  // y and its rest, for delta, in the ring's first places; then keys and values
@@ -751,13 +759,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dq_kernel(const __gri
     }
     __syncwarp();
   } else if (warp == 10) {
-    if (clear && wait(go, 0)) clear_rows<DP>(ring.at(ring.place(2 * n)), 0, g.ctx - kt.tile(n - 1) * kT, cleared);
+    uint32_t clears = 0;
+    for (int j = 0; j < n; ++j) {
+      if (!unseen(j)) continue;
+      if (!wait(go, clears++ & 1)) break;
+      const int k0 = kt.tile(j) * kT;
+      clear_rows<DP>(ring.at(ring.place(2 * j + 2)), [&](int r) { return seen.has(k0 + r); }, cleared);
+    }
   } else if (warp == 8) {
     if (n > 0 && elect_one()) {
       typename Ring<SLOTS>::Place k_at, v_at, old_k;  // of the next scores, the next dP, the next dS
       k_at = old_k = ring.place(2), v_at = ring.place(3);
+      uint32_t clears = 0;
       auto scores = [&](int j) {  // of tile j into buffer j % 2
-        if (!(ring.wait_full(wait, k_at) && (j + 1 < n || !clear || have_cleared(wait, go, cleared, 0)))) return false;
+        if (!(ring.wait_full(wait, k_at) && (!unseen(j) || have_cleared(wait, go, cleared, clears++ & 1)))) return false;
         product_scores<DP>(tmem + (j & 1) * kT, qs, ring.at(k_at));
         mma_commit(s_full + (j & 1));
         k_at.next(), k_at.next();
@@ -1014,7 +1029,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tensor_dkv_kernel(const __gr
       if (padded(entry)) {
         if (!wait(go, clears++ & 1)) break;
         const int first = g.start + entry.row();
-        clear_rows<DP>(ring.at(ring.place(i)), -first, g.ctx - first, cleared);
+        clear_rows<DP>(ring.at(ring.place(i)), [&](int r) { return first + r >= 0 && first + r < g.ctx; }, cleared);
       }
       if (i & 1) entry.next();
     }

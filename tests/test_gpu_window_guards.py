@@ -132,3 +132,34 @@ def test_decode_with_scores_of_minus_infinity(dtype, d):
     assert y[1].isnan().all()
     y = ncn.window_attention_decode(q[:, :2], k, v, torch.tensor([1, 0]), 2, window, n_sink=sinks)
     assert (y[0, 0] == 0).all() and y[0, 1].isnan().all() and (y[1] == 0).all()  # a position below zero; one key; none
+
+
+# ---------------------------------------------------------------- places that no query of the call sees
+@pytest.mark.parametrize("dtype,d", FORMS + [(F32, 128)])
+@pytest.mark.parametrize("Nq,Nk,lo,window,sinks", [
+    (40, 700, 300, 90, 3),      # before the window, between it and the sinks, behind the last query
+    (1, 300, 299, 7, 1), (130, 700, 520, 300, 0), (5, 64, 20, 10, 4), (200, 900, 600, 128, 130), (129, 1000, 700, 1, 257), (3, 400, 140, 200, 300),
+])
+def test_unseen_places_hold_anything(dtype, d, Nq, Nk, lo, window, sinks):
+    q, k, v, dy = make(Nk + d, 3, Nq, Nk, 4, 2, d, dtype)
+    starts = torch.tensor([lo, max(lo - 37, 0), 0], device="cuda")
+    ctxlen = torch.tensor([Nk, Nk, min(Nk, Nq + 2)], device="cuda")
+    see = O.visible(3, Nq, Nk, window, sinks, ctxlen, starts, "cuda").any(-2)[:, 0]
+    assert not see.all()
+    k[~see], v[~see] = math.nan, math.inf
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    y = ncn.fused_window_attention(*leaves, 4, window, n_sink=sinks, ctxlen=ctxlen, q_start=starts)
+    grads = torch.autograd.grad(y, leaves, dy)
+    torch.cuda.synchronize()
+    ops.device_status()
+    want = O.attention(q, k, v, 4, window, sinks, 1 / math.sqrt(d), ctxlen, starts, dy)
+    O.close("y", y.detach(), want["y"])
+    for name, g in zip(("dq", "dk", "dv"), grads):
+        O.close(name, g, want[name])
+    assert (grads[1][~see] == 0).all() and (grads[2][~see] == 0).all()
+    # one start for all rows, no lengths
+    see = O.visible(3, Nq, Nk, window, sinks, Nk, lo, "cuda").any(-2)[:, 0]
+    k, v = torch.randn_like(k), torch.randn_like(v)
+    k[~see], v[~see] = -math.inf, math.nan
+    y = ncn.fused_window_attention(q, k, v, 4, window, n_sink=sinks, q_start=lo)
+    O.close("y", y, O.attention(q, k, v, 4, window, sinks, 1 / math.sqrt(d), Nk, lo)["y"])
