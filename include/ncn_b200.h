@@ -40,7 +40,7 @@ enum {
   NCN_OK = 0,
   NCN_ERR_SHAPE = 1,       /* n_cache does not divide N, n_head does not divide E, sizes <= 0 */
   NCN_ERR_DTYPE = 2,       /* dtype is neither NCN_F32 nor NCN_BF16 */
-  NCN_ERR_ALIGN = 3,       /* a tensor pointer is not 16-byte aligned (fused path only) */
+  NCN_ERR_ALIGN = 3,       /* a tensor pointer (fused path), a state or workspace (windowed attention) is not 16-byte aligned */
   NCN_ERR_SMEM = 4,        /* the tile does not fit the shared memory of one SM */
   NCN_ERR_UNSUPPORTED = 5, /* the fused all-stage path does not cover these arguments; use the per-stage calls */
   NCN_ERR_WORKSPACE = 6,   /* workspace missing or smaller than ncn_bwd_workspace_bytes() */

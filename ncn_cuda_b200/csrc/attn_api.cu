@@ -106,6 +106,7 @@ int ncn_window_fwd(const void* q, const void* k, const void* v, void* y, void* s
   int rc = attn_params(p, q, k, v, ctxlen, q_start, strides, 6, B, Nq, Nk, E, Ek, n_head, window, n_sink, start, scale, dtype);
   if (rc != NCN_OK || B == 0 || Nq == 0) return rc;
   if (!y) return NCN_ERR_NULL;
+  if (!aligned16(state)) return NCN_ERR_ALIGN;
   if (!grid_ok(p)) return NCN_ERR_TOO_LARGE;
   DevInfo dev;
   if ((rc = get_dev(dev)) != NCN_OK) return rc;
@@ -139,6 +140,7 @@ int ncn_window_bwd(const void* q, const void* k, const void* v, const void* y, c
   int rc = attn_params(p, q, k, v, ctxlen, q_start, strides, 8, B, Nq, Nk, E, Ek, n_head, window, n_sink, start, scale, dtype);
   if (rc != NCN_OK || B == 0 || Nq == 0) return rc;
   if (!y || !dy || !state || !dq || ((!dk || !dv) && Nk > 0)) return NCN_ERR_NULL;
+  if (!aligned16(state) || !aligned16(workspace)) return NCN_ERR_ALIGN;  // (read by bulk copies and 16 bytes at a time)
   if (!grid_ok(p)) return NCN_ERR_TOO_LARGE;
   DevInfo dev;
   if ((rc = get_dev(dev)) != NCN_OK) return rc;

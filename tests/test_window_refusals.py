@@ -43,6 +43,14 @@ def test_backward_refuses(status, args):
     assert bwd(**args) == status
 
 
+@pytest.mark.parametrize("off", [1, 4, 8])
+def test_states_and_workspaces_off_the_boundary(off):
+    """What bulk copies and 16-byte accesses read has to lie on 16 bytes: a status, not a fault."""
+    ALIGN = 3
+    assert bwd(ws=P + off) == ALIGN and bwd(state=P + off) == ALIGN
+    assert _lib.load().ncn_window_fwd(P, P, P, P, P + off, None, None, None, 1, 8, 8, 64, 64, 2, 4, 0, 0, 1.0, 0, None) == ALIGN
+
+
 def test_decode_refuses():
     assert decode(ctxlen=None) == NULL
     assert decode(H=5) == SHAPE
