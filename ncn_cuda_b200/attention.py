@@ -269,23 +269,28 @@ class NCNWindowAttention(nn.Module):
         q, k, v = self._rotated(x, None)
         return self.out(fused_window_attention(q, k, v, self.n_head, self.window, n_sink=self.n_sink, ctxlen=ctxlen))
 
-    def new_cache(self, B: int, length: int):
-        """Keys and values of B rows of up to `length` positions, in the weights' type.  (The place behind them takes what has none.)"""
+    def new_cache(self, B: int, length: int, dtype: Optional[torch.dtype] = None):
+        """Keys and values of B rows of up to `length` positions, in `dtype`: unless given, autocast's where it is on, else the weights'.
+        (The place behind them takes what has none.)"""
         w = self.qkv.weight
+        if dtype is None:
+            dtype = torch.get_autocast_dtype(w.device.type) if torch.is_autocast_enabled(w.device.type) else w.dtype
         width = self.n_kv_head * (self.embed_dim // self.n_head)
-        return tuple(torch.zeros(B, length + 1, width, dtype=w.dtype, device=w.device) for _ in range(2))
+        return tuple(torch.zeros(B, length + 1, width, dtype=dtype, device=w.device) for _ in range(2))
 
     @torch.no_grad()
     def step(self, x, cache, ctxlen):
         """The next positions of each row: x [B, n, embed_dim], ctxlen int tensor [B], the rows' lengths with these n counted.  Enters their
-        keys and values into the cache and returns [B, n, embed_dim].  Rows shorter than n are padded in front: what stands there is not
-        entered and gives out(0).  Positions beyond the cache's length are lost: make it long enough."""
+        keys and values into the cache, in whose type the attention is computed, and returns [B, n, embed_dim].  Rows shorter than n are
+        padded in front: what stands there is not entered and gives out(0).  Positions beyond the cache's length are lost: make it long enough."""
         k_cache, v_cache = cache
         B, n, _ = x.shape
         length = k_cache.shape[1] - 1
         ctxlen = torch.as_tensor(ctxlen).to(device=x.device, dtype=torch.int64)
         positions = ctxlen[:, None] - n + torch.arange(n, device=x.device)
         q, k, v = self._rotated(x, positions)
+        dtype = q.dtype
+        q, k, v = (t.to(k_cache.dtype) for t in (q, k, v))
         place = torch.where((positions < 0) | (positions >= length), length, positions)
         rows = torch.arange(B, device=x.device)[:, None]
         k_cache[rows, place] = k
@@ -295,4 +300,4 @@ class NCNWindowAttention(nn.Module):
             y = window_attention_decode(q, k_cache, v_cache, ctxlen, self.n_head, self.window, n_sink=self.n_sink)
         else:
             y = fused_window_attention(q, k_cache, v_cache, self.n_head, self.window, n_sink=self.n_sink, ctxlen=ctxlen, q_start=ctxlen - n)
-        return self.out(y)
+        return self.out(y.to(dtype))

@@ -163,3 +163,24 @@ def test_unseen_places_hold_anything(dtype, d, Nq, Nk, lo, window, sinks):
     k[~see], v[~see] = -math.inf, math.nan
     y = ncn.fused_window_attention(q, k, v, 4, window, n_sink=sinks, q_start=lo)
     O.close("y", y, O.attention(q, k, v, 4, window, sinks, 1 / math.sqrt(d), Nk, lo)["y"])
+
+
+# ---------------------------------------------------------------- the layer
+@pytest.mark.parametrize("dtype", ["default", F32, BF16])
+def test_layer_under_autocast(dtype):
+    """fp32 weights, bf16 arithmetic: forward, and step by step over a cache of either type."""
+    torch.manual_seed(4)
+    B, N, E, H = 2, 50, 128, 2
+    layer = ncn.NCNWindowAttention(E, H, 20, n_sink=2, n_kv_head=1).cuda()
+    x = torch.randn(B, N, E, device="cuda")
+    with torch.autocast("cuda", torch.bfloat16), torch.no_grad():
+        y = layer(x)
+        cache = layer.new_cache(B, N) if dtype == "default" else layer.new_cache(B, N, dtype=dtype)
+        assert cache[0].dtype == (BF16 if dtype == "default" else dtype)
+        got = [layer.step(x[:, :20], cache, torch.full((B,), 20))]
+        got += [layer.step(x[:, n : n + 1], cache, torch.full((B,), n + 1)) for n in range(20, N)]
+    assert y.dtype == BF16 and all(t.dtype == BF16 for t in got)
+    # roundings of the projection, the rotated heads, the inner result and the last one, on both sides: 8 * 2^-8 of the largest
+    assert (torch.cat(got, 1) - y).abs().max() <= 8 * 2.0**-8 * y.abs().max()
+    assert layer.new_cache(B, N)[0].dtype == F32  # (without autocast: the weights' type)
+    assert layer.new_cache(B, N, dtype=BF16)[1].dtype == BF16

@@ -140,3 +140,12 @@ def test_layer_arguments():
         layer = ncn.NCNWindowAttention(64, 4, 8)
     assert layer.qkv.weight.is_meta and layer.freqs.device.type == "cpu"
     assert layer.to_empty(device="cpu").freqs.dtype == torch.float64
+
+
+def test_types_of_a_cache():
+    layer = ncn.NCNWindowAttention(64, 4, 8, n_kv_head=2)
+    assert [t.dtype for t in layer.new_cache(2, 5)] == [torch.float32] * 2 and layer.new_cache(2, 5)[0].shape == (2, 6, 32)
+    assert [t.dtype for t in layer.new_cache(2, 5, dtype=torch.bfloat16)] == [torch.bfloat16] * 2
+    with torch.autocast("cpu", torch.bfloat16):
+        assert [t.dtype for t in layer.new_cache(2, 5)] == [torch.bfloat16] * 2
+        assert layer.new_cache(2, 5, dtype=torch.float32)[0].dtype == torch.float32
