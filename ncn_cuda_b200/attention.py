@@ -282,7 +282,7 @@ class NCNWindowAttention(nn.Module):
     def step(self, x, cache, ctxlen):
         """The next positions of each row: x [B, n, embed_dim], ctxlen int tensor [B], the rows' lengths with these n counted.  Enters their
         keys and values into the cache, in whose type the attention is computed, and returns [B, n, embed_dim].  Rows shorter than n are
-        padded in front: what stands there is not entered and gives out(0).  Positions beyond the cache's length are lost: make it long enough."""
+        padded in front: what stands there is not entered and gives out(0).  So do positions beyond the cache's length, which are lost: make it long enough."""
         k_cache, v_cache = cache
         B, n, _ = x.shape
         length = k_cache.shape[1] - 1
@@ -296,7 +296,8 @@ class NCNWindowAttention(nn.Module):
         k_cache[rows, place] = k
         v_cache[rows, place] = v
         k_cache, v_cache = k_cache[:, :length], v_cache[:, :length]
-        if n == 1:
+        if n == 1:  # (a row whose position has no place sees nothing, as in the other form)
+            ctxlen = torch.where(ctxlen > length, 0, ctxlen)
             y = window_attention_decode(q, k_cache, v_cache, ctxlen, self.n_head, self.window, n_sink=self.n_sink)
         else:
             y = fused_window_attention(q, k_cache, v_cache, self.n_head, self.window, n_sink=self.n_sink, ctxlen=ctxlen, q_start=ctxlen - n)

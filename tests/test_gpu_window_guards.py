@@ -184,3 +184,20 @@ def test_layer_under_autocast(dtype):
     assert (torch.cat(got, 1) - y).abs().max() <= 8 * 2.0**-8 * y.abs().max()
     assert layer.new_cache(B, N)[0].dtype == F32  # (without autocast: the weights' type)
     assert layer.new_cache(B, N, dtype=BF16)[1].dtype == BF16
+
+
+def test_layer_beyond_its_cache():
+    """A position that has no place in the cache is lost, and gives out(0), whether it comes alone or with others."""
+    torch.manual_seed(5)
+    layer = ncn.NCNWindowAttention(64, 2, 20).cuda()
+    x = torch.randn(2, 10, 64, device="cuda")
+    cache = layer.new_cache(2, 8)
+    y = layer(x)
+    first = layer.step(x[:, :6], cache, torch.tensor([6, 6]))
+    two = layer.step(x[:, 6:8], cache, torch.tensor([8, 8]))
+    assert (torch.cat([first, two], 1) - y[:, :8]).abs().max() <= 1e-5 * y.abs().max() + 6 * 64 * 2.0**-24 * y.abs().max()
+    kept = [t[:, :8].clone() for t in cache]
+    for n in (1, 2):
+        got = layer.step(x[:, 8 : 8 + n], cache, torch.tensor([8 + n, 8 + n]))
+        assert (got == 0).all(), n
+    assert all(torch.equal(a, b[:, :8]) for a, b in zip(kept, cache))
