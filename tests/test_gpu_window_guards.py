@@ -165,6 +165,45 @@ def test_unseen_places_hold_anything(dtype, d, Nq, Nk, lo, window, sinks):
     O.close("y", y, O.attention(q, k, v, 4, window, sinks, 1 / math.sqrt(d), Nk, lo)["y"])
 
 
+# ---------------------------------------------------------------- views off the 16-byte grid
+def taken(call):
+    """Bytes that a call takes beyond its result"""
+    call()  # (whatever the first call of its kind takes)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    base = torch.cuda.memory_allocated()
+    y = call()
+    return torch.cuda.max_memory_allocated() - base - y.numel() * y.element_size()
+
+
+@pytest.mark.parametrize("dtype,d,extra", [(F32, 9, 0), (BF16, 20, 0), (BF16, 36, 0), (F32, 64, 1), (BF16, 64, 3), (BF16, 128, 2)])
+def test_decode_takes_no_copy_of_a_cache(dtype, d, extra):
+    """A slice of a longer cache, of an odd width or at an odd place of a joint cache, is read where it lies."""
+    B, S = 3, 5000
+    q, _, _, _ = make(d, B, 1, 1, 3, 1, d, dtype)
+    g = torch.Generator(device="cuda").manual_seed(d)
+    joint = torch.randn(B, S + 1, 2 * d + extra, generator=g, device="cuda").to(dtype)
+    k, v = joint[:, :S, extra : d + extra], joint[:, :S, d + extra :]
+    if not extra:
+        k, v = (t.contiguous()[:, :S] for t in (joint[..., :d], joint[..., d:]))
+    ctxlen = torch.tensor([S, 2000, 1], dtype=torch.int32, device="cuda")
+    call = lambda: ncn.window_attention_decode(q, k, v, ctxlen, 3, 100, n_sink=2)  # noqa: E731
+    O.close("y", call(), O.attention(q, k, v, 3, 100, 2, 1 / math.sqrt(d), ctxlen, ctxlen - 1)["y"])
+    assert taken(call) < 16384 < k.numel() * k.element_size()
+
+
+@pytest.mark.parametrize("dtype,d", [(F32, 9), (BF16, 20), (F32, 33)])
+def test_no_copy_where_it_would_not_help(dtype, d):
+    """Rows of an odd width have no 16-byte boundaries in a copy either."""
+    B, S = 2, 6000
+    cache = torch.randn(2, B, S + 1, d, device="cuda").to(dtype)
+    q, _, _, _ = make(d, B, 4, 1, 3, 1, d, dtype)
+    k, v = cache[0][:, :S], cache[1][:, :S]
+    call = lambda: ncn.fused_window_attention(q, k, v, 3, 100, n_sink=2)  # noqa: E731
+    O.close("y", call(), O.attention(q, k, v, 3, 100, 2, 1 / math.sqrt(d), S, S - 4)["y"])
+    assert taken(call) < 16384 < k.numel() * k.element_size()
+
+
 # ---------------------------------------------------------------- the layer
 @pytest.mark.parametrize("dtype", ["default", F32, BF16])
 def test_layer_under_autocast(dtype):
