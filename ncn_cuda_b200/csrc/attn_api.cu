@@ -82,9 +82,17 @@ void set_state(AttnParams& p, void* state, int dtype) {
   p.rest = state && dtype == NCN_BF16 ? reinterpret_cast<__nv_bfloat16*>(p.lse + delta_floats(p)) : nullptr;
 }
 
-bool grid_ok(const AttnParams& p) {
-  const long long tq = (p.Nq + 31) / 32, tk = (p.Nk + 31) / 32 + 64 * ((p.n_sink + 63) / 64);
-  return tq * p.H <= kMaxGrid / p.B && (tk > p.n_sink ? tk : p.n_sink) * p.Hk <= kMaxGrid / p.B && 8ll * p.Hk * p.G * p.Nq <= kMaxGrid / p.B;
+// Whether a launch's CTAs can be counted: one per 64 queries of a head at most (also in the backward); in the backward one per 64 keys of
+// a head and piece of the sinks' queries (after plan_sinks), and one per sink; in decode one per two of the rows that share keys, or per row
+// where there is one (several share them only where there are fewer of these than SMs).
+bool grid_fwd_ok(const AttnParams& p) { return (p.Nq + 63ll) / 64 * p.H <= kMaxGrid / p.B; }
+bool grid_bwd_ok(const AttnParams& p) {
+  const long long items = (p.Nk + 63ll) / 64 + (long long)p.sink_tiles * p.chunks;
+  return grid_fwd_ok(p) && items * p.Hk <= kMaxGrid / p.B && (p.chunks == 0 || (long long)p.n_sink * p.Hk <= kMaxGrid / p.B);
+}
+bool grid_decode_ok(const AttnParams& p) {
+  const long long rows = (long long)p.G * p.Nq;
+  return rows <= 1 << 30 && (rows + 1) / 2 * p.Hk <= kMaxGrid / p.B;
 }
 
 }  // namespace
@@ -107,7 +115,7 @@ int ncn_window_fwd(const void* q, const void* k, const void* v, void* y, void* s
   if (rc != NCN_OK || B == 0 || Nq == 0) return rc;
   if (!y) return NCN_ERR_NULL;
   if (!aligned16(state)) return NCN_ERR_ALIGN;
-  if (!grid_ok(p)) return NCN_ERR_TOO_LARGE;
+  if (!grid_fwd_ok(p)) return NCN_ERR_TOO_LARGE;
   DevInfo dev;
   if ((rc = get_dev(dev)) != NCN_OK) return rc;
   p.y = y, p.status = dev.status;
@@ -141,7 +149,6 @@ int ncn_window_bwd(const void* q, const void* k, const void* v, const void* y, c
   if (rc != NCN_OK || B == 0 || Nq == 0) return rc;
   if (!y || !dy || !state || !dq || ((!dk || !dv) && Nk > 0)) return NCN_ERR_NULL;
   if (!aligned16(state) || !aligned16(workspace)) return NCN_ERR_ALIGN;  // (read by bulk copies and 16 bytes at a time)
-  if (!grid_ok(p)) return NCN_ERR_TOO_LARGE;
   DevInfo dev;
   if ((rc = get_dev(dev)) != NCN_OK) return rc;
   p.y_in = y, p.dy = dy, p.dq = dq, p.dk = dk, p.dv = dv, p.status = dev.status;
@@ -150,6 +157,7 @@ int ncn_window_bwd(const void* q, const void* k, const void* v, const void* y, c
   int T, TQ;
   bwd_tiles(p, dtype, T, TQ);
   plan_sinks(p, T, TQ);
+  if (!grid_bwd_ok(p)) return NCN_ERR_TOO_LARGE;
   if (!workspace || workspace_bytes < (delta_floats(p) + part_floats(p)) * sizeof(float)) return NCN_ERR_WORKSPACE;
   p.delta = static_cast<float*>(workspace);
   p.part = p.delta + delta_floats(p);
@@ -163,7 +171,7 @@ int ncn_window_decode(const void* q, const void* k, const void* v, void* y, cons
   int rc = attn_params(p, q, k, v, ctxlen, nullptr, strides, 6, B, Nq, S, E, Ek, n_head, window, n_sink, 0, scale, dtype);
   if (rc != NCN_OK || B == 0 || Nq == 0) return rc;
   if (!y || !ctxlen) return NCN_ERR_NULL;
-  if (!grid_ok(p)) return NCN_ERR_TOO_LARGE;
+  if (!grid_decode_ok(p)) return NCN_ERR_TOO_LARGE;
   DevInfo dev;
   if ((rc = get_dev(dev)) != NCN_OK) return rc;
   p.y = y, p.start_at_end = 1;

@@ -1181,7 +1181,7 @@ const char* ncn_status_string(int s) {
     case NCN_ERR_CUDA: return "CUDA runtime error";
     case NCN_ERR_NULL: return "null pointer";
     case NCN_ERR_DEVICE_WAIT: return "a kernel abandoned a bounded wait on an asynchronous copy";
-    case NCN_ERR_TOO_LARGE: return "problem needs more scratch than the fixed array of ncn_net_bwd_noalloc holds";
+    case NCN_ERR_TOO_LARGE: return "problem needs more scratch than the fixed array of ncn_net_bwd_noalloc holds, or more CTAs than a launch has";
     default: return "unknown status";
   }
 }

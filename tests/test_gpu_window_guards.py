@@ -240,3 +240,24 @@ def test_layer_beyond_its_cache():
         got = layer.step(x[:, 8 : 8 + n], cache, torch.tensor([8 + n, 8 + n]))
         assert (got == 0).all(), n
     assert all(torch.equal(a, b[:, :8]) for a, b in zip(kept, cache))
+
+
+# ---------------------------------------------------------------- many rows
+def test_more_queries_than_decode_takes():
+    """Forward and backward have a CTA per tile of queries, and are not bound by what the form for single tokens would launch."""
+    H, d, Nq, Nk = 128, 8, 1 << 21, 64
+    if torch.cuda.mem_get_info()[0] < 48 << 30:
+        pytest.skip("needs 48 GB")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v, first, dy = (torch.randn(1, Nk, n * d, generator=g, device="cuda").to(BF16) for n in (1, 1, H, H))
+    wide = lambda t: torch.cat([t, t.new_zeros(1, Nq - Nk, H * d)], 1)  # noqa: E731
+    leaves = [t.requires_grad_(True) for t in (wide(first), k, v)]
+    y = ncn.fused_window_attention(*leaves, H, 9, q_start=0)
+    want = O.attention(first, k, v, H, 9, 0, 1 / math.sqrt(d), Nk, 0, dy)
+    O.close("y", y.detach()[:, :Nk], want["y"])
+    assert not y[:, Nk:].any()
+    dq, dk, dv = torch.autograd.grad(y, leaves, wide(dy))
+    O.close("dq", dq[:, :Nk], want["dq"])
+    assert not dq[:, Nk:].any()
+    O.close("dk", dk, want["dk"])
+    O.close("dv", dv, want["dv"])

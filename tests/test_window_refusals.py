@@ -56,6 +56,8 @@ def test_decode_refuses():
     assert decode(H=5) == SHAPE
     assert decode(dtype=7) == DTYPE
     assert decode(B=0) == OK
+    assert _lib.load().ncn_window_decode(P, P, P, P, P, None, 1 << 30, 1, 8, 64, 64, 2, 4, 0, 1.0, 1, None) == 10  # two heads of 2^30 rows
+    assert _lib.load().ncn_window_decode(P, P, P, P, P, None, 1, 1 << 28, 8, 512, 64, 8, 4, 0, 1.0, 1, None) == 10  # 2^31 rows share keys
 
 
 @pytest.mark.parametrize("status,args", [
