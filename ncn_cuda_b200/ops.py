@@ -410,8 +410,10 @@ def window_decode(q, k, v, ctxlen, n_head, window, n_sink, scale):
     return y
 
 
-def _rotary_args(q, k, freqs, positions, n_head):
+def _rotary_args(q, k, wq, wk, freqs, positions, n_head):
     _check_inputs(q)
+    if k is not None and (wq is None) != (wk is None):
+        raise ValueError("both weights or none")
     B, N, E = q.shape
     if k is not None and (k.dim() != 3 or k.shape[:2] != q.shape[:2] or k.dtype != q.dtype or k.device != q.device):
         raise ValueError("q and k must agree in batch size, positions, dtype and device")
@@ -422,6 +424,8 @@ def _rotary_args(q, k, freqs, positions, n_head):
     freqs = freqs.detach().to(device=q.device, dtype=torch.float64).contiguous()
     stride = 0
     if positions is not None:
+        if positions.is_floating_point() or positions.is_complex() or positions.dtype == torch.bool:
+            raise TypeError("positions are whole numbers")
         shared = positions.dim() == 1 or (positions.dim() == 2 and positions.shape[0] == 1)
         if positions.dim() not in (1, 2) or positions.shape[-1] != N or (not shared and positions.shape[0] != B):
             raise ValueError("positions must be [N] or [B, N] for tensors [B, N, E]")
@@ -433,7 +437,7 @@ def _rotary_args(q, k, freqs, positions, n_head):
 def qk_rotary(q, k, wq, wk, freqs, positions, n_head, start, interleaved, eps, magnitude, inverse=False):
     """Returns (q', k'): with weights the heads are normalised first."""
     lib = _lib.load()
-    freqs, positions, pos_stride = _rotary_args(q, k, freqs, positions, n_head)
+    freqs, positions, pos_stride = _rotary_args(q, k, wq, wk, freqs, positions, n_head)
     B, N, E = q.shape
     ts, strides = _strided(*(t for t in (q, k) if t is not None))
     q, k = ts[0], ts[1] if len(ts) > 1 else None
@@ -457,7 +461,7 @@ def qk_rotary(q, k, wq, wk, freqs, positions, n_head, start, interleaved, eps, m
 def qk_norm_rotary_bwd(q, k, wq, wk, freqs, positions, dyq, dyk, n_head, start, interleaved, eps, magnitude):
     """Returns (dq, dk, dwq, dwk); the weights' gradients are fp32 [E / n_head]."""
     lib = _lib.load()
-    freqs, positions, pos_stride = _rotary_args(q, k, freqs, positions, n_head)
+    freqs, positions, pos_stride = _rotary_args(q, k, wq, wk, freqs, positions, n_head)
     (B, N, E), d = q.shape, q.shape[2] // n_head
     wq = _weights(wq, d, q.device)
     dwq = torch.zeros(d, dtype=torch.float32, device=q.device)

@@ -74,6 +74,16 @@ def test_transforms_are_refused(kind):
         call(*args)
 
 
+def test_the_function_form_refuses_what_the_node_refuses():
+    q, k, _, _ = make(1, 2, 8, 8, 2, 1, 32, F32)
+    freqs, _ = ncn.rotary_frequencies(32, device="cuda")
+    apply = torch.autograd.Function.apply.__func__
+    with pytest.raises(TypeError, match="whole numbers"):
+        apply(ncn.RotaryFunction, q, k, None, None, freqs, torch.arange(8).float(), 2, 0, False, 0.0, 1.0)
+    with pytest.raises(ValueError, match="weights"):
+        apply(ncn.RotaryFunction, q, k, torch.ones(32, device="cuda"), None, freqs, None, 2, 0, False, 0.0, 1.0)
+
+
 def test_function_form_of_decode_agrees():
     for dtype, d in ((BF16, 64), (F32, 40), (BF16, 20)):
         q, k, v, _ = make(9, 3, 2, 130, 4, 1, d, dtype)
