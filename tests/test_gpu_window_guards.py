@@ -1,6 +1,7 @@
 """Attention operators at the edges of what they take: traced and transformed calls, scores that overflow, places that nobody sees, views
 off the 16-byte grid, mixed precision, many rows."""
 import math
+import re
 
 import pytest
 import torch
@@ -8,6 +9,7 @@ import torch
 import ncn_cuda_b200 as ncn
 from ncn_cuda_b200 import ops
 from tests import window_oracle as O
+from tests.kernels_util import kernels_of, launched
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -271,3 +273,36 @@ def test_more_queries_than_decode_takes():
     assert not dq[:, Nk:].any()
     O.close("dk", dk, want["dk"])
     O.close("dv", dv, want["dv"])
+
+
+# ---------------------------------------------------------------- kernels by name
+@pytest.mark.parametrize("kind,dtype,d,wanted", [
+    ("train", F32, 64, ("attn_split_fwd_kernel<64", "attn_split_dq_kernel<64", "attn_split_dkv_kernel<64", "attn_sink_sum_kernel<float")),
+    ("train", BF16, 64, ("attn_tensor_fwd_kernel<64", "attn_tensor_dq_kernel<64", "attn_tensor_dkv_kernel<64")),
+    ("train", BF16, 160, ("attn_simt_fwd_kernel", "attn_simt_dq_kernel", "attn_simt_dkv_kernel")),
+    ("decode", BF16, 128, ("attn_decode_kernel<128, 1>",)), ("decode", BF16, 64, ("attn_decode_kernel<64, 1>",)), ("decode", F32, 64, ("attn_decode_any_kernel<float",)),
+    ("norm", BF16, 128, ("rotary_kernel<__nv_bfloat16, 8, 1>", "rotary_kernel<__nv_bfloat16, 8, 2>")), ("norm", F32, 96, ("rotary_kernel<float, 8, 1>", "rotary_kernel<float, 8, 2>")),
+    ("turn", BF16, 64, ("rotary_kernel<__nv_bfloat16, 4, 0>",)), ("turn", F32, 40, ("rotary_any_kernel<float",)),
+])
+def test_the_kernels_are_reached(kind, dtype, d, wanted):
+    q, k, v, dy = make(1, 2, 200, 200, 4, 2, d, dtype)
+    freqs, _ = ncn.rotary_frequencies(d, device="cuda")
+    lengths = torch.tensor([200, 90], dtype=torch.int32, device="cuda")
+    w = torch.ones(d, device="cuda", requires_grad=True)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+
+    def call():
+        if kind == "train":
+            return torch.autograd.grad(ncn.fused_window_attention(*leaves, 4, 50, n_sink=2), leaves, dy)
+        if kind == "decode":
+            with torch.no_grad():
+                return ncn.window_attention_decode(q[:, :1], k, v, lengths, 4, 50, n_sink=2)
+        if kind == "norm":
+            y = ncn.fused_qk_norm_rotary(q, k, w, w, freqs, 4)
+        else:
+            y = ncn.fused_rotary(q, k, freqs, 4)
+        return torch.autograd.grad(y, leaves[:2], (dy, dy[..., : k.shape[2]]))
+
+    _, names = kernels_of(call)
+    for part in wanted:
+        assert launched(names, re.escape(part)), (part, sorted(names))
