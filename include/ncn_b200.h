@@ -226,7 +226,7 @@ size_t ncn_ckpt_bytes(int64_t B, int64_t N, int64_t E, int L, int ckpt_every, in
  * A query that sees keys, all of whose scores are minus infinity (products that overflow), gives NaN, as the formula does.
  * A query that sees nothing (padding behind ctx_b, a position below zero) gives zeros and no gradient; what q and dy hold in such
  * places, and k and v in places that no query of the row sees (behind ctx_b, behind the last query, in front of the window), is not used, NaN included.  (Keys that one query sees and a neighbour does not may share a tile: a NaN or infinity in such a
- * key's v reaches, in the forward and backward, queries up to 256 positions from those that see it.)  ctxlen (int32 [B] on the device) null: Nk.
+ * key's v reaches, in the forward, in the backward and in decode of several positions, queries up to 256 positions from those that see it.)  ctxlen (int32 [B] on the device) null: Nk.
  * q_start (int32 [B] on the device) null: start for every row.  window >= 1, n_sink >= 0, scale > 0.  Nq and Nk up to 2^28; a launch has a CTA per
  * 64 queries of a head of each row (backward: and per 64 keys, and per sink), and NCN_ERR_TOO_LARGE is the answer to more than 2^31 - 1. */
 

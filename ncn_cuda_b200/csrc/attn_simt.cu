@@ -8,8 +8,9 @@
 //
 // What bounds it: the reads of shared memory.  A product over 4 features takes a thread 8 reads of 16 bytes, which return to a
 // warp in 32 cycles, for 64 FMAs, which take 16: half the FMA rate (36 of 72 TFLOP/s) is the most this split can give.  Measured:
-// fp32, heads of 128, 2 x 4096 positions of 8 heads, windows of 1024, forward 928 us (32.4 TFLOP/s), dq 1332 (33.9), dk and dv
-// 1761 (34.2); bf16, heads of 256, 2 x 2048 positions, windows of 512: 556, 833, 1031 us (27 to 29).  Tiles of 8 rows a thread would
+// heads of 256, 2 x 2048 positions of 8 heads, windows of 512: fp32 forward 568 us (26.5 TFLOP/s), dq 847 (26.6), dk and dv 1076 (28.0), bf16
+// 571, 846, 1046; fp32 heads of 16, 2 x 4096 positions of 8 heads, windows of 1024: 281, 374, 521 us (13 to 15 TFLOP/s: half of a tile's
+// features are zeros); bf16 heads of 12, the same: 321, 433, 562.  Tiles of 8 rows a thread would
 // lower the reads by a quarter, but with large heads the backward's four tiles then no longer fit in shared memory.
 #include "attn_common.cuh"
 #include "ncn_common.cuh"

@@ -13,7 +13,8 @@
 // a pair is worked on, the other's successor is on its way (cp.async).
 //
 // Measured, 2 x 4096 positions of 8 heads, windows of 1024: heads of 128 forward 616 us (48.8 TFLOP/s), dq 949 (47.5), dk and dv 1262
-// (47.7); heads of 80 401, 634, 828 (in tiles of 96 features 472, 733, 983); heads of 64 317, 462, 624 (48); on the FMA pipes 928, 1332, 1761 and 453, 649, 862.  The matrix unit is 50 to 56 % busy (three
+// (47.7); heads of 80 401, 634, 828 (in tiles of 96 features 472, 733, 983); heads of 64 317, 462, 624 (48); as fp32 products on the FMA pipes
+// (attn_simt.cu, when it had tiles of these sizes) 928, 1332, 1761 and 453, 649, 862.  The matrix unit is 50 to 56 % busy (three
 // products: 275 TFLOP/s of tf32 would be 92 here); more CTAs, smaller tiles and more independent accumulators change nothing.
 #include "attn_common.cuh"
 #include "ncn_common.cuh"

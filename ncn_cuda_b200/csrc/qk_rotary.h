@@ -18,7 +18,7 @@ struct RotaryParams {
   const double* freqs;      // [R / 2], radians per position
   const long long* pos;     // positions, [N] or [B, N], or null: start, start + 1, ...
   long long pos_b, start;   // stride of a row of positions (0: the same for all)
-  float* partial;           // backward of the norm: [grid][2][d]
+  float* partial;           // backward of the norm: [2][grid][d]
   int B, N, d, R;
   int interleaved, backward, vec;
   int span, parts;          // positions that a CTA takes at a time, CTAs that share their heads
