@@ -274,7 +274,9 @@ class NCNWindowAttention(nn.Module):
         (The place behind them takes what has none.)"""
         w = self.qkv.weight
         if dtype is None:
-            dtype = torch.get_autocast_dtype(w.device.type) if torch.is_autocast_enabled(w.device.type) else w.dtype
+            kind = w.device.type
+            cast = torch.amp.is_autocast_available(kind) and torch.is_autocast_enabled(kind)
+            dtype = torch.get_autocast_dtype(kind) if cast else w.dtype
         width = self.n_kv_head * (self.embed_dim // self.n_head)
         return tuple(torch.zeros(B, length + 1, width, dtype=dtype, device=w.device) for _ in range(2))
 

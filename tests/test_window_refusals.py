@@ -151,3 +151,5 @@ def test_types_of_a_cache():
     with torch.autocast("cpu", torch.bfloat16):
         assert [t.dtype for t in layer.new_cache(2, 5)] == [torch.bfloat16] * 2
         assert layer.new_cache(2, 5, dtype=torch.float32)[0].dtype == torch.float32
+    cache = ncn.NCNWindowAttention(64, 4, 8).to("meta").new_cache(2, 5)  # (a device without autocast)
+    assert cache[0].is_meta and cache[0].dtype == torch.float32
