@@ -194,7 +194,7 @@ std::optional<Tensor> py_window(const Tensor& q, const Tensor& k, const Tensor& 
 
 std::optional<Tensor> py_decode(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& ctxlen, int64_t n_head, int64_t window,
                                 int64_t n_sink, double scale) {
-  if (needs_function({&q, &k, &v})) return std::nullopt;
+  if (needs_function({&q, &k, &v}) || wants_grad({&q, &k, &v})) return std::nullopt;  // (the Function's backward is an error)
   check_tensors("q and the caches of keys and values", q, {&k, &v});
   if (k.sizes() != v.sizes()) throw py::value_error("k and v must agree in shape");
   head_size(q, k, n_head);

@@ -93,6 +93,9 @@ def test_function_form_of_decode_agrees():
         a = ncn.WindowDecodeFunction.apply(q, k, v, *args)
         b = torch.autograd.Function.apply.__func__(ncn.WindowDecodeFunction, q, k, v, *args)
         assert torch.equal(a, b)
+    y = ncn.WindowDecodeFunction.apply(q.requires_grad_(True), k, v, *args)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        y.sum().backward()
     with pytest.raises(TypeError, match="whole numbers"):
         ops.window_decode(q, k, v, torch.tensor([1.0, 2.0, 3.0]), 4, 20, 3, 0.125)
     with pytest.raises(ValueError, match="ctxlen has 2"):
